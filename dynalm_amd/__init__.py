@@ -19,6 +19,9 @@ dynacore/include/dynacore/device/device.h:89-161):
     matmul_many(jobs)                  Device::matmul_many
     act_mul(act, gate, up, ...)        Device::act_mul
     matmul_gated(act, x, wg, wu, ...)  Device::matmul_gated
+    qk_norm_rope(...)              head norms and rotation (Device::rms_norm, rope)
+    kv_append(cache, ...)          keys and values into a paged cache (Device::kv_store)
+    shared_attention(cache, ...)   attention over a shared prefix and own pages
     GgufFile.open(path)                dynalm's GgufFile::open / open_parts (host mmap + parse)
     GgufFile.upload(name)              Device::upload of a GGUF tensor
 
@@ -37,6 +40,8 @@ __all__ = [
     "DqError", "lib", "lib_path", "row_bytes", "act_row_bytes", "act_format_for", "Weight",
     "act_quantize", "gemv", "gemm", "matmul", "matmul_many", "MatmulJob", "partials_count", "debug_partials",
     "SILU", "GELU", "GELU_TANH", "act_mul", "matmul_gated", "GgufFile", "GgufTensor", "EXPORTS",
+    "F32", "F16", "BF16", "ROPE_HALVES", "ROPE_PAIRS", "MAX_HEAD_DIM", "Heads", "Rope", "KvCache", "Attention", "qk_norm_rope",
+    "kv_append", "shared_attention", "shared_attention_workspace", "ATTENTION_WORKSPACE_BYTES",
     "MatmulShape", "External", "matmul_noalloc", "NOALLOC_SCRATCH_BYTES", "Plan", "Selection",
     "plan_defaults", "plan_ffn_down", "select", "matmul_plan", "KERNEL_NAMES", "KERNEL_QMM_GEMM", "KERNEL_QMM_GEMV",
 ]
@@ -118,6 +123,10 @@ EXPORTS = {
     "dq_plan_defaults": (_I, [_P]),
     "dq_plan_ffn_down": (_I, [_P, _P]),
     "dq_select": (_I, [_P, _P, _P]),
+    "dq_qk_norm_rope": (_I, [_I64, _I64, _P, _P, _P, _P, _P, _P, C.c_float, _P, _P, _P]),
+    "dq_kv_append": (_I, [_P, _I64, _P, _P, _P, _P, C.c_float, _P, _P, _P]),
+    "dq_shared_attention_workspace": (_I64, [_P, _P]),
+    "dq_shared_attention": (_I, [_P, _P, _P, _I64, _P]),
     "dq_matmul_plan": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P]),
 }
 
@@ -318,6 +327,82 @@ def partials_count(dtype: int, fmt: int, k: int) -> tuple[int, int]:
 
 def debug_partials(w: Weight, fmt: int, acts, m: int, units, sb=None, stream: int = 0) -> None:
     _check(lib().dq_debug_partials(w.handle, fmt, _ptr(acts), m, _ptr(units), _ptr(sb), stream))
+
+
+# ---------------------------------------------------------------- attention block
+
+F32, F16, BF16 = 0, 1, 2  # dq_float
+ROPE_HALVES, ROPE_PAIRS = 0, 1  # dq_rope_style
+MAX_HEAD_DIM = 256
+ATTENTION_WORKSPACE_BYTES = 128 << 20  # DQ_ATTENTION_WORKSPACE_BYTES
+
+
+class Heads(C.Structure):
+    """dq_heads: rows of heads, Heads(pointer, dtype, heads, token_stride, head_stride)."""
+    _fields_ = [("p", _P), ("dtype", C.c_int32), ("heads", C.c_int32), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+class Rope(C.Structure):
+    """dq_rope: cosine and sine tables, Rope(cos, sin, max_pos, rot_dim, style)."""
+    _fields_ = [("cos", _P), ("sin", _P), ("max_pos", _I64), ("rot_dim", C.c_int32), ("style", C.c_int32)]
+
+
+class KvCache(C.Structure):
+    """dq_kv_cache: a layer's pages of keys and values in the caller's memory."""
+    _fields_ = [("k", _P), ("v", _P), ("dtype", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_size", C.c_int32), ("n_pages", _I64), ("page_stride", _I64), ("token_stride", _I64),
+                ("head_stride", _I64)]
+
+
+class Attention(C.Structure):
+    """dq_attention: one shared_attention call."""
+    _fields_ = [("q", C.POINTER(Heads)), ("out", C.POINTER(Heads)), ("lse", _P), ("tokens", _I64), ("batch", _I64),
+                ("q_offsets", _P), ("max_q", _I64), ("prefix_pages", _P), ("prefix_len", _I64), ("pages", _P),
+                ("pages_stride", _I64), ("lens", _P), ("max_len", _I64), ("scale", C.c_float)]
+
+
+def _ref(s):
+    return C.addressof(s) if s is not None else None
+
+
+def qk_norm_rope(tokens: int, head_dim: int, q: Heads, q_out: Heads, q_weight=None, k: Heads | None = None,
+                 k_out: Heads | None = None, k_weight=None, eps: float = 0.0, rope: Rope | None = None, positions=None,
+                 stream: int = 0) -> None:
+    """q_out = rope(norm(q)), k_out = rope(norm(k)) for each head (dq_qk_norm_rope)."""
+    _check(lib().dq_qk_norm_rope(tokens, head_dim, _ref(q), _ref(q_out), _ptr(q_weight), _ref(k), _ref(k_out),
+                                 _ptr(k_weight), eps, _ref(rope), _ptr(positions), stream))
+
+
+def kv_append(cache: KvCache, tokens: int, k: Heads, v: Heads, slots, k_weight=None, eps: float = 0.0,
+              rope: Rope | None = None, positions=None, stream: int = 0) -> None:
+    """rope(norm(k)) and v into the cache's slots (dq_kv_append)."""
+    _check(lib().dq_kv_append(_ref(cache), tokens, _ref(k), _ref(v), _ptr(slots), _ptr(k_weight), eps, _ref(rope),
+                              _ptr(positions), stream))
+
+
+def _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
+               max_len, scale) -> Attention:
+    return Attention(C.pointer(q) if q is not None else None, C.pointer(out) if out is not None else None, _ptr(lse), tokens, batch, _ptr(q_offsets), max_q, _ptr(prefix_pages),
+                     prefix_len, _ptr(pages), pages_stride, _ptr(lens), max_len, scale)
+
+
+def shared_attention_workspace(cache: KvCache, q: Heads, out: Heads, tokens: int, batch: int, max_q: int,
+                               prefix_len: int, pages_stride: int, max_len: int, scale: float = 1.0) -> int:
+    """Workspace bytes of a shared_attention call of this shape (no GPU needed)."""
+    a = _attention(q, out, None, tokens, batch, None, max_q, None, prefix_len, None, pages_stride, None, max_len, scale)
+    n = lib().dq_shared_attention_workspace(_ref(cache), C.addressof(a))
+    if n < 0:
+        raise DqError(1, lib().dq_last_error().decode(errors="replace"))
+    return int(n)
+
+
+def shared_attention(cache: KvCache, q: Heads, out: Heads, lse, tokens: int, batch: int, q_offsets, max_q: int,
+                     prefix_pages, prefix_len: int, pages, pages_stride: int, lens, max_len: int, scale: float,
+                     workspace, workspace_bytes: int, stream: int = 0) -> None:
+    """out = attention of q over the shared prefix and each sequence's own keys (dq_shared_attention)."""
+    a = _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
+                   max_len, scale)
+    _check(lib().dq_shared_attention(_ref(cache), C.addressof(a), _ptr(workspace), workspace_bytes, stream))
 
 
 # ------------------------------------------------------------------ GGUF files

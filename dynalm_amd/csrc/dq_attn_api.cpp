@@ -1,0 +1,263 @@
+// dq_attn_api.cpp -- the attention block's C ABI (declared in include/dynaq.h): argument
+// checks with dynacore's status codes, then the launches. Nothing is allocated or kept.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "../../include/dynaq.h"
+#include "dq_attn.h"
+#include "dq_internal.h"
+
+namespace {
+
+typedef long long ll;
+
+int bad(const char* what) { return dq::set_error(DQ_INVALID_ARGUMENT, "%s", what); }
+
+int hip_fail(hipError_t e, const char* what) {
+  return dq::set_error(e == hipErrorOutOfMemory ? DQ_OUT_OF_MEMORY : DQ_INTERNAL, "%s: %s", what, hipGetErrorString(e));
+}
+
+bool float_ok(int t) { return t == DQ_F32 || t == DQ_F16 || t == DQ_BF16; }
+size_t float_bytes(int t) { return t == DQ_F32 ? 4 : 2; }
+
+int check_dim(int64_t dim) {
+  if (dim <= 0 || dim % 8 != 0) return dq::set_error(DQ_INVALID_ARGUMENT, "head_dim %lld is not a multiple of 8", (ll)dim);
+  if (dim > DQ_MAX_HEAD_DIM) return dq::set_error(DQ_UNSUPPORTED, "head_dim %lld is over %d", (ll)dim, DQ_MAX_HEAD_DIM);
+  return DQ_OK;
+}
+
+// What can be said of rows without their data: `need` heads (0: any), values addressable by int64.
+int check_rows(const char* name, const dq_heads* r, int64_t tokens) {
+  if (r == nullptr) return dq::set_error(DQ_INVALID_ARGUMENT, "%s: null argument", name);
+  if (!float_ok(r->dtype)) return dq::set_error(DQ_UNSUPPORTED, "%s: type %d is not supported", name, r->dtype);
+  if (r->heads <= 0) return dq::set_error(DQ_INVALID_ARGUMENT, "%s: heads must be positive", name);
+  if (r->token_stride < 0 || r->head_stride < 0) return dq::set_error(DQ_INVALID_ARGUMENT, "%s: negative stride", name);
+  const int64_t most = (int64_t)1 << 58;
+  if ((tokens > 1 && r->token_stride > most / tokens) || (r->heads > 1 && r->head_stride > most / r->heads))
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%s: strides too large", name);
+  return DQ_OK;
+}
+
+int check_data(const char* name, const dq_heads* r) {
+  if (r->p == nullptr) return dq::set_error(DQ_INVALID_ARGUMENT, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(r->p) % float_bytes(r->dtype) != 0)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%s: misaligned pointer", name);
+  return DQ_OK;
+}
+
+// An output's rows must not run into each other.
+int check_apart(const char* name, const dq_heads* r, int64_t tokens, int64_t dim) {
+  const int64_t th = r->head_stride, tt = r->token_stride, nh = r->heads;
+  if (nh > 1 && th < dim) return dq::set_error(DQ_INVALID_ARGUMENT, "%s: head_stride %lld < head_dim %lld", name, (ll)th, (ll)dim);
+  if (tokens > 1 && tt < dim)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%s: token_stride %lld < head_dim %lld", name, (ll)tt, (ll)dim);
+  if (tokens > 1 && nh > 1 && tt < (nh - 1) * th + dim && th < (tokens - 1) * tt + dim)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%s: tokens and heads overlap (strides %lld, %lld)", name, (ll)tt, (ll)th);
+  return DQ_OK;
+}
+
+int check_rope(const dq_rope* r, const int32_t* positions, int64_t dim, int64_t tokens, dq::RopeArgs* out) {
+  if (r == nullptr) return DQ_OK;
+  if (r->style != DQ_ROPE_HALVES && r->style != DQ_ROPE_PAIRS)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "unknown rotation style %d", r->style);
+  if (r->rot_dim < 2 || r->rot_dim % 2 != 0 || r->rot_dim > dim)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "rot_dim %d is not even and in 2..head_dim %lld", r->rot_dim, (ll)dim);
+  if (r->max_pos < 0) return bad("max_pos must be >= 0");
+  if (tokens > 0 && (positions == nullptr || ((r->cos == nullptr || r->sin == nullptr) && r->max_pos > 0)))
+    return bad("rotation: null argument");
+  *out = dq::RopeArgs{r->cos, r->sin, positions, r->max_pos, r->rot_dim / 2, r->style == DQ_ROPE_PAIRS};
+  return DQ_OK;
+}
+
+int check_eps(const float* weight, float eps) {
+  if (weight != nullptr && !(eps >= 0 && std::isfinite(eps))) return bad("eps must be finite and >= 0");
+  return DQ_OK;
+}
+
+int check_cache(const dq_kv_cache* c, bool data) {
+  if (c == nullptr) return bad("cache: null argument");
+  if (c->dtype != DQ_F16 && c->dtype != DQ_BF16) return dq::set_error(DQ_UNSUPPORTED, "cache: type %d is not supported", c->dtype);
+  if (int rc = check_dim(c->head_dim); rc != DQ_OK) return rc;
+  if (c->kv_heads <= 0) return bad("cache: kv_heads must be positive");
+  if (c->page_size <= 0 || c->page_size % 16 != 0)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "cache: page_size %d is not a multiple of 16", c->page_size);
+  if (c->n_pages < 0 || c->n_pages > INT32_MAX) return dq::set_error(DQ_INVALID_ARGUMENT, "cache: n_pages %lld", (ll)c->n_pages);
+  for (int64_t st : {c->page_stride, c->token_stride, c->head_stride})
+    if (st < 0 || st % 8 != 0 || st > ((int64_t)1 << 58) / (st == c->page_stride ? c->n_pages + 1 : c->page_size + c->kv_heads))
+      return dq::set_error(DQ_INVALID_ARGUMENT, "cache: stride %lld is negative, no multiple of 8 or too large", (ll)st);
+  if (c->token_stride < c->head_dim || (c->kv_heads > 1 && c->head_stride < c->head_dim) || (c->n_pages > 1 && c->page_stride < c->head_dim))
+    return bad("cache: a stride is less than head_dim");
+  if (data && c->n_pages > 0) {
+    if (c->k == nullptr || c->v == nullptr) return bad("cache: null pointer");
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0) return bad("cache: k and v must be 16-byte aligned");
+  }
+  return DQ_OK;
+}
+
+dq::CacheArgs cache_args(const dq_kv_cache* c) {
+  return dq::CacheArgs{static_cast<uint16_t*>(c->k), static_cast<uint16_t*>(c->v), c->n_pages, c->page_stride,
+                       c->token_stride, c->head_stride, c->page_size, c->kv_heads};
+}
+
+dq::HeadRows rows(const dq_heads* in, const dq_heads* out, const float* w) {
+  dq::HeadRows r;
+  r.in = in->p;
+  r.weight = w;
+  r.heads = in->heads;
+  r.in_token = in->token_stride;
+  r.in_head = in->head_stride;
+  if (out != nullptr) {
+    r.out = out->p;
+    r.out_token = out->token_stride;
+    r.out_head = out->head_stride;
+  }
+  return r;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int64_t kMaxRows = (int64_t)1 << 31;  // head rows of a launch (a grid's workgroups)
+
+int check_tokens(int64_t tokens, int64_t heads) {
+  if (tokens < 0) return bad("tokens must be >= 0");
+  if (tokens > kMaxRows / heads) return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %lld heads are too many", (ll)tokens, (ll)heads);
+  return DQ_OK;
+}
+
+int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
+  if (a == nullptr) return bad("null argument");
+  if (int rc = check_cache(c, data); rc != DQ_OK) return rc;
+  if (a->tokens < 0 || a->batch < 0) return bad("tokens and batch must be >= 0");
+  if (int rc = check_rows("q", a->q, a->tokens); rc != DQ_OK) return rc;
+  if (int rc = check_rows("out", a->out, a->tokens); rc != DQ_OK) return rc;
+  if (int rc = check_apart("out", a->out, a->tokens, c->head_dim); rc != DQ_OK) return rc;
+  if (a->q->dtype != a->out->dtype || (a->q->dtype != DQ_F32 && a->q->dtype != c->dtype))
+    return dq::set_error(DQ_UNSUPPORTED, "q type %d, out type %d with cache type %d: q and out have the cache's type or fp32",
+                         a->q->dtype, a->out->dtype, c->dtype);
+  if (a->q->heads != a->out->heads || a->q->heads % c->kv_heads != 0)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%d query heads, %d of out, %d kv heads", a->q->heads, a->out->heads, c->kv_heads);
+  if (int rc = check_tokens(a->tokens, a->q->heads); rc != DQ_OK) return rc;
+  if (a->batch > INT32_MAX - 1 || a->tokens > INT32_MAX / 2) return dq::set_error(DQ_UNSUPPORTED, "batch %lld, tokens %lld", (ll)a->batch, (ll)a->tokens);
+  if (a->max_q < 1 || a->max_q > INT32_MAX / 2) return dq::set_error(DQ_INVALID_ARGUMENT, "max_q %lld", (ll)a->max_q);
+  if (data && a->q_offsets == nullptr && (a->tokens != a->batch || a->max_q != 1))
+    return bad("without q_offsets every sequence has one token");
+  const int64_t most = (int64_t)1 << 30;
+  if (a->prefix_len < 0 || a->prefix_len > most || a->max_len < 0 || a->max_len > most)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "prefix_len %lld, max_len %lld", (ll)a->prefix_len, (ll)a->max_len);
+  if (a->pages_stride < (a->max_len + c->page_size - 1) / c->page_size || a->pages_stride > most)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "pages_stride %lld: max_len %lld needs %lld pages", (ll)a->pages_stride, (ll)a->max_len,
+                         (ll)((a->max_len + c->page_size - 1) / c->page_size));
+  if (!(a->scale > 0) || !std::isfinite(a->scale * kLog2e)) return bad("scale must be positive and finite");
+  return DQ_OK;
+}
+
+dq::AttnArgs attn_args(const dq_kv_cache* c, const dq_attention* a) {
+  dq::AttnArgs r;
+  r.cache = cache_args(c);
+  r.q = a->q->p;
+  r.out = a->out->p;
+  r.lse = a->lse;
+  r.q_token = a->q->token_stride;
+  r.q_head = a->q->head_stride;
+  r.out_token = a->out->token_stride;
+  r.out_head = a->out->head_stride;
+  r.heads = a->q->heads;
+  r.group = a->q->heads / c->kv_heads;
+  r.dim = c->head_dim;
+  r.tokens = (int32_t)a->tokens;
+  r.batch = (int32_t)a->batch;
+  r.max_q = (int32_t)a->max_q;
+  r.q_offsets = a->q_offsets;
+  r.prefix_pages = a->prefix_pages;
+  r.pages = a->pages;
+  r.lens = a->lens;
+  r.pages_stride = a->pages_stride;
+  r.prefix_len = (int32_t)a->prefix_len;
+  r.max_len = (int32_t)a->max_len;
+  r.scale_log2 = a->scale * kLog2e;
+  return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dq_qk_norm_rope(int64_t tokens, int64_t head_dim, const dq_heads* q, const dq_heads* q_out, const float* q_weight,
+                    const dq_heads* k, const dq_heads* k_out, const float* k_weight, float eps, const dq_rope* rope,
+                    const int32_t* positions, void* stream) {
+  if (int rc = check_dim(head_dim); rc != DQ_OK) return rc;
+  if ((k == nullptr) != (k_out == nullptr)) return bad("k and k_out go together");
+  const int sides = k != nullptr ? 2 : 1;
+  const dq_heads* const in[2] = {q, k};
+  const dq_heads* const out[2] = {q_out, k_out};
+  const char* const in_name[2] = {"q", "k"};
+  const char* const out_name[2] = {"q_out", "k_out"};
+  int64_t heads = 0;
+  for (int i = 0; i < sides; ++i) {
+    if (int rc = check_rows(in_name[i], in[i], tokens); rc != DQ_OK) return rc;
+    if (int rc = check_rows(out_name[i], out[i], tokens); rc != DQ_OK) return rc;
+    if (int rc = check_apart(out_name[i], out[i], tokens, head_dim); rc != DQ_OK) return rc;
+    if (in[i]->heads != out[i]->heads)
+      return dq::set_error(DQ_INVALID_ARGUMENT, "%s: %d heads into %d", in_name[i], in[i]->heads, out[i]->heads);
+    if (in[i]->dtype != q->dtype || out[i]->dtype != q_out->dtype)
+      return dq::set_error(DQ_UNSUPPORTED, "q and k differ in type");
+    heads += in[i]->heads;
+  }
+  if (int rc = check_tokens(tokens, heads); rc != DQ_OK) return rc;
+  if (int rc = check_eps(q_weight != nullptr ? q_weight : k_weight, eps); rc != DQ_OK) return rc;
+  dq::RopeArgs ra;
+  if (int rc = check_rope(rope, positions, head_dim, tokens, &ra); rc != DQ_OK) return rc;
+  if (tokens == 0) return DQ_OK;
+  for (int i = 0; i < sides; ++i) {
+    if (int rc = check_data(in_name[i], in[i]); rc != DQ_OK) return rc;
+    if (int rc = check_data(out_name[i], out[i]); rc != DQ_OK) return rc;
+  }
+  dq::HeadRows a = rows(q, q_out, q_weight), b;
+  if (k != nullptr) b = rows(k, k_out, k_weight);
+  const hipError_t e = dq::launch_norm_rope(q->dtype, q_out->dtype, tokens, (int)head_dim, a, b, eps, ra, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? DQ_OK : hip_fail(e, "qk_norm_rope launch");
+}
+
+int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, const dq_heads* v, const int64_t* slots,
+                 const float* k_weight, float eps, const dq_rope* rope, const int32_t* positions, void* stream) {
+  if (int rc = check_cache(cache, tokens > 0); rc != DQ_OK) return rc;
+  if (int rc = check_rows("k", k, tokens); rc != DQ_OK) return rc;
+  if (int rc = check_rows("v", v, tokens); rc != DQ_OK) return rc;
+  if (k->dtype != v->dtype) return dq::set_error(DQ_UNSUPPORTED, "k and v differ in type");
+  if (k->heads != cache->kv_heads || v->heads != cache->kv_heads)
+    return dq::set_error(DQ_INVALID_ARGUMENT, "%d and %d heads, the cache has %d", k->heads, v->heads, cache->kv_heads);
+  if (int rc = check_tokens(tokens, 2 * (int64_t)cache->kv_heads); rc != DQ_OK) return rc;
+  if (int rc = check_eps(k_weight, eps); rc != DQ_OK) return rc;
+  dq::RopeArgs ra;
+  if (int rc = check_rope(rope, positions, cache->head_dim, tokens, &ra); rc != DQ_OK) return rc;
+  if (tokens == 0) return DQ_OK;
+  if (slots == nullptr) return bad("slots: null argument");
+  if (int rc = check_data("k", k); rc != DQ_OK) return rc;
+  if (int rc = check_data("v", v); rc != DQ_OK) return rc;
+  if (cache->n_pages == 0) return DQ_OK;  // no slot is inside
+  const hipError_t e = dq::launch_kv_append(k->dtype, cache->dtype, tokens, cache->head_dim, rows(k, nullptr, k_weight),
+                                            rows(v, nullptr, nullptr), cache_args(cache), slots, eps, ra,
+                                            static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? DQ_OK : hip_fail(e, "kv_append launch");
+}
+
+int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a) {
+  if (check_attention(cache, a, false) != DQ_OK) return -1;
+  return 0;
+}
+
+int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+  if (int rc = check_attention(cache, a, true); rc != DQ_OK) return rc;
+  if (a->tokens == 0 || a->batch == 0) return DQ_OK;
+  if (int rc = check_data("q", a->q); rc != DQ_OK) return rc;
+  if (int rc = check_data("out", a->out); rc != DQ_OK) return rc;
+  if (a->prefix_len > 0 && a->prefix_pages == nullptr) return bad("prefix_pages: null argument");
+  if (a->max_len > 0 && (a->pages == nullptr || a->lens == nullptr)) return bad("pages, lens: null argument");
+  (void)workspace;
+  (void)workspace_bytes;
+  const hipError_t e = dq::launch_attention(a->q->dtype, cache->dtype, attn_args(cache, a), static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? DQ_OK : hip_fail(e, "shared_attention launch");
+}
+
+}  // extern "C"

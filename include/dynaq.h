@@ -411,6 +411,143 @@ DQ_API int dq_select(const dq_matmul_shape* s, const dq_plan* plan, dq_selection
 DQ_API int dq_matmul_plan(const dq_weight* w, const dq_plan* plan, const float* x, int64_t m, int64_t x_stride,
                           float* y, int64_t y_stride, const float* bias, void* stream);
 
+/* ---- the attention block: head norms and rotation, KV cache, attention -----
+ * What a decoder layer does between its matmuls: dq_matmul_many writes the q, k and
+ * v rows, dq_qk_norm_rope normalizes and rotates the heads, dq_kv_append stores the new
+ * keys and values in a paged cache (with the norm and the rotation on the way, where no
+ * one else needs the rotated keys), and dq_shared_attention lets a batch of sequences
+ * attend to a prefix they share and to their own tokens; dq_matmul takes its rows.
+ * The counterparts are dynacore's Device::rms_norm / rope / kv_store / attention
+ * members, which a quantized-matmul Device leaves to the engine's own backend.
+ *
+ * These calls run on the current device, enqueue their launches on `stream`, allocate
+ * nothing and keep nothing: they can be captured, and calls on different streams do not
+ * share memory of the library's. Lengths, offsets, positions, slots and page numbers
+ * are device memory, read when the kernels run; whatever they hold, no access leaves the
+ * buffers that the arguments describe. */
+
+/* Number types of these calls' tensors: dynacore::DType values. */
+typedef enum dq_float {
+  DQ_F32 = 0,
+  DQ_F16 = 1,
+  DQ_BF16 = 2,
+} dq_float;
+
+/* Rows of heads in device memory: head h of token t is the head_dim values from
+ * p + t * token_stride + h * head_stride (strides in values, >= 0; a head's values are
+ * contiguous). Any alignment of whole values; 16-byte aligned heads are read faster. */
+typedef struct dq_heads {
+  void* p;
+  int32_t dtype; /* dq_float */
+  int32_t heads;
+  int64_t token_stride;
+  int64_t head_stride;
+} dq_heads;
+
+/* The pairs of a head's first rot_dim values that a rotation turns together. */
+typedef enum dq_rope_style {
+  DQ_ROPE_HALVES = 0, /* (i, i + rot_dim / 2) */
+  DQ_ROPE_PAIRS = 1,  /* (2i, 2i + 1) */
+} dq_rope_style;
+
+/* A position rotation as tables: pair i of a token at position p turns by the angle whose
+ * cosine and sine are cos[p * rot_dim / 2 + i] and sin[p * rot_dim / 2 + i] (device memory,
+ * max_pos rows each); values from rot_dim on stay as they are. The tables carry whatever
+ * frequency scaling the model uses. A token whose position is not in [0, max_pos) gets NaN
+ * in place of its rotated heads. */
+typedef struct dq_rope {
+  const float* cos;
+  const float* sin;
+  int64_t max_pos;
+  int32_t rot_dim; /* even, 2..head_dim */
+  int32_t style;   /* dq_rope_style */
+} dq_rope;
+
+/* Head sizes of the attention block: multiples of 8 up to this. */
+#define DQ_MAX_HEAD_DIM 256
+
+/* q_out[t, h] = rope(norm(q[t, h])) and the same for k, in one launch. norm(x) = x / sqrt(mean
+ * x^2 + eps) * weight over the head's head_dim values (weight: head_dim floats; NULL: no
+ * norm). rope NULL: no rotation (positions is not read), else positions has one entry a token.
+ * k and k_out may be NULL (both): queries alone. All arithmetic is fp32, rounded once to the
+ * output's type (to nearest even). An output may be its input (the same pointer, type and
+ * strides), and must not overlap an input otherwise. */
+DQ_API int dq_qk_norm_rope(int64_t tokens, int64_t head_dim, const dq_heads* q, const dq_heads* q_out,
+                           const float* q_weight, const dq_heads* k, const dq_heads* k_out, const float* k_weight,
+                           float eps, const dq_rope* rope, const int32_t* positions, void* stream);
+
+/* A paged cache of keys and values of one layer: place i of page p of head h is the head_dim
+ * values from k (v) + p * page_stride + i * token_stride + h * head_stride (strides in values:
+ * any order of pages, places and heads; multiples of 8, as k and v are 16-byte aligned). The
+ * memory is the caller's. */
+typedef struct dq_kv_cache {
+  void* k;
+  void* v;
+  int32_t dtype; /* DQ_F16 or DQ_BF16 */
+  int32_t kv_heads;
+  int32_t head_dim;  /* multiple of 8, up to DQ_MAX_HEAD_DIM */
+  int32_t page_size; /* tokens a page: a multiple of 16 */
+  int64_t n_pages;
+  int64_t page_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+} dq_kv_cache;
+
+/* Appends token t's keys rope(norm(k[t])) and values v[t] (kv_heads heads of the cache's
+ * head_dim each) at slots[t] = page * page_size + place. A slot outside [0, n_pages *
+ * page_size) leaves its token out (padding: -1); a slot that is given twice holds one of the
+ * two tokens' heads. k_weight, eps, rope and positions are dq_qk_norm_rope's; without a norm
+ * and a rotation keys are converted as values are (to nearest even). */
+DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, const dq_heads* v,
+                        const int64_t* slots, const float* k_weight, float eps, const dq_rope* rope,
+                        const int32_t* positions, void* stream);
+
+/* Attention of a batch whose sequences share a prefix. The `tokens` query rows of q belong to
+ * `batch` sequences: sequence b has rows [q_offsets[b], q_offsets[b + 1]) (batch + 1 entries from 0
+ * on, not decreasing, at most max_q apart; NULL: one row each). Its keys are
+ * the prefix_len first places of the pages prefix_pages[0], [1], ... (the same for all), then
+ * the lens[b] (at most max_len) first places of pages[b * pages_stride], ...: its own tokens, the last
+ * of which are its query rows, already appended. Row i of n sees the prefix and the own keys j <=
+ * lens[b] - n + i:
+ *     out[t, h] = sum_j p_j v_j,  p = softmax over the visible j of scale * q[t, h] . k_j
+ * with the key head h / (q heads / kv_heads). A row that sees no key gets zeros (and lse -inf); so
+ * does one whose every score is -inf.
+ * lse (NULL, or tokens x q heads floats): log sum_j exp(scale * q . k_j).
+ * q and out have one type: the cache's, with 16-bit products and the softmax weights rounded
+ * to that type before the second product, or DQ_F32, where queries and weights are split so that
+ * products keep fp32's precision; sums, maxima and the softmax are fp32 always. out must not
+ * overlap q.
+ * The prefix is read once for the whole batch, not once a sequence. A row's bits depend on the call's shape (batch, tokens,
+ * max_q, prefix_len, max_len), not on timing. Rows outside every sequence are not written.
+ * A row that would read a page number outside [0, n_pages) gets NaN.
+ * workspace: dq_shared_attention_workspace bytes of device memory (16-byte aligned) that the call may overwrite; its
+ * contents need not be kept. */
+typedef struct dq_attention {
+  const dq_heads* q;
+  const dq_heads* out;
+  float* lse;
+  int64_t tokens;
+  int64_t batch;
+  const int32_t* q_offsets;
+  int64_t max_q;
+  const int32_t* prefix_pages;
+  int64_t prefix_len;
+  const int32_t* pages;
+  int64_t pages_stride;
+  const int32_t* lens;
+  int64_t max_len;
+  float scale; /* > 0 */
+} dq_attention;
+
+/* Bytes that any dq_shared_attention call can do with. */
+#define DQ_ATTENTION_WORKSPACE_BYTES (128u << 20)
+
+/* Workspace bytes of a call (0: none; -1 with dq_last_error() set if the arguments are
+ * refused). A function of the shape only: the device pointers in it may be NULL. */
+DQ_API int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a);
+DQ_API int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 /* ---- GGUF files ----------------------------------------------------------
  * A GGUF v2 / v3 model mapped read-only (mmap): header, metadata and tensor
  * directory parsed with every length and offset checked against the file
