@@ -67,8 +67,30 @@ struct AttnArgs {
   int32_t prefix_len = 0;
   int32_t max_len = 0;
   float scale_log2 = 0;  // scale * log2(e): the softmax runs on powers of two
+  bool q_vec = false, out_vec = false;  // rows of q (out) can be read (written) in 16 (16 or 8) bytes
+  float* part_o = nullptr;   // [slot][kv head][row][dim] (nullptr: one item a row, which finishes it)
+  float* part_ml = nullptr;  // [slot][kv head][row] maximum (in powers of two), sum
 };
 
-hipError_t launch_attention(int type, int cache_type, const AttnArgs& a, hipStream_t s);
+// One kind of work items: (key range, kv head, row tile), for every sequence of `own` items.
+struct AttnPart {
+  int32_t rows = 0;    // rows of a tile: 16, 64, 128
+  int32_t tiles = 0;   // row tiles (of a sequence)
+  int32_t splits = 0;  // key ranges (0: no such items)
+  int32_t chunk = 0;   // keys of a range, a multiple of 128
+  int32_t slot = 0;    // the first range's slot of the workspace
+  int32_t own_from = 0;  // with the prefix before them: where the own keys begin in the ranges
+  bool with_prefix = false;
+  bool backward = false;  // the last rows, which see most keys, first
+};
+
+// How a call's work is split: `shared` items take the prefix with the rows of all sequences,
+// `own` ones a sequence's own keys (with the prefix before them where there are no shared items).
+struct AttnPlan {
+  AttnPart shared, own;
+  int64_t slots = 0;  // parts of a row (0: none, every item finishes its rows)
+};
+
+hipError_t launch_attention(int type, int cache_type, const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 
 }  // namespace dq

@@ -137,6 +137,7 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
   if (a->q->heads != a->out->heads || a->q->heads % c->kv_heads != 0)
     return dq::set_error(DQ_INVALID_ARGUMENT, "%d query heads, %d of out, %d kv heads", a->q->heads, a->out->heads, c->kv_heads);
   if (int rc = check_tokens(a->tokens, a->q->heads); rc != DQ_OK) return rc;
+  if (c->token_stride > (1 << 25)) return dq::set_error(DQ_UNSUPPORTED, "cache: token_stride %lld", (ll)c->token_stride);
   if (a->batch > INT32_MAX - 1 || a->tokens > INT32_MAX / 2) return dq::set_error(DQ_UNSUPPORTED, "batch %lld, tokens %lld", (ll)a->batch, (ll)a->tokens);
   if (a->max_q < 1 || a->max_q > INT32_MAX / 2) return dq::set_error(DQ_INVALID_ARGUMENT, "max_q %lld", (ll)a->max_q);
   if (data && a->q_offsets == nullptr && (a->tokens != a->batch || a->max_q != 1))
@@ -149,6 +150,63 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
                          (ll)((a->max_len + c->page_size - 1) / c->page_size));
   if (!(a->scale > 0) || !std::isfinite(a->scale * kLog2e)) return bad("scale must be positive and finite");
   return DQ_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Workgroups that run at once: two on each of the 256 CUs.
+constexpr int64_t kWorkgroups = 512;
+
+// Ranges of `keys` keys for `items` row tiles: as many as fill the card, of at least `least` keys.
+void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target, int64_t least) {
+  int64_t n = target / items;
+  n = n < ceil_div(keys, least) ? n : ceil_div(keys, least);
+  n = n > 1 ? n : 1;
+  p->chunk = (int32_t)(ceil_div(ceil_div(keys, n), 128) * 128);
+  if (p->chunk == 0) p->chunk = 128;
+  p->splits = (int32_t)(keys > 0 ? ceil_div(keys, p->chunk) : 1);
+}
+
+// Bytes of the parts: O and (m, l) of every slot.
+int64_t part_bytes(const dq_kv_cache* c, const dq_attention* a, int64_t slots) {
+  return slots * a->tokens * a->q->heads * (c->head_dim + 2) * 4;
+}
+
+dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
+  const int64_t group = a->q->heads / c->kv_heads, all = a->tokens * group;
+  const int64_t max_q = a->max_q < a->tokens ? a->max_q : a->tokens, rows = max_q * group;
+  const bool f32 = a->q->dtype == DQ_F32;
+  auto tile = [&](int64_t n) { return n <= 16 ? 16 : n <= 64 || f32 ? 64 : 128; };
+  dq::AttnPlan p;
+  for (int64_t target = kWorkgroups;; target /= 2) {
+    p = dq::AttnPlan{};
+    p.own.rows = tile(rows);
+    p.own.tiles = (int32_t)ceil_div(rows, p.own.rows);
+    p.own.backward = true;
+    // The prefix with all sequences' rows, unless one sequence's rows fill tiles by themselves.
+    if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && target > 0) {
+      p.shared.rows = tile(all);
+      p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
+      split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, target, 256);
+      if (a->max_len > 0) {
+        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, target, 256);
+        p.own.slot = p.shared.splits;
+      }
+    } else {
+      p.own.with_prefix = a->prefix_len > 0;
+      p.own.own_from = (int32_t)(ceil_div(a->prefix_len, 128) * 128);
+      const int64_t items = a->batch * p.own.tiles * c->kv_heads;
+      split_keys(&p.own, items, p.own.own_from + a->max_len, target > 0 ? target : 1, 256);
+    }
+    const int64_t slots = p.shared.splits + p.own.splits;
+    p.slots = slots > 1 ? slots : 0;
+    if (part_bytes(c, a, p.slots) <= (int64_t)DQ_ATTENTION_WORKSPACE_BYTES) return p;
+  }
+}
+
+bool aligned(const dq_heads* r, size_t bytes) {
+  const size_t v = float_bytes(r->dtype);
+  return reinterpret_cast<uintptr_t>(r->p) % bytes == 0 && r->token_stride * v % bytes == 0 && r->head_stride * v % bytes == 0;
 }
 
 dq::AttnArgs attn_args(const dq_kv_cache* c, const dq_attention* a) {
@@ -174,7 +232,9 @@ dq::AttnArgs attn_args(const dq_kv_cache* c, const dq_attention* a) {
   r.pages_stride = a->pages_stride;
   r.prefix_len = (int32_t)a->prefix_len;
   r.max_len = (int32_t)a->max_len;
-  r.scale_log2 = a->scale * kLog2e;
+  r.scale_log2 = std::fmax(a->scale * kLog2e, 1.2e-38f);
+  r.q_vec = aligned(a->q, 16);
+  r.out_vec = aligned(a->out, 4 * float_bytes(a->out->dtype));
   return r;
 }
 
@@ -243,7 +303,8 @@ int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, co
 
 int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a) {
   if (check_attention(cache, a, false) != DQ_OK) return -1;
-  return 0;
+  if (a->tokens == 0 || a->batch == 0) return 0;
+  return part_bytes(cache, a, plan(cache, a).slots);
 }
 
 int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace, int64_t workspace_bytes,
@@ -254,9 +315,19 @@ int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* w
   if (int rc = check_data("out", a->out); rc != DQ_OK) return rc;
   if (a->prefix_len > 0 && a->prefix_pages == nullptr) return bad("prefix_pages: null argument");
   if (a->max_len > 0 && (a->pages == nullptr || a->lens == nullptr)) return bad("pages, lens: null argument");
-  (void)workspace;
-  (void)workspace_bytes;
-  const hipError_t e = dq::launch_attention(a->q->dtype, cache->dtype, attn_args(cache, a), static_cast<hipStream_t>(stream));
+  if (cache->n_pages == 0 && (a->prefix_len > 0 || a->max_len > 0)) return bad("cache: no pages");
+  const dq::AttnPlan p = plan(cache, a);
+  dq::AttnArgs args = attn_args(cache, a);
+  if (p.slots > 0) {
+    const int64_t need = part_bytes(cache, a, p.slots);
+    if (workspace == nullptr) return bad("workspace: null argument");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return bad("workspace: must be 16-byte aligned");
+    if (workspace_bytes < need)
+      return dq::set_error(DQ_RESOURCE_EXHAUSTED, "workspace: %lld bytes, the call needs %lld", (ll)workspace_bytes, (ll)need);
+    args.part_o = static_cast<float*>(workspace);
+    args.part_ml = args.part_o + p.slots * a->tokens * a->q->heads * cache->head_dim;
+  }
+  const hipError_t e = dq::launch_attention(a->q->dtype, cache->dtype, args, p, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? DQ_OK : hip_fail(e, "shared_attention launch");
 }
 
