@@ -107,47 +107,63 @@ DQ_DEV float row_sum(float x) {
   return as_f(b[0]) + as_f(b[1]);
 }
 
+// A load of 16 bytes a lane straight to LDS: lane l's from base + off to the LDS address lds + 16 l. Written
+// as an instruction because the compiler would wait for every load under way before any read of
+// LDS; the wait is where the tile changes hands (wait_loads, then the barrier). M0, which holds the
+// LDS address, is left as it was.
+DQ_DEV void load_to_lds(const void* base, u32 off, u32 lds) {
+  u32 m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "s"(lds), "v"(off), "s"(base)
+      : "memory");
+}
+DQ_DEV void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+DQ_DEV u32 lds_address(const void* p) { return (u32)(uintptr_t)(DQ_LDS(const void)*)p; }
+
+// A page number through the scalar cache.
+DQ_DEV int page_at(const int32_t* pages, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)pages)[i];
+}
+
 // ---- infinite and NaN values that only some rows of a tile see ------------
 // A masked key has weight 0, but 0 times an infinite value is NaN in a matrix product. In tiles
-// that some rows see in part, such values are taken out of the product and added to the rows that
-// see them.
+// that some rows see in part, such values are taken out of the product and noted, and the rows that
+// see them get them at the end. A row sees every key that an earlier row of its item sees, so
+// the first row is all that is noted of a value's column: first[0] for +inf and NaN, first[1]
+// for -inf and NaN.
 template <int TC>
 constexpr u32 kExp = TC == DQ_F16 ? 0x7C00u : 0x7F80u;
-template <int TC>
-constexpr u32 kOne = TC == DQ_F16 ? 0x3C00u : 0x3F80u;
 
 template <int TC>
-DQ_DEV bool has_nonfinite(v4u x) {
-  bool nf = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    nf |= (x[i] & kExp<TC>) == kExp<TC> || (x[i] & (kExp<TC> << 16)) == (kExp<TC> << 16);
-  return nf;
+DQ_DEV bool nonfinite(u32 x) {
+  return (x & kExp<TC>) == kExp<TC> || (x & (kExp<TC> << 16)) == (kExp<TC> << 16);
 }
-template <int TC>
-DQ_DEV void take_nonfinite(v4u& x, v4u& pos, v4u& neg) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    u32 c = 0, p = 0, n = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32 v = (x[i] >> (16 * h)) & 0xFFFFu;
-      const bool nf = (v & kExp<TC>) == kExp<TC>, nan = nf && (v & 0x7FFFu) != kExp<TC>, sign = v >> 15;
-      c |= (nf ? 0u : v) << (16 * h);
-      p |= (nf && (nan || !sign) ? kOne<TC> : 0u) << (16 * h);
-      n |= (nf && (nan || sign) ? kOne<TC> : 0u) << (16 * h);
+// Notes the infinite and NaN values of a dword (columns d, d + 1; seen from row `row` on, by none if
+// it is past the item) and returns it without them.
+template <int TC, int DP>
+DQ_DEV u32 take_nonfinite(u32 x, int d, int row, int rows, int (&first)[2][DP]) {
+  u32 clean = 0;
+  for (int h = 0; h < 2; ++h) {
+    const u32 v = (x >> (16 * h)) & 0xFFFFu;
+    if ((v & kExp<TC>) != kExp<TC>) {
+      clean |= v << (16 * h);
+    } else if (row < rows) {
+      const bool nan = (v & 0x7FFFu) != kExp<TC>;
+      if (nan || v < 0x8000u) atomicMin(&first[0][d + h], row);
+      if (nan || v >= 0x8000u) atomicMin(&first[1][d + h], row);
     }
-    x[i] = c;
-    pos[i] = p;
-    neg[i] = n;
   }
+  return clean;
 }
-template <int TC>
-DQ_DEV v4f add_nonfinite(v4u pos, v4u neg, v4u sees, v4f o) {
-  const v4f p = mma<TC>(pos, sees, v4f{0, 0, 0, 0}), n = mma<TC>(neg, sees, v4f{0, 0, 0, 0});
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] += (p[i] > 0 ? INFINITY : 0.f) + (n[i] > 0 ? -INFINITY : 0.f);
-  return o;
+template <int DP>
+DQ_DEV float noted(const int (&first)[2][DP], int row, int d) {
+  return (row >= first[0][d] ? INFINITY : 0.f) + (row >= first[1][d] ? -INFINITY : 0.f);
 }
 
 // ---- rows ------------------------------------------------------------------
@@ -220,6 +236,12 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
 // Own keys that row r sees.
 DQ_DEV int own_limit(const AttnArgs& a, const Item& it, int token) {
   return it.b < 0 ? 0 : min(max(it.own0 + token - it.token0, 0), it.len);
+}
+
+// The first row of the item that sees own key `key` (its count or more: none does); of the
+// prefix every row sees every key.
+DQ_DEV int first_row(const AttnArgs& a, const Item& it, int key) {
+  return max(0, (it.token0 + key + 1 - it.own0) * a.group - it.first);
 }
 
 // The query fragments of rows: lane l has row l % 16 and, of every 32 values, 8 (l / 16) .. + 7. Returns
@@ -333,18 +355,29 @@ struct KvRegs {
   u32 v[8][DP / 32];  // [key slot][dword]: DP / 16 values
 };
 
+template <int DP>
+struct FewLds {
+  v4f o[4][16][DP / 4];
+  float ml[4][16][2];
+  int first[2][DP];
+  int bad, noted;
+};
+
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a, AttnPart w, bool stacked) {
+DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int index, FewLds<DP>& sh) {
   constexpr int NP = kParts<T, TC>;
   constexpr int NC = DP / 16;
-  __shared__ float s_ml[4][16][2];
-  __shared__ v4f s_o[4][16][DP / 4];
-  __shared__ int s_bad;
+  auto &s_o = sh.o;
+  auto &s_ml = sh.ml;
+  auto &s_first = sh.first;
+  int &s_bad = sh.bad, &s_noted = sh.noted;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   Item it;
-  if (!find_item(a, w, stacked, blockIdx.x, 16, it)) return;
-  if (threadIdx.x == 0) s_bad = 0;
+  if (!find_item(a, w, stacked, index, 16, it)) return;
+  if (threadIdx.x == 0) s_bad = s_noted = 0;
+  for (int i = threadIdx.x; i < 2 * DP; i += 256) (&s_first[0][0])[i] = 1 << 30;
+  __syncthreads();
 
   const bool valid = n < it.count;
   const int row = it.first + (valid ? n : 0);
@@ -372,19 +405,40 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a,
     voff[s] = d < a.dim ? 4 * g * token_bytes + d * 2 : kOut;
   }
 
-  auto base_of = [&](const int32_t* pages, int key) -> int64_t {
-    const int p = key / ca.page_size;
-    int id = uniform(pages[p]);
-    if ((u32)id >= (u32)ca.n_pages) {
-      bad = true;
-      id = 0;
-    }
-    return (int64_t)id * ca.page + (int64_t)(key - p * ca.page_size) * ca.token + (int64_t)it.head * ca.head;
+  // The keys in tiles of 32, the prefix's before the own; a wave takes every fourth. The page numbers
+  // of a tile are read one step ahead of its loads.
+  const int tiles_p = (it.pk1 - it.pk0 + 31) / 32;
+  const int tiles = tiles_p + max(0, (it.ok1 - it.ok0 + 31) / 32);
+  const int32_t* own_pages = a.pages + (int64_t)max(it.b, 0) * a.pages_stride;
+  struct Place {
+    int id[2], in[2];  // of each half's page: its number, the half's first place
   };
-  auto load = [&](const int32_t* pages, int kb, int kend, KvRegs<DP>& r) {
+  auto place = [&](int tile) {
+    const bool pre = tile < tiles_p;
+    const int32_t* pages = pre ? a.prefix_pages : own_pages;
+    const int kend = pre ? it.pk1 : it.ok1;
+    const int kb = pre ? it.pk0 + tile * 32 : it.ok0 + (tile - tiles_p) * 32;
+    Place r;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = t == 0 || kb + 16 < kend ? kb + 16 * t : kb;
+      const int p = key / ca.page_size;
+      r.id[t] = page_at(pages, p);
+      r.in[t] = key - p * ca.page_size;
+    }
+    return r;
+  };
+  auto load = [&](const Place& pl, KvRegs<DP>& r) {
     int64_t base[2];
-    base[0] = base_of(pages, kb);
-    base[1] = kb + 16 < kend ? base_of(pages, kb + 16) : base[0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int id = pl.id[t];
+      if ((u32)id >= (u32)ca.n_pages) {
+        bad = true;
+        id = 0;
+      }
+      base[t] = (int64_t)id * ca.page + (int64_t)pl.in[t] * ca.token + (int64_t)it.head * ca.head;
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const auto kr = rsrc(ca.k + base[t], 0x7FFFFFFFu);
@@ -411,7 +465,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a,
       }
     }
   };
-  auto compute = [&](int kb, int kend, int lim, int least, KvRegs<DP>& r) {
+  auto compute = [&](int tile, KvRegs<DP>& r) {
+    const bool own = tile >= tiles_p;
+    const int kb = own ? it.ok0 + (tile - tiles_p) * 32 : it.pk0 + tile * 32;
+    const int kend = own ? it.ok1 : it.pk1;
+    const int lim = !valid ? 0 : own ? own_lim : it.pk1, least = own ? own_least : it.pk1;
     float x[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -423,18 +481,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a,
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * t + i] = acc[i];
     }
-    const bool edge = kb + 32 > least || kb + 32 > kend;
-    v4u sees = {0, 0, 0, 0};
-    if (edge) {
+    if (kb + 32 > least || kb + 32 > kend) {
+      bool nf = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-        const bool in = key < lim && key < kend;
-        x[j] = in ? x[j] : -INFINITY;
-        sees[j >> 1] |= in ? kOne<TC> << (16 * (j & 1)) : 0u;
-        if (key >= kend)  // places past the keys may hold anything
+        x[j] = key < lim && key < kend ? x[j] : -INFINITY;
 #pragma unroll
-          for (int e = 0; e < DP / 32; ++e) r.v[j][e] = 0;
+        for (int e = 0; e < DP / 32; ++e) {
+          if (key >= kend) r.v[j][e] = 0;  // places past the keys may hold anything
+          nf |= nonfinite<TC>(r.v[j][e]);
+        }
+      }
+      if (__any(nf)) {
+        if (lane == 0) s_noted = 1;
+        u32* tmp = reinterpret_cast<u32*>(&s_o[wave][0][0]) + lane;
+#pragma unroll
+        for (int j = 0; j < 8 * (DP / 32); ++j) tmp[64 * j] = r.v[j / (DP / 32)][j % (DP / 32)];
+#pragma unroll 1
+        for (int j = 0; j < 8 * (DP / 32); ++j) {
+          const int slot = j / (DP / 32), key = kb + 16 * (slot >> 2) + 4 * g + (slot & 3);
+          if (nonfinite<TC>(tmp[64 * j]))
+            tmp[64 * j] = take_nonfinite<TC, DP>(tmp[64 * j], n * NC + j % (DP / 32) * 2, own ? first_row(a, it, key) : 0,
+                                                 it.count, s_first);
+        }
+#pragma unroll
+        for (int j = 0; j < 8 * (DP / 32); ++j) r.v[j / (DP / 32)][j % (DP / 32)] = tmp[64 * j];
       }
     }
     const float alpha = softmax_step<TC, 8>(x, c, m, l);
@@ -456,41 +528,42 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a,
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         vt[e] = __builtin_amdgcn_perm(r.v[2 * e + 1][i >> 1], r.v[2 * e][i >> 1], (i & 1) ? 0x07060302u : 0x05040100u);
-      if (edge && __any(has_nonfinite<TC>(vt))) {
-        v4u pos, neg;
-        take_nonfinite<TC>(vt, pos, neg);
-        o[i] = add_nonfinite<TC>(pos, neg, sees, o[i]);
-      }
 #pragma unroll
       for (int k = NP - 1; k >= 0; --k) o[i] = mma<TC>(vt, p[k], o[i]);
     }
   };
-  auto range = [&](const int32_t* pages, int k0, int k1, int lim, int least) {
-    int kb = k0 + 32 * wave;
-    if (kb >= k1) return;
-    if constexpr (DP <= 128) {
-      KvRegs<DP> r0, r1;
-      load(pages, kb, k1, r0);
-      while (true) {
-        if (kb + 128 < k1) load(pages, kb + 128, k1, r1);
-        compute(kb, k1, lim, least, r0);
-        kb += 128;
-        if (kb >= k1) break;
-        if (kb + 128 < k1) load(pages, kb + 128, k1, r0);
-        compute(kb, k1, lim, least, r1);
-        kb += 128;
-        if (kb >= k1) break;
-      }
-    } else {
-      for (; kb < k1; kb += 128) {
-        KvRegs<DP> r;
-        load(pages, kb, k1, r);
-        compute(kb, k1, lim, least, r);
-      }
+  // Two tiles' registers, one loading while the other is used, where the row's operands leave room.
+  int tile = wave;
+  if constexpr (DP * NP <= 128) {
+    KvRegs<DP> r0, r1;
+    Place next;
+    if (tile < tiles) {
+      load(place(tile), r0);
+      next = place(min(tile + 4, tiles - 1));
     }
-  };
-  range(a.prefix_pages, it.pk0, it.pk1, valid ? it.pk1 : 0, it.pk1);
-  if (it.b >= 0) range(a.pages + it.b * a.pages_stride, it.ok0, it.ok1, valid ? own_lim : 0, own_least);
+    auto step = [&](KvRegs<DP>& cur, KvRegs<DP>& other) {
+      if (tile + 4 < tiles) {
+        load(next, other);
+        next = place(min(tile + 8, tiles - 1));
+      }
+      compute(tile, cur);
+      tile += 4;
+    };
+    while (tile < tiles) {
+      step(r0, r1);
+      if (tile >= tiles) break;
+      step(r1, r0);
+    }
+  } else {
+    Place next;
+    if (tile < tiles) next = place(tile);
+    for (; tile < tiles; tile += 4) {
+      KvRegs<DP> r;
+      load(next, r);
+      next = place(min(tile + 4, tiles - 1));
+      compute(tile, r);
+    }
+  }
 
   // the waves' sums join in LDS
   l = row_sum(l);
@@ -523,6 +596,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_few(AttnArgs a,
       if (mk != -INFINITY) y += s_o[k][r][d4] * f;
     }
     if (s_bad) sum = __builtin_nanf("");
+    if (s_noted)
+      for (int e = 0; e < 4; ++e) y[e] += noted<DP>(s_first, r, 4 * d4 + e);
     const int rw = it.first + r, tk = rw / a.group, h = it.head * a.group + rw % a.group;
     if (a.part_o == nullptr) {
       if (it.b < 0 && a.q_offsets != nullptr && (tk < a.q_offsets[0] || tk >= a.q_offsets[a.batch])) continue;
@@ -557,19 +632,28 @@ DQ_DEV int swizzle_v(int key) {
   return DP == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
 }
 
+template <int DP>
+struct TileLds {
+  uint16_t k[2][kTileKeys<DP> * DP];
+  uint16_t v[2][kTileKeys<DP> * DP];
+  int first[2][DP];
+  int bad;
+};
+
 template <int T, int TC, int DP, int RT>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_tile(AttnArgs a, AttnPart w, bool stacked) {
+DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int index, TileLds<DP>& sh) {
   constexpr int NP = kParts<T, TC>;
   constexpr int NC = DP / 16, KT = kTileKeys<DP>, CH = DP / 8;
   constexpr int KW = KT / 4, KI = 64 / CH;  // keys a wave loads of a tile, and with one instruction
-  __shared__ __align__(16) uint16_t s_k[2][KT * DP];
-  __shared__ __align__(16) uint16_t s_v[2][KT * DP];
-  __shared__ int s_bad;
+  auto &s_k = sh.k, &s_v = sh.v;
+  auto& s_first = sh.first;
+  int& s_bad = sh.bad;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   Item it;
-  if (!find_item(a, w, stacked, blockIdx.x, 64 * RT, it)) return;
+  if (!find_item(a, w, stacked, index, 64 * RT, it)) return;
   if (threadIdx.x == 0) s_bad = 0;
+  for (int i = threadIdx.x; i < 2 * DP; i += 256) (&s_first[0][0])[i] = 1 << 30;
   if (a.dim < DP) {  // the loads leave the places past a head's values as they are: zero
     for (int i = threadIdx.x; i < 2 * KT * DP / 8; i += 256) {
       reinterpret_cast<v4u*>(&s_k[0][0])[i] = v4u{0, 0, 0, 0};
@@ -580,80 +664,150 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_tile(AttnArgs a
 
   const int wr = wave * 16 * RT;  // the wave's first row of the tile
   const int wrows = min(max(it.count - wr, 0), 16 * RT);
-  int row[RT], lim[RT];
-  bool valid[RT];
+  int own_lim[RT];
   float c[RT], m[RT], l[RT];
   v4u q[RT][NP][DP / 32];
   v4f o[RT][NC];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    valid[t] = 16 * t + n < wrows;
-    row[t] = it.first + (valid[t] ? wr + 16 * t + n : 0);
-    const int token = row[t] / a.group;
-    lim[t] = valid[t] ? own_limit(a, it, token) : 0;
-    c[t] = load_q<T, TC, DP>(a, valid[t], token, it.head * a.group + row[t] % a.group, g, q[t]);
+    const bool valid = 16 * t + n < wrows;
+    const int row = it.first + (valid ? wr + 16 * t + n : 0);
+    const int token = row / a.group;
+    own_lim[t] = valid ? own_limit(a, it, token) : 0;
+    c[t] = load_q<T, TC, DP>(a, valid, token, it.head * a.group + row % a.group, g, q[t]);
     m[t] = -INFINITY;
     l[t] = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[t][i] = v4f{0, 0, 0, 0};
   }
-  // own keys that the wave's first and last row see
-  const int least = wrows > 0 ? own_limit(a, it, (it.first + wr) / a.group) : 0;
-  const int most = wrows > 0 ? own_limit(a, it, (it.first + wr + wrows - 1) / a.group) : 0;
-  bool bad = false;
+  // own keys that the wave's first and last row see, and the item's first
+  const int own_least = wrows > 0 ? own_limit(a, it, (it.first + wr) / a.group) : 0;
+  const int own_most = wrows > 0 ? own_limit(a, it, (it.first + wr + wrows - 1) / a.group) : 0;
+  const int item_least = own_limit(a, it, it.first / a.group);
+  bool bad = false, noting = false;
 
   const CacheArgs& ca = a.cache;
+  const u32 token_bytes = (u32)ca.token * 2;
   const int32_t* own_pages = a.pages + (int64_t)max(it.b, 0) * a.pages_stride;
   const int tiles_p = (it.pk1 - it.pk0 + KT - 1) / KT;
   const int tiles = tiles_p + max(0, (it.ok1 - it.ok0 + KT - 1) / KT);
 
-  auto issue = [&](int tile, int buf) {
+  // Chunk places of this lane's loads and reads (swizzle_k and swizzle_v repeat every 16 keys).
+  const int lrow = lane / CH;
+  u32 kpos[KW / KI], vpos[KW / KI];
+#pragma unroll
+  for (int i = 0; i < KW / KI; ++i) {
+    kpos[i] = ((lane % CH) ^ swizzle_k<DP>(wave * KW + i * KI + lrow)) * 16;
+    vpos[i] = ((lane % CH) ^ swizzle_v<DP>(wave * KW + i * KI + lrow)) * 16;
+  }
+  u32 kread[DP / 32], vread[NC];
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) kread[e] = n * DP + ((4 * e + g) ^ swizzle_k<DP>(n)) * 8;
+  const int vkey = 4 * g + (n >> 2);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) vread[i] = vkey * DP + ((2 * i + ((n >> 1) & 1)) ^ swizzle_v<DP>(vkey)) * 8 + (n & 1) * 4;
+
+  // The wave's keys of a tile lie in one page; its number is read one tile ahead of the loads.
+  struct Place {
+    int in, start, id, last;
+  };
+  auto place = [&](int tile) {
     const bool pre = tile < tiles_p;
-    const int32_t* pages = pre ? a.prefix_pages : own_pages;
     const int kend = pre ? it.pk1 : it.ok1;
     const int kb = (pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT) + wave * KW;
-    const int in = min(kb, kend - 1);
-    const int p = in / ca.page_size;
-    int id = uniform(pages[p]);
+    Place r;
+    r.in = min(kb, kend - 1);  // (past the keys the last one is loaded again)
+    const int p = r.in / ca.page_size;
+    r.start = p * ca.page_size;
+    r.id = page_at(pre ? a.prefix_pages : own_pages, p);
+    r.last = kend - 1 - r.in;
+    return r;
+  };
+  const u32 lds_k = lds_address(&s_k[0][wave * KW * DP]), lds_v = lds_address(&s_v[0][wave * KW * DP]);
+  auto issue = [&](const Place& r, int buf) {
+    int id = r.id;
     if ((u32)id >= (u32)ca.n_pages) {
       bad = true;
       id = 0;
     }
-    const int64_t base = (int64_t)id * ca.page + (int64_t)it.head * ca.head;
+    const int64_t base = (int64_t)id * ca.page + (int64_t)(r.in - r.start) * ca.token + (int64_t)it.head * ca.head;
     const uint16_t *kp = ca.k + base, *vp = ca.v + base;
-    const int start = p * ca.page_size;
+    const u32 to = buf * KT * DP * 2;
 #pragma unroll
     for (int i = 0; i < KW / KI; ++i) {
-      const int local = wave * KW + i * KI + lane / CH, pos = lane % CH;
-      const int64_t at = (int64_t)(min(kb + i * KI + lane / CH, kend - 1) - start) * ca.token;
-      const int ck = pos ^ swizzle_k<DP>(local), cv = pos ^ swizzle_v<DP>(local);
-      if (ck * 8 < a.dim)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp + at + ck * 8),
-                                         (DQ_LDS(void)*)&s_k[buf][(wave * KW + i * KI) * DP], 16, 0, 0);
-      if (cv * 8 < a.dim)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp + at + cv * 8),
-                                         (DQ_LDS(void)*)&s_v[buf][(wave * KW + i * KI) * DP], 16, 0, 0);
+      const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes;
+      if (a.dim == DP) {
+        load_to_lds(kp, at + kpos[i], lds_k + to + i * 1024);
+        load_to_lds(vp, at + vpos[i], lds_v + to + i * 1024);
+      } else {
+        if (kpos[i] < (u32)a.dim * 2) load_to_lds(kp, at + kpos[i], lds_k + to + i * 1024);
+        if (vpos[i] < (u32)a.dim * 2) load_to_lds(vp, at + vpos[i], lds_v + to + i * 1024);
+      }
     }
   };
 
-  auto compute = [&](int kb, const int (&limit)[RT], int least_, int most_, const uint16_t* sk, const uint16_t* sv) {
-    if (kb >= most_) return;
+  Place next = {};
+  if (tiles > 0) {
+    issue(place(0), 0);
+    next = place(min(1, tiles - 1));
+  }
+  for (int tile = 0; tile < tiles; ++tile) {
+    wait_loads();     // this wave's part of the tile is in LDS
+    __syncthreads();  // everyone's is, and the other buffer is read out
+    if (tile + 1 < tiles) {
+      issue(next, (tile + 1) & 1);
+      next = place(min(tile + 2, tiles - 1));
+    }
+    const bool pre = tile < tiles_p;
+    const int kb = pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT;
+    const int least = wrows == 0 ? 0 : pre ? it.pk1 : own_least;
+    const int most = wrows == 0 ? 0 : pre ? it.pk1 : own_most;
+    const uint16_t* sk = s_k[tile & 1];
+    uint16_t* sv = s_v[tile & 1];
+
+    if (kb + KT > (pre ? it.pk1 : item_least)) {  // some row sees the tile in part
+      bool nf = false;
+      for (int i = threadIdx.x; i < KT * DP / 2; i += 256) nf |= nonfinite<TC>(reinterpret_cast<const u32*>(sv)[i]);
+      if (__syncthreads_or(nf)) {
+        noting = true;
+        for (int i = threadIdx.x; i < KT * DP / 2; i += 256) {
+          const u32 x = reinterpret_cast<const u32*>(sv)[i];
+          if (!nonfinite<TC>(x)) continue;
+          const int local = i / (DP / 2), pos = i % (DP / 2) / 4;
+          const int d = (pos ^ swizzle_v<DP>(local)) * 8 + i % 4 * 2, key = kb + local;
+          const int from = key >= (pre ? it.pk1 : it.ok1) ? it.count : pre ? 0 : first_row(a, it, key);
+          reinterpret_cast<u32*>(sv)[i] = take_nonfinite<TC, DP>(x, d, from, it.count, s_first);
+        }
+        __syncthreads();
+      }
+    }
+    if (kb >= most) continue;  // (the wave's rows see none of it)
+
     v4f s[RT][KT / 16];
 #pragma unroll
     for (int u = 0; u < KT / 16; ++u) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) s[t][u] = v4f{0, 0, 0, 0};
-      const int key = 16 * u + n;
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e) {
-        const v4u kf = *reinterpret_cast<const v4u*>(sk + key * DP + ((4 * e + g) ^ swizzle_k<DP>(key)) * 8);
+        const v4u kf = *reinterpret_cast<const v4u*>(sk + kread[e] + 16 * u * DP);
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int p = NP - 1; p >= 0; --p) s[t][u] = mma<TC>(kf, q[t][p][e], s[t][u]);
       }
     }
-    const bool edge = kb + KT > least_;
+    if (kb + KT > least) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int lim = pre ? it.pk1 : own_lim[t];
+#pragma unroll
+        for (int u = 0; u < KT / 16; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (kb + 16 * u + 4 * g + i >= lim) s[t][u][i] = -INFINITY;
+      }
+    }
     u32 pw[RT][NP][KT / 32][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -661,10 +815,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_tile(AttnArgs a
 #pragma unroll
       for (int u = 0; u < KT / 16; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[4 * u + i] = s[t][u][i];
-          if (edge) x[4 * u + i] = kb + 16 * u + 4 * g + i < limit[t] ? x[4 * u + i] : -INFINITY;
-        }
+        for (int i = 0; i < 4; ++i) x[4 * u + i] = s[t][u][i];
       const float alpha = softmax_step<TC, KT / 4>(x, c[t], m[t], l[t]);
       if (__any(alpha != 1.f)) {
 #pragma unroll
@@ -678,176 +829,221 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn_tile(AttnArgs a
         for (int p = 0; p < NP; ++p) pw[t][p][u / 4][u % 4] = parts[p];
       }
     }
-    auto value = [&](int u, int i) {  // the operand of values 16 i .. + 15 and keys 32 u .. + 31
-      v4u x;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = 32 * u + 16 * h + 4 * g + (n >> 2);
-        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (DQ_LDS(v4s)*)(sv + key * DP + ((2 * i + ((n >> 1) & 1)) ^ swizzle_v<DP>(key)) * 8 + (n & 1) * 4));
-        const v2u z = __builtin_bit_cast(v2u, y);
-        x[2 * h] = z[0];
-        x[2 * h + 1] = z[1];
-      }
-      return x;
-    };
-    if (!edge) {
+    for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-      for (int u = 0; u < KT / 32; ++u)
+      for (int i = 0; i < NC; ++i) {
+        v4u vt;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const v4u vt = value(u, i);
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-              o[t][i] = mma<TC>(vt, v4u{pw[t][p][u][0], pw[t][p][u][1], pw[t][p][u][2], pw[t][p][u][3]}, o[t][i]);
+        for (int h = 0; h < 2; ++h) {
+          const v2u z = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                    (DQ_LDS(v4s)*)(sv + vread[i] + (32 * u + 16 * h) * DP)));
+          vt[2 * h] = z[0];
+          vt[2 * h + 1] = z[1];
         }
-    } else {
-#pragma unroll
-      for (int u = 0; u < KT / 32; ++u) {
-        v4u sees[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = kb + 32 * u + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-            sees[t][j] = (key < limit[t] ? kOne<TC> : 0u) | (key + 1 < limit[t] ? kOne<TC> << 16 : 0u);
-          }
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          v4u vt = value(u, i);
-          if (__any(has_nonfinite<TC>(vt))) {
-            v4u pos, neg;
-            take_nonfinite<TC>(vt, pos, neg);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) o[t][i] = add_nonfinite<TC>(pos, neg, sees[t], o[t][i]);
-          }
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-              o[t][i] = mma<TC>(vt, v4u{pw[t][p][u][0], pw[t][p][u][1], pw[t][p][u][2], pw[t][p][u][3]}, o[t][i]);
-        }
+          for (int p = NP - 1; p >= 0; --p)
+            o[t][i] = mma<TC>(vt, v4u{pw[t][p][u][0], pw[t][p][u][1], pw[t][p][u][2], pw[t][p][u][3]}, o[t][i]);
       }
-    }
-  };
-
-  int pre_lim[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) pre_lim[t] = valid[t] ? it.pk1 : 0;
-  const int pre = wrows > 0 ? it.pk1 : 0;
-  if (tiles > 0) issue(0, 0);
-  for (int tile = 0; tile < tiles; ++tile) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile is in LDS
-    __syncthreads();                     // everyone's is, and the other buffer is read out
-    if (tile + 1 < tiles) issue(tile + 1, (tile + 1) & 1);
-    const uint16_t *sk = s_k[tile & 1], *sv = s_v[tile & 1];
-    if (tile < tiles_p)
-      compute(it.pk0 + tile * KT, pre_lim, pre, pre, sk, sv);
-    else
-      compute(it.ok0 + (tile - tiles_p) * KT, lim, least, most, sk, sv);
   }
   if (bad) s_bad = 1;
   __syncthreads();
   const bool nan = s_bad != 0;
+  const int64_t part = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group;
+  auto covered = [&](int token) {
+    return it.b >= 0 || a.q_offsets == nullptr || (token >= a.q_offsets[0] && token < a.q_offsets[a.batch]);
+  };
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     float sum = row_sum(l[t]);
     if (nan) sum = __builtin_nanf("");
-    if (!valid[t]) continue;
-    const int tk = row[t] / a.group, h = it.head * a.group + row[t] % a.group;
+    if (16 * t + n >= wrows) continue;
+    const int row = it.first + wr + 16 * t + n, token = row / a.group, h = it.head * a.group + row % a.group;
     if (a.part_o == nullptr) {
-      if (it.b < 0 && a.q_offsets != nullptr && (tk < a.q_offsets[0] || tk >= a.q_offsets[a.batch])) continue;
+      if (!covered(token)) continue;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t at = (int64_t)tk * a.out_token + (int64_t)h * a.out_head;
+      const int64_t at = (int64_t)token * a.out_token + (int64_t)h * a.out_head;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (16 * i + 4 * g < a.dim) store4<T>(a, at, 16 * i + 4 * g, o[t][i] * inv);
-      if (a.lse != nullptr && g == 0) a.lse[(int64_t)tk * a.heads + h] = lse_of(m[t], sum, kShift<TC>);
+      if (a.lse != nullptr && g == 0) a.lse[(int64_t)token * a.heads + h] = lse_of(m[t], sum, kShift<TC>);
     } else {
-      const int64_t at = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group + row[t];
+      const int64_t at = part + row;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (16 * i + 4 * g < a.dim) *reinterpret_cast<v4f*>(a.part_o + at * a.dim + 16 * i + 4 * g) = o[t][i];
       if (g == 0) *reinterpret_cast<v2f*>(a.part_ml + at * 2) = v2f{m[t], sum};
     }
   }
+  if (noting) {  // the infinite and NaN values go to what has just been written
+    __syncthreads();
+    for (int i = threadIdx.x; i < it.count * a.dim; i += 256) {
+      const int r = i / a.dim, d = i % a.dim, row = it.first + r;
+      const float y = noted<DP>(s_first, r, d);
+      if (y == 0.f) continue;
+      const int token = row / a.group;
+      if (a.part_o != nullptr) {
+        a.part_o[(part + row) * a.dim + d] += y;
+      } else if (covered(token)) {
+        const int64_t at = (int64_t)token * a.out_token + (int64_t)(it.head * a.group + row % a.group) * a.out_head + d;
+        store1<T>(a.out, at, load1<T>(a.out, at) + y);
+      }
+    }
+  }
+}
+
+// ---- the launch: shared items, then own ones ---------------------------------
+
+// Item of workgroup b of n. Workgroups go to the 8 XCDs in turn: consecutive items, which read the same keys for
+// other rows, stay on one XCD and its L2.
+DQ_DEV int xcd_item(int b, int n) {
+  const int each = n / 8;
+  return b < 8 * each ? b % 8 * each + b / 8 : b;
+}
+
+template <int T, int TC, int DP, int ROWS, class Lds>
+DQ_DEV void run_item(const AttnArgs& a, const AttnPart& w, bool stacked, int index, Lds& sh) {
+  if constexpr (ROWS == 16)
+    few_rows<T, TC, DP>(a, w, stacked, index, sh.few);
+  else
+    many_rows<T, TC, DP, ROWS / 64>(a, w, stacked, index, sh.tile);
+}
+
+template <int DP, int MOST>
+union AttnLds {
+  FewLds<DP> few;
+  TileLds<DP> tile;
+};
+template <int DP>
+union AttnLds<DP, 16> {
+  FewLds<DP> few;
+};
+
+// RS, RO: rows of the shared and of the own items' tiles.
+template <int T, int TC, int DP, int RS, int RO>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
+  __shared__ __align__(16) AttnLds<DP, RS> sh;
+  const int b = blockIdx.x;
+  if constexpr (RS == RO) {
+    const bool stacked = b < shared;
+    AttnPart w;
+    w.tiles = stacked ? ws.tiles : wo.tiles;
+    w.splits = stacked ? ws.splits : wo.splits;
+    w.chunk = stacked ? ws.chunk : wo.chunk;
+    w.slot = stacked ? ws.slot : wo.slot;
+    w.own_from = wo.own_from;
+    w.with_prefix = wo.with_prefix;
+    w.backward = wo.backward;
+    run_item<T, TC, DP, RS>(a, w, stacked, stacked ? xcd_item(b, shared) : xcd_item(b - shared, own), sh);
+  } else {
+    if (b < shared)
+      run_item<T, TC, DP, RS>(a, ws, true, xcd_item(b, shared), sh);
+    else
+      run_item<T, TC, DP, RO>(a, wo, false, xcd_item(b - shared, own), sh);
+  }
 }
 
 // ---- the join: the parts of a row, one wave a row ----------------------------
 
-// The sequence of token t: the last b with q_offsets[b] <= t (-1: none).
-DQ_DEV int find_seq(const AttnArgs& a, int t) {
+// The sequence of token t, the last b with q_offsets[b] <= t (-1: none): a wave's lanes look at 64 places
+// at a time.
+DQ_DEV int find_seq(const AttnArgs& a, int t, int lane) {
   if (a.q_offsets == nullptr) return t;
-  int lo = -1, hi = a.batch;  // q_offsets[lo] <= t < q_offsets[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.q_offsets[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
+  int lo = 0, n = a.batch + 1;  // entries still in question: the count of those <= t is in lo .. lo + n
+  while (n > 0) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const bool le = lane * step < n && a.q_offsets[i] <= t;
+    const int cnt = __popcll(__ballot(le));
+    if (cnt == 0) break;
+    if (step == 1) {
+      lo += cnt;
+      break;
+    }
+    const int last = (cnt - 1) * step;  // entry lo + last is <= t, the next looked at is not
+    n = min(step, n - last) - 1;
+    lo += last + 1;
   }
-  return lo >= 0 && t < a.q_offsets[lo + 1] ? lo : -1;
+  lo = uniform(lo);
+  return lo >= 1 && lo <= a.batch ? lo - 1 : -1;
 }
 
+// Weights of up to 64 parts at a time lie one to a lane; their sums of v are read 8 at a time.
 template <int T, int TC>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, AttnPart wb) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   const int t = uniform((int)(id / a.heads)), h = uniform((int)(id % a.heads));
   if (t >= a.tokens) return;
-  const int b = find_seq(a, t);
+  const int b = find_seq(a, t, lane);
   if (b < 0) return;
   // the own parts that were written: those that begin inside the sequence, and the first
   const int len = a.max_len > 0 ? min(max(a.lens[b], 0), a.max_len) : 0;
   const int end = wb.with_prefix ? (len > 0 ? wb.own_from + len : a.prefix_len) : len;
-  const int own = min(wb.splits, max(1, (end + wb.chunk - 1) / max(wb.chunk, 1)));
-  const int parts = wa.splits + (wb.splits > 0 ? own : 0);
+  const int own = wb.splits > 0 ? min(wb.splits, max(1, (end + wb.chunk - 1) / wb.chunk)) : 0;
+  const int parts = wa.splits + own;
   const int64_t R = (int64_t)a.tokens * a.group, step = R * a.cache.kv_heads;
   const int64_t at = (int64_t)(h / a.group) * R + (int64_t)t * a.group + h % a.group;
-  float mx = -INFINITY;
-  for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, a.part_ml[(at + s * step) * 2]);
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
-  const float base = mx == -INFINITY ? 0.f : mx;
-  v4f y = {0, 0, 0, 0};
-  float sum = 0;
   const int d = 4 * lane;
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const v2f ml = *reinterpret_cast<const v2f*>(a.part_ml + (at + s * step) * 2);
-    const float f = exp2_fast(ml[0] - base);
-    sum = fmaf(ml[1], f, sum);
-    if (d < a.dim) {
-      const v4f x = *reinterpret_cast<const v4f*>(a.part_o + (at + s * step) * a.dim + d);
-      y += f > 0.f ? x * f : v4f{0, 0, 0, 0};
+  const bool in = d < a.dim;
+  const float* po = a.part_o + at * a.dim + (in ? d : 0);
+  float mx = -INFINITY, sum = 0;
+  v4f y = {0, 0, 0, 0};
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const int n = min(64, parts - s0);
+    v2f ml = {-INFINITY, 0};
+    if (lane < n) ml = *reinterpret_cast<const v2f*>(a.part_ml + (at + (s0 + lane) * step) * 2);
+    float top = ml[0];
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+    top = fmaxf(top, mx);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float f = exp2_fast(ml[0] - base), before = exp2_fast(mx - base);
+    float l = ml[1] * f;
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k, 64);
+    sum = fmaf(sum, before, l);
+    y *= before;
+    mx = top;
+    for (int s = 0; s < n; s += 8) {
+      v4f x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const v4f*>(po + (s0 + min(s + i, n - 1)) * step * a.dim);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float fi = as_f(__builtin_amdgcn_readlane(as_u(f), (s + i) & 63));  // (past the parts: 0)
+        if (s + i < n && fi > 0.f) y += x[i] * fi;
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (d < a.dim) store4<T>(a, (int64_t)t * a.out_token + (int64_t)h * a.out_head, d, y * inv);
+  if (in) store4<T>(a, (int64_t)t * a.out_token + (int64_t)h * a.out_head, d, y * inv);
   if (a.lse != nullptr && lane == 0) a.lse[(int64_t)t * a.heads + h] = lse_of(mx, sum, kShift<TC>);
 }
 
-template <int T, int TC, int DP>
-hipError_t launch_part(const AttnArgs& a, const AttnPart& w, bool stacked, hipStream_t s) {
-  const uint32_t items = (uint32_t)((int64_t)w.tiles * a.cache.kv_heads * w.splits * (stacked ? 1 : a.batch));
-  if (w.rows == 16)
-    hipLaunchKernelGGL((k_attn_few<T, TC, DP>), dim3(items), dim3(256), 0, s, a, w, stacked);
-  else if (w.rows == 64)
-    hipLaunchKernelGGL((k_attn_tile<T, TC, DP, 1>), dim3(items), dim3(256), 0, s, a, w, stacked);
-  else if constexpr (T != DQ_F32)
-    hipLaunchKernelGGL((k_attn_tile<T, TC, DP, 2>), dim3(items), dim3(256), 0, s, a, w, stacked);
+template <int T, int TC, int DP, int RS, int RO>
+hipError_t launch_items(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  const int64_t shared = (int64_t)p.shared.tiles * a.cache.kv_heads * p.shared.splits;
+  const int64_t own = (int64_t)p.own.tiles * a.cache.kv_heads * p.own.splits * a.batch;
+  hipLaunchKernelGGL((k_attn<T, TC, DP, RS, RO>), dim3((uint32_t)(shared + own)), dim3(256), 0, s, a, p.shared, p.own,
+                     (int)shared, (int)own);
   return hipGetLastError();
 }
 
 template <int T, int TC, int DP>
 hipError_t launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-  if (p.shared.splits > 0)
-    if (hipError_t e = launch_part<T, TC, DP>(a, p.shared, true, s); e != hipSuccess) return e;
-  if (p.own.splits > 0)
-    if (hipError_t e = launch_part<T, TC, DP>(a, p.own, false, s); e != hipSuccess) return e;
-  if (a.part_o == nullptr) return hipSuccess;
+  const int rs = p.shared.splits > 0 ? p.shared.rows : p.own.rows, ro = p.own.rows;
+  hipError_t e = hipErrorInvalidValue;
+  if (rs == 16 && ro == 16) e = launch_items<T, TC, DP, 16, 16>(a, p, s);
+  if (rs == 64 && ro == 16) e = launch_items<T, TC, DP, 64, 16>(a, p, s);
+  if (rs == 64 && ro == 64) e = launch_items<T, TC, DP, 64, 64>(a, p, s);
+  if constexpr (T != DQ_F32) {
+    if (rs == 128 && ro == 16) e = launch_items<T, TC, DP, 128, 16>(a, p, s);
+    if (rs == 128 && ro == 64) e = launch_items<T, TC, DP, 128, 64>(a, p, s);
+    if (rs == 128 && ro == 128) e = launch_items<T, TC, DP, 128, 128>(a, p, s);
+  }
+  if (e != hipSuccess || a.part_o == nullptr) return e;
   hipLaunchKernelGGL((k_attn_join<T, TC>), dim3((uint32_t)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(256), 0, s, a, p.shared,
                      p.own);
   return hipGetLastError();
