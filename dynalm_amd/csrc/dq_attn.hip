@@ -77,10 +77,12 @@ DQ_DEV void split(float a, float b, u32 (&out)[kParts<T, TC>]) {
   }
 }
 
-// The weights run as 2^(s - m + kShift): f16 weights far below the largest stay normal numbers
-// (2^14 is the largest; what l and O share cancels).
+// The running maximum m of a row moves only when a score passes it by more than kSlack (in powers of
+// two), so that the sums are seldom rescaled; weights run as 2^(s - m + kShift), at most 2^14: f16 weights
+// far below the largest stay normal numbers (what l and O share cancels).
+constexpr float kSlack = 8.f;
 template <int TC>
-constexpr float kShift = TC == DQ_F16 ? 14.f : 0.f;
+constexpr float kShift = TC == DQ_F16 ? 6.f : 0.f;
 
 // C + A . B over a 16 x 16 x 32 tile: lane l supplies row (A) / column (B) l % 16 and K = 8 (l / 16)
 // .. + 7; it holds column l % 16, rows 4 (l / 16) .. + 3 of C.
@@ -130,6 +132,26 @@ DQ_DEV u32 lds_address(const void* p) { return (u32)(uintptr_t)(DQ_LDS(const voi
 DQ_DEV int page_at(const int32_t* pages, int i) {
   return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)pages)[i];
 }
+
+// Where a run of keys lies in its pages: key `key` is place `in` of entry `p` of the page list.
+struct PageWalk {
+  int key, p, in;
+  DQ_DEV void start(int k, int page_size) {
+    key = k;
+    p = k / page_size;
+    in = k - p * page_size;
+  }
+  // `pages` whole pages and `rest` places on
+  DQ_DEV void skip(int keys, int pages, int rest, int page_size) {
+    key += keys;
+    p += pages;
+    in += rest;
+    if (in >= page_size) {
+      in -= page_size;
+      ++p;
+    }
+  }
+};
 
 // ---- infinite and NaN values that only some rows of a tile see ------------
 // A masked key has weight 0, but 0 times an infinite value is NaN in a matrix product. In tiles
@@ -303,24 +325,35 @@ DQ_DEV float load_q(const AttnArgs& a, bool valid, int token, int head, int g, v
   }
 }
 
-// One step of a row's running maximum over N scores a lane (products x, which become weights):
-// returns the factor of what was summed before.
-template <int TC, int N>
-DQ_DEV float softmax_step(float (&x)[N], float c, float& m, float& l) {
-  float mx = -INFINITY;
+DQ_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));  // (fmaxf would quieten each operand first)
+  return r;
+}
+
+// A row's running maximum m and the base that its weights are taken from.
+struct RowMax {
+  float m = -INFINITY, base = 0;
+};
+
+// Whether one of the lane's N products x passes its row's maximum.
+template <int N>
+DQ_DEV bool passes(const float (&x)[N], float c, const RowMax& r, float& mx) {
+  mx = max3(x[0], x[1], x[2]);
 #pragma unroll
-  for (int i = 0; i < N; ++i) mx = fmaxf(mx, x[i]);
-  mx = fmaxf(m, row_max(mx) * c);
-  const float base = mx == -INFINITY ? 0.f : mx - kShift<TC>;
-  const float alpha = m == mx ? 1.f : exp2_fast(m - mx);
-  float sum = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    x[i] = exp2_fast(fmaf(x[i], c, -base));
-    sum += x[i];
-  }
-  l = fmaf(l, alpha, sum);
-  m = mx;
+  for (int i = 3; i + 1 < N; i += 2) mx = max3(mx, x[i], x[i + 1]);
+  if (N % 2 == 0) mx = fmaxf(mx, x[N - 1]);
+  return mx * c > r.m + kSlack;
+}
+// Moves the maximum of the rows that are passed (mx: the lane's largest product) and returns the
+// factor of what was summed before; a row does not move for another.
+template <int TC>
+DQ_DEV float move_max(float mx, float c, RowMax& r) {
+  mx = row_max(mx) * c;
+  if (!(mx > r.m + kSlack)) return 1.f;
+  const float alpha = exp2_fast(r.m - mx);
+  r.m = mx;
+  r.base = mx - kShift<TC>;
   return alpha;
 }
 
@@ -387,7 +420,8 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
   v4u q[NP][DP / 32];
   const float c = load_q<T, TC, DP>(a, valid, token, qh, g, q);
 
-  float m = -INFINITY, l = 0;
+  RowMax rm;
+  float l = 0;
   v4f o[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) o[i] = v4f{0, 0, 0, 0};
@@ -413,18 +447,25 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
   struct Place {
     int id[2], in[2];  // of each half's page: its number, the half's first place
   };
-  auto place = [&](int tile) {
+  PageWalk walk;
+  walk.key = -1;
+  bool walk_pre = true;
+  const int skip_pages = 128 / ca.page_size, skip_rest = 128 % ca.page_size;
+  auto place = [&](int tile) {  // tiles wave, wave + 4, ... in turn
     const bool pre = tile < tiles_p;
     const int32_t* pages = pre ? a.prefix_pages : own_pages;
-    const int kend = pre ? it.pk1 : it.ok1;
-    const int kb = pre ? it.pk0 + tile * 32 : it.ok0 + (tile - tiles_p) * 32;
+    if (walk.key < 0 || walk_pre != pre)
+      walk.start(pre ? it.pk0 + tile * 32 : it.ok0 + (tile - tiles_p) * 32, ca.page_size);
+    else
+      walk.skip(128, skip_pages, skip_rest, ca.page_size);
+    walk_pre = pre;
     Place r;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = t == 0 || kb + 16 < kend ? kb + 16 * t : kb;
-      const int p = key / ca.page_size;
-      r.id[t] = page_at(pages, p);
-      r.in[t] = key - p * ca.page_size;
+    r.id[0] = r.id[1] = page_at(pages, walk.p);
+    r.in[0] = r.in[1] = walk.in;
+    if (walk.key + 16 < (pre ? it.pk1 : it.ok1)) {  // (else the second half's keys do not count)
+      const bool over = walk.in + 16 == ca.page_size;
+      if (over) r.id[1] = page_at(pages, walk.p + 1);
+      r.in[1] = over ? 0 : walk.in + 16;
     }
     return r;
   };
@@ -509,7 +550,18 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
         for (int j = 0; j < 8 * (DP / 32); ++j) r.v[j / (DP / 32)][j % (DP / 32)] = tmp[64 * j];
       }
     }
-    const float alpha = softmax_step<TC, 8>(x, c, m, l);
+    float mx;
+    if (__any(passes<8>(x, c, rm, mx))) {
+      const float alpha = move_max<TC>(mx, c, rm);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i] *= alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = exp2_fast(fmaf(x[j], c, -rm.base));
+      l += x[j];
+    }
     v4u p[NP];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -517,10 +569,6 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       split<T, TC>(x[2 * j], x[2 * j + 1], parts);
 #pragma unroll
       for (int k = 0; k < NP; ++k) p[k][j] = parts[k];
-    }
-    if (__any(alpha != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) o[i] *= alpha;
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -539,12 +587,12 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
     Place next;
     if (tile < tiles) {
       load(place(tile), r0);
-      next = place(min(tile + 4, tiles - 1));
+      if (tile + 4 < tiles) next = place(tile + 4);
     }
     auto step = [&](KvRegs<DP>& cur, KvRegs<DP>& other) {
       if (tile + 4 < tiles) {
         load(next, other);
-        next = place(min(tile + 8, tiles - 1));
+        if (tile + 8 < tiles) next = place(tile + 8);
       }
       compute(tile, cur);
       tile += 4;
@@ -560,7 +608,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
     for (; tile < tiles; tile += 4) {
       KvRegs<DP> r;
       load(next, r);
-      next = place(min(tile + 4, tiles - 1));
+      if (tile + 4 < tiles) next = place(tile + 4);
       compute(tile, r);
     }
   }
@@ -568,7 +616,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
   // the waves' sums join in LDS
   l = row_sum(l);
   if (g == 0) {
-    s_ml[wave][n][0] = m;
+    s_ml[wave][n][0] = rm.m;
     s_ml[wave][n][1] = l;
   }
 #pragma unroll
@@ -665,7 +713,9 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   const int wr = wave * 16 * RT;  // the wave's first row of the tile
   const int wrows = min(max(it.count - wr, 0), 16 * RT);
   int own_lim[RT];
-  float c[RT], m[RT], l[RT];
+  float c[RT];
+  RowMax rm[RT];
+  float l[RT];
   v4u q[RT][NP][DP / 32];
   v4f o[RT][NC];
 #pragma unroll
@@ -675,7 +725,6 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     const int token = row / a.group;
     own_lim[t] = valid ? own_limit(a, it, token) : 0;
     c[t] = load_q<T, TC, DP>(a, valid, token, it.head * a.group + row % a.group, g, q[t]);
-    m[t] = -INFINITY;
     l[t] = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[t][i] = v4f{0, 0, 0, 0};
@@ -692,13 +741,15 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   const int tiles_p = (it.pk1 - it.pk0 + KT - 1) / KT;
   const int tiles = tiles_p + max(0, (it.ok1 - it.ok0 + KT - 1) / KT);
 
-  // Chunk places of this lane's loads and reads (swizzle_k and swizzle_v repeat every 16 keys).
+  // This lane's loads of a whole tile and its reads (swizzle_k and swizzle_v repeat every 16 keys).
   const int lrow = lane / CH;
-  u32 kpos[KW / KI], vpos[KW / KI];
+  auto kpos = [&](int i) { return (u32)((lane % CH) ^ swizzle_k<DP>(wave * KW + i * KI + lrow)) * 16; };
+  auto vpos = [&](int i) { return (u32)((lane % CH) ^ swizzle_v<DP>(wave * KW + i * KI + lrow)) * 16; };
+  u32 kload[KW / KI], vload[KW / KI];
 #pragma unroll
   for (int i = 0; i < KW / KI; ++i) {
-    kpos[i] = ((lane % CH) ^ swizzle_k<DP>(wave * KW + i * KI + lrow)) * 16;
-    vpos[i] = ((lane % CH) ^ swizzle_v<DP>(wave * KW + i * KI + lrow)) * 16;
+    kload[i] = (i * KI + lrow) * token_bytes + kpos(i);
+    vload[i] = (i * KI + lrow) * token_bytes + vpos(i);
   }
   u32 kread[DP / 32], vread[NC];
 #pragma unroll
@@ -709,19 +760,24 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
 
   // The wave's keys of a tile lie in one page; its number is read one tile ahead of the loads.
   struct Place {
-    int in, start, id, last;
+    int id, in, last;  // the page, the wave's first place of it, and the last place that counts after that
   };
-  auto place = [&](int tile) {
+  PageWalk walk;
+  walk.key = -1;
+  bool walk_pre = true;
+  const int skip_pages = KT / ca.page_size, skip_rest = KT % ca.page_size;
+  auto place = [&](int tile) {  // the tiles in turn
     const bool pre = tile < tiles_p;
+    const int32_t* pages = pre ? a.prefix_pages : own_pages;
     const int kend = pre ? it.pk1 : it.ok1;
-    const int kb = (pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT) + wave * KW;
-    Place r;
-    r.in = min(kb, kend - 1);  // (past the keys the last one is loaded again)
-    const int p = r.in / ca.page_size;
-    r.start = p * ca.page_size;
-    r.id = page_at(pre ? a.prefix_pages : own_pages, p);
-    r.last = kend - 1 - r.in;
-    return r;
+    if (walk.key < 0 || walk_pre != pre)
+      walk.start((pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT) + wave * KW, ca.page_size);
+    else
+      walk.skip(KT, skip_pages, skip_rest, ca.page_size);
+    walk_pre = pre;
+    PageWalk at = walk;
+    if (at.key >= kend) at.start(kend - 1, ca.page_size);  // past the keys the last one is loaded again
+    return Place{page_at(pages, at.p), at.in, kend - 1 - at.key};
   };
   const u32 lds_k = lds_address(&s_k[0][wave * KW * DP]), lds_v = lds_address(&s_v[0][wave * KW * DP]);
   auto issue = [&](const Place& r, int buf) {
@@ -730,18 +786,21 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
       bad = true;
       id = 0;
     }
-    const int64_t base = (int64_t)id * ca.page + (int64_t)(r.in - r.start) * ca.token + (int64_t)it.head * ca.head;
+    const int64_t base = (int64_t)id * ca.page + (int64_t)r.in * ca.token + (int64_t)it.head * ca.head;
     const uint16_t *kp = ca.k + base, *vp = ca.v + base;
     const u32 to = buf * KT * DP * 2;
+    if (r.last >= KW - 1 && a.dim == DP) {
 #pragma unroll
-    for (int i = 0; i < KW / KI; ++i) {
-      const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes;
-      if (a.dim == DP) {
-        load_to_lds(kp, at + kpos[i], lds_k + to + i * 1024);
-        load_to_lds(vp, at + vpos[i], lds_v + to + i * 1024);
-      } else {
-        if (kpos[i] < (u32)a.dim * 2) load_to_lds(kp, at + kpos[i], lds_k + to + i * 1024);
-        if (vpos[i] < (u32)a.dim * 2) load_to_lds(vp, at + vpos[i], lds_v + to + i * 1024);
+      for (int i = 0; i < KW / KI; ++i) {
+        load_to_lds(kp, kload[i], lds_k + to + i * 1024);
+        load_to_lds(vp, vload[i], lds_v + to + i * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KW / KI; ++i) {
+        const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes, k = kpos(i), v = vpos(i);
+        if (k < (u32)a.dim * 2) load_to_lds(kp, at + k, lds_k + to + i * 1024);
+        if (v < (u32)a.dim * 2) load_to_lds(vp, at + v, lds_v + to + i * 1024);
       }
     }
   };
@@ -749,14 +808,14 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   Place next = {};
   if (tiles > 0) {
     issue(place(0), 0);
-    next = place(min(1, tiles - 1));
+    if (tiles > 1) next = place(1);
   }
   for (int tile = 0; tile < tiles; ++tile) {
     wait_loads();     // this wave's part of the tile is in LDS
     __syncthreads();  // everyone's is, and the other buffer is read out
     if (tile + 1 < tiles) {
       issue(next, (tile + 1) & 1);
-      next = place(min(tile + 2, tiles - 1));
+      if (tile + 2 < tiles) next = place(tile + 2);
     }
     const bool pre = tile < tiles_p;
     const int kb = pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT;
@@ -816,10 +875,17 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
       for (int u = 0; u < KT / 16; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * u + i] = s[t][u][i];
-      const float alpha = softmax_step<TC, KT / 4>(x, c[t], m[t], l[t]);
-      if (__any(alpha != 1.f)) {
+      float mx;
+      if (__any(passes<KT / 4>(x, c[t], rm[t], mx))) {
+        const float alpha = move_max<TC>(mx, c[t], rm[t]);
+        l[t] *= alpha;
 #pragma unroll
         for (int i = 0; i < NC; ++i) o[t][i] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < KT / 4; ++i) {
+        x[i] = exp2_fast(fmaf(x[i], c[t], -rm[t].base));
+        l[t] += x[i];
       }
 #pragma unroll
       for (int u = 0; u < KT / 8; ++u) {
@@ -868,13 +934,13 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (16 * i + 4 * g < a.dim) store4<T>(a, at, 16 * i + 4 * g, o[t][i] * inv);
-      if (a.lse != nullptr && g == 0) a.lse[(int64_t)token * a.heads + h] = lse_of(m[t], sum, kShift<TC>);
+      if (a.lse != nullptr && g == 0) a.lse[(int64_t)token * a.heads + h] = lse_of(rm[t].m, sum, kShift<TC>);
     } else {
       const int64_t at = part + row;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (16 * i + 4 * g < a.dim) *reinterpret_cast<v4f*>(a.part_o + at * a.dim + 16 * i + 4 * g) = o[t][i];
-      if (g == 0) *reinterpret_cast<v2f*>(a.part_ml + at * 2) = v2f{m[t], sum};
+      if (g == 0) *reinterpret_cast<v2f*>(a.part_ml + at * 2) = v2f{rm[t].m, sum};
     }
   }
   if (noting) {  // the infinite and NaN values go to what has just been written
@@ -925,9 +991,14 @@ union AttnLds<DP, 16> {
 template <int T, int TC, int DP, int RS, int RO>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
-  const int b = blockIdx.x;
+  // Eight of one kind (one for each XCD), eight of the other, while both last: a CU has a shared item,
+  // which computes, beside an own one, which reads.
+  const int pairs = min(shared, own) / 8, b = blockIdx.x;
+  const bool mixed = b < 16 * pairs;
+  const bool stacked = mixed ? (b >> 3 & 1) == 0 : b - 8 * pairs < shared;
+  const int of = mixed ? (b >> 4) * 8 + (b & 7) : stacked ? b - 8 * pairs : b - shared;
+  const int index = xcd_item(of, stacked ? shared : own);
   if constexpr (RS == RO) {
-    const bool stacked = b < shared;
     AttnPart w;
     w.tiles = stacked ? ws.tiles : wo.tiles;
     w.splits = stacked ? ws.splits : wo.splits;
@@ -936,12 +1007,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, Att
     w.own_from = wo.own_from;
     w.with_prefix = wo.with_prefix;
     w.backward = wo.backward;
-    run_item<T, TC, DP, RS>(a, w, stacked, stacked ? xcd_item(b, shared) : xcd_item(b - shared, own), sh);
+    run_item<T, TC, DP, RS>(a, w, stacked, index, sh);
+  } else if (stacked) {
+    run_item<T, TC, DP, RS>(a, ws, true, index, sh);
   } else {
-    if (b < shared)
-      run_item<T, TC, DP, RS>(a, ws, true, xcd_item(b, shared), sh);
-    else
-      run_item<T, TC, DP, RO>(a, wo, false, xcd_item(b - shared, own), sh);
+    run_item<T, TC, DP, RO>(a, wo, false, index, sh);
   }
 }
 

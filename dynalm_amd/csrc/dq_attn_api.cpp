@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdlib>
 
 #include "../../include/dynaq.h"
 #include "dq_attn.h"
@@ -155,7 +156,8 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workgroups that run at once: two on each of the 256 CUs.
-constexpr int64_t kWorkgroups = 512;
+const int64_t kWorkgroups = getenv("SHT") ? atoi(getenv("SHT")) : 512;
+const int64_t kOwnT = getenv("OWT") ? atoi(getenv("OWT")) : 512;const int64_t kShL = getenv("SHL") ? atoi(getenv("SHL")) : 256;const int64_t kOwL = getenv("OWL") ? atoi(getenv("OWL")) : 256;
 
 // Ranges of `keys` keys for `items` row tiles: as many as fill the card, of at least `least` keys.
 void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target, int64_t least) {
@@ -187,16 +189,16 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
     if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && target > 0) {
       p.shared.rows = tile(all);
       p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
-      split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, target, 256);
+      split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, target, kShL);
       if (a->max_len > 0) {
-        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, target, 256);
+        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, kOwnT, kOwL);
         p.own.slot = p.shared.splits;
       }
     } else {
       p.own.with_prefix = a->prefix_len > 0;
       p.own.own_from = (int32_t)(ceil_div(a->prefix_len, 128) * 128);
       const int64_t items = a->batch * p.own.tiles * c->kv_heads;
-      split_keys(&p.own, items, p.own.own_from + a->max_len, target > 0 ? target : 1, 256);
+      split_keys(&p.own, items, p.own.own_from + a->max_len, target > 0 ? target : 1, kOwL);
     }
     const int64_t slots = p.shared.splits + p.own.splits;
     p.slots = slots > 1 ? slots : 0;
