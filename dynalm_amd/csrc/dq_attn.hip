@@ -731,7 +731,6 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   }
   // own keys that the wave's first and last row see, and the item's first
   const int own_least = wrows > 0 ? own_limit(a, it, (it.first + wr) / a.group) : 0;
-  const int own_most = wrows > 0 ? own_limit(a, it, (it.first + wr + wrows - 1) / a.group) : 0;
   const int item_least = own_limit(a, it, it.first / a.group);
   bool bad = false, noting = false;
 
@@ -780,48 +779,99 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     return Place{page_at(pages, at.p), at.in, kend - 1 - at.key};
   };
   const u32 lds_k = lds_address(&s_k[0][wave * KW * DP]), lds_v = lds_address(&s_v[0][wave * KW * DP]);
-  auto issue = [&](const Place& r, int buf) {
+  auto issue = [&](const Place& r, bool values, int buf) {
     int id = r.id;
     if ((u32)id >= (u32)ca.n_pages) {
       bad = true;
       id = 0;
     }
-    const int64_t base = (int64_t)id * ca.page + (int64_t)r.in * ca.token + (int64_t)it.head * ca.head;
-    const uint16_t *kp = ca.k + base, *vp = ca.v + base;
-    const u32 to = buf * KT * DP * 2;
+    const uint16_t* from = (values ? ca.v : ca.k) + ((int64_t)id * ca.page + (int64_t)r.in * ca.token + (int64_t)it.head * ca.head);
+    const u32 to = (values ? lds_v : lds_k) + buf * KT * DP * 2;
     if (r.last >= KW - 1 && a.dim == DP) {
 #pragma unroll
-      for (int i = 0; i < KW / KI; ++i) {
-        load_to_lds(kp, kload[i], lds_k + to + i * 1024);
-        load_to_lds(vp, vload[i], lds_v + to + i * 1024);
-      }
+      for (int i = 0; i < KW / KI; ++i) load_to_lds(from, values ? vload[i] : kload[i], to + i * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < KW / KI; ++i) {
-        const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes, k = kpos(i), v = vpos(i);
-        if (k < (u32)a.dim * 2) load_to_lds(kp, at + k, lds_k + to + i * 1024);
-        if (v < (u32)a.dim * 2) load_to_lds(vp, at + v, lds_v + to + i * 1024);
+        const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes, pos = values ? vpos(i) : kpos(i);
+        if (pos < (u32)a.dim * 2) load_to_lds(from, at + pos, to + i * 1024);
       }
     }
   };
+  auto first_key = [&](int tile) { return tile < tiles_p ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT; };
 
+  // S^T of a tile
+  auto scores = [&](const uint16_t* sk, v4f (&s)[RT][KT / 16]) {
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+      for (int u = 0; u < KT / 16; ++u) {
+        const v4u kf = *reinterpret_cast<const v4u*>(sk + kread[e] + 16 * u * DP);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if (e == 0) s[t][u] = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) s[t][u] = mma<TC>(kf, q[t][p][e], s[t][u]);
+        }
+      }
+  };
+  // One pair of weights of scores whose maxima have been looked at.
+  auto weigh = [&](const v4f (&s)[RT][KT / 16], int pair, u32 (&pw)[RT][NP][KT / 32][4]) {
+    const int t = pair / (KT / 8), u = pair % (KT / 8) / 2, i = pair % 2 * 2;
+    const float x0 = exp2_fast(fmaf(s[t][u][i], c[t], -rm[t].base));
+    const float x1 = exp2_fast(fmaf(s[t][u][i + 1], c[t], -rm[t].base));
+    l[t] += x0;
+    l[t] += x1;
+    u32 parts[NP];
+    split<T, TC>(x0, x1, parts);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) pw[t][p][u / 2][u % 2 * 2 + i / 2] = parts[p];
+  };
+  auto key_operand = [&](const uint16_t* sk, int i) {
+    return *reinterpret_cast<const v4u*>(sk + kread[i / (KT / 16)] + i % (KT / 16) * 16 * DP);
+  };
+  auto value_operand = [&](const uint16_t* sv, int i) {
+    v4u x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v2u z = __builtin_bit_cast(
+          v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((DQ_LDS(v4s)*)(sv + vread[i % NC] + (i / NC * 32 + 16 * h) * DP)));
+      x[2 * h] = z[0];
+      x[2 * h + 1] = z[1];
+    }
+    return x;
+  };
+
+  // Keys run one tile before values: while a tile's weights are computed, which is vector work,
+  // the matrix cores form the next tile's scores.
+  v4f s[RT][KT / 16];
   Place next = {};
   if (tiles > 0) {
-    issue(place(0), 0);
-    if (tiles > 1) next = place(1);
+    Place first = place(0);
+    issue(first, false, 0);
+    wait_loads();
+    __syncthreads();
+    issue(first, true, 0);
+    if (tiles > 1) {
+      next = place(1);
+      issue(next, false, 1);
+    }
+    scores(s_k[0], s);
   }
   for (int tile = 0; tile < tiles; ++tile) {
-    wait_loads();     // this wave's part of the tile is in LDS
-    __syncthreads();  // everyone's is, and the other buffer is read out
+    wait_loads();     // this wave's part of the tile's values and of the next one's keys is in LDS
+    __syncthreads();  // everyone's is, and the other buffers are read out
     if (tile + 1 < tiles) {
-      issue(next, (tile + 1) & 1);
-      if (tile + 2 < tiles) next = place(tile + 2);
+      issue(next, true, (tile + 1) & 1);
+      if (tile + 2 < tiles) {
+        next = place(tile + 2);
+        issue(next, false, tile & 1);
+      }
     }
     const bool pre = tile < tiles_p;
-    const int kb = pre ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT;
+    const int kb = first_key(tile);
     const int least = wrows == 0 ? 0 : pre ? it.pk1 : own_least;
-    const int most = wrows == 0 ? 0 : pre ? it.pk1 : own_most;
-    const uint16_t* sk = s_k[tile & 1];
+    const uint16_t* sk = s_k[(tile + 1) & 1];
     uint16_t* sv = s_v[tile & 1];
 
     if (kb + KT > (pre ? it.pk1 : item_least)) {  // some row sees the tile in part
@@ -840,26 +890,10 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
         __syncthreads();
       }
     }
-    if (kb >= most) continue;  // (the wave's rows see none of it)
-
-    v4f s[RT][KT / 16];
-#pragma unroll
-    for (int u = 0; u < KT / 16; ++u) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) s[t][u] = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < DP / 32; ++e) {
-        const v4u kf = *reinterpret_cast<const v4u*>(sk + kread[e] + 16 * u * DP);
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p) s[t][u] = mma<TC>(kf, q[t][p][e], s[t][u]);
-      }
-    }
     if (kb + KT > least) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const int lim = pre ? it.pk1 : own_lim[t];
+        const int lim = wrows == 0 ? 0 : pre ? it.pk1 : own_lim[t];
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u)
 #pragma unroll
@@ -867,52 +901,56 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
             if (kb + 16 * u + 4 * g + i >= lim) s[t][u][i] = -INFINITY;
       }
     }
-    u32 pw[RT][NP][KT / 32][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      float x[KT / 4];
+      float x[KT / 4], mx;
 #pragma unroll
-      for (int u = 0; u < KT / 16; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * u + i] = s[t][u][i];
-      float mx;
+      for (int i = 0; i < KT / 4; ++i) x[i] = s[t][i / 4][i % 4];
       if (__any(passes<KT / 4>(x, c[t], rm[t], mx))) {
         const float alpha = move_max<TC>(mx, c[t], rm[t]);
         l[t] *= alpha;
 #pragma unroll
         for (int i = 0; i < NC; ++i) o[t][i] *= alpha;
       }
+    }
+    // The order below is kept (sched_barrier): operands are read kAhead steps before their products, and
+    // the vector work of the weights goes between the products of the next tile's scores.
+    constexpr int F = KT * DP / 512, kAhead = 4, kPairs = RT * KT / 8;
+    u32 pw[RT][NP][KT / 32][4];
+    v4f ahead[RT][KT / 16];  // (after the last tile of what the buffer holds: not used)
+    v4u ring[kAhead];
 #pragma unroll
-      for (int i = 0; i < KT / 4; ++i) {
-        x[i] = exp2_fast(fmaf(x[i], c[t], -rm[t].base));
-        l[t] += x[i];
+    for (int i = 0; i < kAhead; ++i) ring[i] = key_operand(sk, i);
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int e = i / (KT / 16), u = i % (KT / 16);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        if (e == 0) ahead[t][u] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p) ahead[t][u] = mma<TC>(ring[i % kAhead], q[t][p][e], ahead[t][u]);
       }
+      ring[i % kAhead] = i + kAhead < F ? key_operand(sk, i + kAhead) : value_operand(sv, i + kAhead - F);
 #pragma unroll
-      for (int u = 0; u < KT / 8; ++u) {
-        u32 parts[NP];
-        split<T, TC>(x[2 * u], x[2 * u + 1], parts);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) pw[t][p][u / 4][u % 4] = parts[p];
-      }
+      for (int k = i * kPairs / F; k < (i + 1) * kPairs / F; ++k) weigh(s, k, pw);
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int u = 0; u < KT / 32; ++u)
+    for (int i = 0; i < F; ++i) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        v4u vt;
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const v2u z = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                    (DQ_LDS(v4s)*)(sv + vread[i] + (32 * u + 16 * h) * DP)));
-          vt[2 * h] = z[0];
-          vt[2 * h + 1] = z[1];
+        for (int p = NP - 1; p >= 0; --p) {
+          const u32(&w4)[4] = pw[t][p][i / NC];
+          o[t][i % NC] = mma<TC>(ring[i % kAhead], v4u{w4[0], w4[1], w4[2], w4[3]}, o[t][i % NC]);
         }
+      if (i + kAhead < F) ring[i % kAhead] = value_operand(sv, i + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int p = NP - 1; p >= 0; --p)
-            o[t][i] = mma<TC>(vt, v4u{pw[t][p][u][0], pw[t][p][u][1], pw[t][p][u][2], pw[t][p][u][3]}, o[t][i]);
-      }
+      for (int u = 0; u < KT / 16; ++u) s[t][u] = ahead[t][u];
   }
   if (bad) s_bad = 1;
   __syncthreads();
