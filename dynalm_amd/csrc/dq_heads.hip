@@ -2,8 +2,13 @@
 // values to a paged cache with both on the way.
 //
 // A head row is D <= 256 values: y = x / sqrt(mean x^2 + eps) * w, then the first 2 * half of
-// them turn in pairs, a' = a c - b s, b' = b c + a s. One wave a row: every value is read once
-// and written once.
+// them turn in pairs, a' = a c - b s, b' = b c + a s. Every value is read once and written once: the
+// bytes are the bound, the launch for a few tokens.
+//
+// Rows that can be read in 16 bytes take up to 16 lanes each, a lane two chunks of 8 values that hold both
+// values of its pairs (chunks j and j + half / 8 for halves, 2j and 2j + 1 for neighbours), so
+// that nothing but the sum of squares crosses lanes; a lane's cosines, sines and weights serve several heads of its token
+// (k_heads). Other rows take a wave each, value by value (k_norm_rope, k_kv_append).
 #include <type_traits>
 
 #include "dq_attn.h"
@@ -112,6 +117,209 @@ __global__ __launch_bounds__(256) void k_kv_append(int64_t tokens, int dim, Head
     if (lane + 64 * j < dim) store1<TC>(is_v ? c.v : c.k, at + lane + 64 * j, y[j]);
 }
 
+template <int T>
+DQ_DEV void load8(const void* p, int64_t i, float (&v)[8]) {
+  if constexpr (T == DQ_F32) {
+    const v4u* q = reinterpret_cast<const v4u*>(static_cast<const float*>(p) + i);
+    const v4u a = q[0], b = q[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = as_f(a[k]), v[4 + k] = as_f(b[k]);
+  } else {
+    const v4u a = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = T == DQ_F16 ? h2f(a[k]) : as_f(a[k] << 16);
+      v[2 * k + 1] = T == DQ_F16 ? h2f(a[k] >> 16) : as_f(a[k] & 0xFFFF0000u);
+    }
+  }
+}
+template <bool kStream>
+DQ_DEV void store16(v4u* p, v4u x) {
+  if constexpr (kStream)
+    __builtin_nontemporal_store(x, p);
+  else
+    *p = x;
+}
+template <int T, bool kStream>
+DQ_DEV void store8(void* p, int64_t i, const float (&v)[8]) {
+  if constexpr (T == DQ_F32) {
+    v4u* q = reinterpret_cast<v4u*>(static_cast<float*>(p) + i);
+    store16<kStream>(q, v4u{as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])});
+    store16<kStream>(q + 1, v4u{as_u(v[4]), as_u(v[5]), as_u(v[6]), as_u(v[7])});
+  } else {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    v4u a;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const v2f x = {v[2 * k], v[2 * k + 1]};
+      a[k] = T == DQ_F16 ? __builtin_bit_cast(u32, __builtin_convertvector(x, v2h))
+                         : __builtin_bit_cast(u32, __builtin_convertvector(x, v2b));
+    }
+    store16<kStream>(reinterpret_cast<v4u*>(static_cast<uint16_t*>(p) + i), a);
+  }
+}
+
+// Heads of one token that a lane group takes: a, then b. N heads a group: their cosines, sines and
+// weights are read once, and their loads are under way together.
+template <int TI, int TO, int N, bool kAppend, bool kStream>
+__global__ __launch_bounds__(256) void k_heads(int64_t tokens, int dim, int lanes_log2, HeadRows a, HeadRows b, CacheArgs c,
+                                               const int64_t* slots, float eps, RopeArgs rp) {
+  const int lanes = 1 << lanes_log2, j = threadIdx.x & (lanes - 1);
+  const u32 group = blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  const u32 na = (a.heads + N - 1) / N, nb = (b.heads + N - 1) / N;
+  const int64_t t = group / (na + nb);
+  if (t >= tokens) return;
+  const u32 part = group % (na + nb);
+  const bool second = part >= na;
+  const int heads = second ? b.heads : a.heads, h0 = (second ? part - na : part) * N;
+  const float* w = second ? b.weight : a.weight;
+  const char* in = static_cast<const char*>(second ? b.in : a.in);
+  const int64_t in_at = t * (second ? b.in_token : a.in_token), in_head = second ? b.in_head : a.in_head;
+  void* out = kAppend ? (void*)(second ? c.v : c.k) : second ? b.out : a.out;
+  int64_t out_at = t * (second ? b.out_token : a.out_token), out_head = second ? b.out_head : a.out_head;
+  if constexpr (kAppend) {
+    const int64_t slot = slots[t];
+    if (slot < 0 || slot >= c.n_pages * c.page_size) return;
+    out_at = slot / c.page_size * c.page + slot % c.page_size * c.token;
+    out_head = c.head;
+  }
+  const int half = kAppend && second ? 0 : rp.half;  // (values are not rotated)
+  // the lane's chunks
+  const int chunks = dim / 8, turned = half / 8;
+  int ca, cb;
+  if (rp.pairs || half == 0) {
+    ca = 2 * j;
+    cb = 2 * j + 1;
+  } else if (j < turned) {
+    ca = j;
+    cb = j + turned;
+  } else {
+    ca = 2 * j;  // (2 turned chunks before the first such lane's)
+    cb = 2 * j + 1;
+  }
+  const bool has_a = ca < chunks, has_b = cb < chunks;
+  const bool turn_a = 8 * ca < 2 * half, turn_b = 8 * cb < 2 * half;
+
+  float x[N][2][8];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int64_t at = in_at + min(h0 + n, heads - 1) * in_head;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[n][0][i] = x[n][1][i] = 0;
+    if (has_a) load8<TI>(in, at + 8 * ca, x[n][0]);
+    if (has_b) load8<TI>(in, at + 8 * cb, x[n][1]);
+  }
+  float cs[8], sn[8];  // of the lane's pairs 8 j .. + 7
+#pragma unroll
+  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+  if (turn_a) {
+    const int64_t pos = rp.positions[t];
+    if (pos >= 0 && pos < rp.max_pos) {
+      const v4u* pc = reinterpret_cast<const v4u*>(rp.cos + pos * half + 8 * j);
+      const v4u* ps = reinterpret_cast<const v4u*>(rp.sin + pos * half + 8 * j);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k == 1 && !turn_b) break;
+        const v4u qc = pc[k], qs = ps[k];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[4 * k + i] = as_f(qc[i]), sn[4 * k + i] = as_f(qs[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < 4 || turn_b) cs[i] = sn[i] = __builtin_nanf("");
+    }
+  }
+  if (w != nullptr) {
+    float wa[8], wb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wa[i] = wb[i] = 0;
+    if (has_a) load8<DQ_F32>(w, 8 * ca, wa);
+    if (has_b) load8<DQ_F32>(w, 8 * cb, wb);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      float s = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(x[n][0][i], x[n][0][i], fmaf(x[n][1][i], x[n][1][i], s));
+      for (int m = lanes >> 1; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+      const float r = 1.f / sqrtf(s / (float)dim + eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[n][0][i] = x[n][0][i] * r * wa[i];
+        x[n][1][i] = x[n][1][i] * r * wb[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (h0 + n >= heads) break;
+    if (turn_a) {
+      if (rp.pairs) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (k == 1 && !turn_b) break;
+            const float p = x[n][k][2 * i], q = x[n][k][2 * i + 1];
+            x[n][k][2 * i] = p * cs[4 * k + i] - q * sn[4 * k + i];
+            x[n][k][2 * i + 1] = q * cs[4 * k + i] + p * sn[4 * k + i];
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = x[n][0][i], q = x[n][1][i];
+          x[n][0][i] = p * cs[i] - q * sn[i];
+          x[n][1][i] = q * cs[i] + p * sn[i];
+        }
+      }
+    }
+    const int64_t at = out_at + (h0 + n) * out_head;
+    if (has_a) store8<TO, kStream>(out, at + 8 * ca, x[n][0]);
+    if (has_b) store8<TO, kStream>(out, at + 8 * cb, x[n][1]);
+  }
+}
+
+bool aligned16(const void* p, int type, int64_t s0, int64_t s1) {
+  const int64_t v = type == DQ_F32 ? 4 : 8;
+  return (uintptr_t)p % 16 == 0 && s0 % v == 0 && s1 % v == 0;
+}
+// Whether a launch's rows, tables and weights can be read and written in 16 bytes, and no chunk of 8
+// values holds turned and other ones.
+bool in_chunks(int in_type, int out_type, const HeadRows& a, const HeadRows& b, const RopeArgs& rp) {
+  for (const HeadRows* r : {&a, &b})
+    if (!aligned16(r->in, in_type, r->in_token, r->in_head) || !aligned16(r->out, out_type, r->out_token, r->out_head) ||
+        (uintptr_t)r->weight % 16 != 0)
+      return false;
+  return rp.half == 0 || (rp.half % (rp.pairs ? 4 : 8) == 0 && ((uintptr_t)rp.cos | (uintptr_t)rp.sin) % 16 == 0);
+}
+
+// Heads a lane group takes: two once that leaves enough groups for every CU, one below, where latency
+// counts; outputs past what the L2s hold (32 MB) are written around them. 8,192 tokens of 40 bf16 heads of 128
+// (172 MB moved): 44.0 us with one head, 43.9 with two, 51.6 with four, 61.3 with eight; with
+// streaming stores 37.3 (4.6 TB/s) and 41.4 with two and four. 16,384 tokens of 8 + 8 heads appended
+// (143 MB): 32.6, 38.4, 39.7, 41.7, and 29.4 (4.85 TB/s) and 31.1. A copy of 1 GiB reaches 4.8 TB/s.
+template <int TI, int TO, bool kAppend>
+hipError_t launch_heads(int64_t tokens, int dim, const HeadRows& a, const HeadRows& b, const CacheArgs& c,
+                        const int64_t* slots, float eps, const RopeArgs& rope, hipStream_t s) {
+  int log2 = 0;
+  while ((16 << log2) < dim) ++log2;
+  const int per = 256 >> log2;
+  const int64_t rows = tokens * (a.heads + b.heads);
+  const bool many = rows >= 1 << 15, stream = many && rows * dim * (TO == DQ_F32 ? 4 : 2) >= 32 << 20;
+  const int n = many ? 2 : 1;
+  const int64_t groups = tokens * ((a.heads + n - 1) / n + (b.heads + n - 1) / n);
+  const dim3 grid((uint32_t)((groups + per - 1) / per)), block(256);
+  if (stream)
+    hipLaunchKernelGGL((k_heads<TI, TO, 2, kAppend, true>), grid, block, 0, s, tokens, dim, log2, a, b, c, slots, eps, rope);
+  else if (many)
+    hipLaunchKernelGGL((k_heads<TI, TO, 2, kAppend, false>), grid, block, 0, s, tokens, dim, log2, a, b, c, slots, eps, rope);
+  else
+    hipLaunchKernelGGL((k_heads<TI, TO, 1, kAppend, false>), grid, block, 0, s, tokens, dim, log2, a, b, c, slots, eps, rope);
+  return hipGetLastError();
+}
+
 template <class F>
 hipError_t by_type(int type, F&& f) {
   switch (type) {
@@ -121,13 +329,21 @@ hipError_t by_type(int type, F&& f) {
   }
 }
 
+template <class F>
+hipError_t by_cache_type(int type, F&& f) {
+  if (type == DQ_F16) return f(std::integral_constant<int, DQ_F16>{});
+  return f(std::integral_constant<int, DQ_BF16>{});
+}
+
 }  // namespace
 
 hipError_t launch_norm_rope(int in_type, int out_type, int64_t tokens, int dim, const HeadRows& a, const HeadRows& b,
                             float eps, const RopeArgs& rope, hipStream_t s) {
   const int64_t blocks = (tokens * (a.heads + b.heads) + 3) / 4;
+  const bool chunks = in_chunks(in_type, out_type, a, b, rope);
   return by_type(in_type, [&](auto ti) {
     return by_type(out_type, [&](auto to) {
+      if (chunks) return launch_heads<ti(), to(), false>(tokens, dim, a, b, CacheArgs{}, nullptr, eps, rope, s);
       hipLaunchKernelGGL((k_norm_rope<ti(), to()>), dim3((uint32_t)blocks), dim3(256), 0, s, tokens, dim, a, b, eps,
                          rope);
       return hipGetLastError();
@@ -139,8 +355,10 @@ hipError_t launch_kv_append(int in_type, int cache_type, int64_t tokens, int dim
                             const CacheArgs& cache, const int64_t* slots, float eps, const RopeArgs& rope,
                             hipStream_t s) {
   const int64_t blocks = (tokens * 2 * cache.kv_heads + 3) / 4;
+  const bool chunks = in_chunks(in_type, cache_type, k, v, rope);  // (the cache's places are 16-byte aligned always)
   return by_type(in_type, [&](auto ti) {
-    return by_type(cache_type, [&](auto tc) {
+    return by_cache_type(cache_type, [&](auto tc) {
+      if (chunks) return launch_heads<ti(), tc(), true>(tokens, dim, k, v, cache, slots, eps, rope, s);
       hipLaunchKernelGGL((k_kv_append<ti(), tc()>), dim3((uint32_t)blocks), dim3(256), 0, s, tokens, dim, k, v, cache,
                          slots, eps, rope);
       return hipGetLastError();
