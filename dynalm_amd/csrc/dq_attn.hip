@@ -121,6 +121,28 @@ DQ_DEV void load_to_lds(const void* base, u32 off, u32 lds) {
       : "s"(lds), "v"(off), "s"(base)
       : "memory");
 }
+// The same for N rows of 1,024 bytes of LDS in one go: load i is offset by 1,024 i on both sides (off[i] leaves
+// that out).
+template <int N>
+DQ_DEV void load_rows_to_lds(const void* base, const u32 (&off)[N], u32 lds) {
+  static_assert(N == 2 || N == 4);
+  u32 m0;
+  if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+        "global_load_lds_dwordx4 %3, %4 offset:1024\n\ts_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %6\n\t"
+        "global_load_lds_dwordx4 %3, %6 offset:1024\n\tglobal_load_lds_dwordx4 %4, %6 offset:2048\n\t"
+        "global_load_lds_dwordx4 %5, %6 offset:3072\n\ts_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
+        : "memory");
+}
 DQ_DEV void wait_loads() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -747,8 +769,8 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   u32 kload[KW / KI], vload[KW / KI];
 #pragma unroll
   for (int i = 0; i < KW / KI; ++i) {
-    kload[i] = (i * KI + lrow) * token_bytes + kpos(i);
-    vload[i] = (i * KI + lrow) * token_bytes + vpos(i);
+    kload[i] = (i * KI + lrow) * token_bytes + kpos(i) - 1024 * i;  // (a whole tile's rows are 1,024 bytes apart at least)
+    vload[i] = (i * KI + lrow) * token_bytes + vpos(i) - 1024 * i;
   }
   u32 kread[DP / 32], vread[NC];
 #pragma unroll
@@ -779,25 +801,33 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     return Place{page_at(pages, at.p), at.in, kend - 1 - at.key};
   };
   const u32 lds_k = lds_address(&s_k[0][wave * KW * DP]), lds_v = lds_address(&s_v[0][wave * KW * DP]);
-  auto issue = [&](const Place& r, bool values, int buf) {
+  struct Source {
+    int64_t base;  // of the wave's first key
+    int last;
+  };
+  const int64_t head_at = (int64_t)it.head * ca.head;
+  auto resolve = [&](const Place& r) {
     int id = r.id;
     if ((u32)id >= (u32)ca.n_pages) {
       bad = true;
       id = 0;
     }
-    const uint16_t* from = (values ? ca.v : ca.k) + ((int64_t)id * ca.page + (int64_t)r.in * ca.token + (int64_t)it.head * ca.head);
-    const u32 to = (values ? lds_v : lds_k) + buf * KT * DP * 2;
+    return Source{(int64_t)id * ca.page + (int64_t)r.in * ca.token + head_at, r.last};
+  };
+  auto issue = [&](const uint16_t* pool, const Source& r, const u32 (&off)[KW / KI], auto pos_of, u32 to) {
+    const uint16_t* from = pool + r.base;
     if (r.last >= KW - 1 && a.dim == DP) {
-#pragma unroll
-      for (int i = 0; i < KW / KI; ++i) load_to_lds(from, values ? vload[i] : kload[i], to + i * 1024);
+      load_rows_to_lds(from, off, to);
     } else {
 #pragma unroll
       for (int i = 0; i < KW / KI; ++i) {
-        const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes, pos = values ? vpos(i) : kpos(i);
+        const u32 at = (u32)min(i * KI + lrow, r.last) * token_bytes, pos = pos_of(i);
         if (pos < (u32)a.dim * 2) load_to_lds(from, at + pos, to + i * 1024);
       }
     }
   };
+  auto issue_keys = [&](const Source& r, int buf) { issue(ca.k, r, kload, kpos, lds_k + buf * KT * DP * 2); };
+  auto issue_values = [&](const Source& r, int buf) { issue(ca.v, r, vload, vpos, lds_v + buf * KT * DP * 2); };
   auto first_key = [&](int tile) { return tile < tiles_p ? it.pk0 + tile * KT : it.ok0 + (tile - tiles_p) * KT; };
 
   // S^T of a tile
@@ -845,28 +875,31 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   // Keys run one tile before values: while a tile's weights are computed, which is vector work,
   // the matrix cores form the next tile's scores.
   v4f s[RT][KT / 16];
-  Place next = {};
+  Source next = {};   // the next tile's
+  Place after = {};   // and where the one after it lies
   if (tiles > 0) {
-    Place first = place(0);
-    issue(first, false, 0);
+    const Place p0 = place(0);
+    const Place p1 = tiles > 1 ? place(1) : p0;
+    if (tiles > 2) after = place(2);
+    const Source first = resolve(p0);
+    next = resolve(p1);
+    issue_keys(first, 0);
+    issue_values(first, 0);
+    if (tiles > 1) issue_keys(next, 1);
     wait_loads();
     __syncthreads();
-    issue(first, true, 0);
-    if (tiles > 1) {
-      next = place(1);
-      issue(next, false, 1);
-    }
     scores(s_k[0], s);
   }
   for (int tile = 0; tile < tiles; ++tile) {
-    wait_loads();     // this wave's part of the tile's values and of the next one's keys is in LDS
-    __syncthreads();  // everyone's is, and the other buffers are read out
-    if (tile + 1 < tiles) {
-      issue(next, true, (tile + 1) & 1);
-      if (tile + 2 < tiles) {
-        next = place(tile + 2);
-        issue(next, false, tile & 1);
-      }
+    if (tile > 0) {
+      wait_loads();     // this wave's part of the tile's values and of the next one's keys is in LDS
+      __syncthreads();  // everyone's is, and the other buffers are read out
+    }
+    if (tile + 1 < tiles) issue_values(next, (tile + 1) & 1);
+    if (tile + 2 < tiles) {
+      next = resolve(after);
+      issue_keys(next, tile & 1);
+      if (tile + 3 < tiles) after = place(tile + 3);
     }
     const bool pre = tile < tiles_p;
     const int kb = first_key(tile);
@@ -1029,13 +1062,11 @@ union AttnLds<DP, 16> {
 template <int T, int TC, int DP, int RS, int RO>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
-  // Eight of one kind (one for each XCD), eight of the other, while both last: a CU has a shared item,
-  // which computes, beside an own one, which reads.
-  const int pairs = min(shared, own) / 8, b = blockIdx.x;
-  const bool mixed = b < 16 * pairs;
-  const bool stacked = mixed ? (b >> 3 & 1) == 0 : b - 8 * pairs < shared;
-  const int of = mixed ? (b >> 4) * 8 + (b & 7) : stacked ? b - 8 * pairs : b - shared;
-  const int index = xcd_item(of, stacked ? shared : own);
+  // The shared items first: one for each CU (the plan makes no more where it can), so that a CU has a
+  // shared item, which computes, beside own ones, which read.
+  const int b = blockIdx.x;
+  const bool stacked = b < shared;
+  const int index = stacked ? xcd_item(b, shared) : xcd_item(b - shared, own);
   if constexpr (RS == RO) {
     AttnPart w;
     w.tiles = stacked ? ws.tiles : wo.tiles;

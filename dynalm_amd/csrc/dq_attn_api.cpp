@@ -187,7 +187,7 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
     p.own.backward = true;
     // The prefix with all sequences' rows, unless one sequence's rows fill tiles by themselves.
     if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && target > 0) {
-      p.shared.rows = tile(all);
+      p.shared.rows = getenv("SHR") ? atoi(getenv("SHR")) : tile(all);
       p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
       split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, target, kShL);
       if (a->max_len > 0) {
