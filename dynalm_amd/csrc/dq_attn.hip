@@ -886,10 +886,11 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     issue_keys(first, 0);
     issue_values(first, 0);
     if (tiles > 1) issue_keys(next, 1);
-    wait_loads();
-    __syncthreads();
-    scores(s_k[0], s);
   }
+  // (waits outside the branch, so that the compiler sees q's loads end here and adds no wait to the loop)
+  wait_loads();
+  __syncthreads();
+  if (tiles > 0) scores(s_k[0], s);
   for (int tile = 0; tile < tiles; ++tile) {
     if (tile > 0) {
       wait_loads();     // this wave's part of the tile's values and of the next one's keys is in LDS
