@@ -250,6 +250,7 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   it.b = b;
   const int lo = a.q_offsets != nullptr ? a.q_offsets[b] : b;
   const int hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
+  const int len = a.max_len > 0 ? a.lens[b] : 0;  // (all three under way together)
   // (whatever the offsets hold, rows stay inside the tensors)
   const int first = min(max(lo, 0), a.tokens);
   const int n = min(min(max(hi, first), a.tokens) - first, a.max_q);
@@ -257,7 +258,7 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   it.count = min(tile, n * a.group - tt * tile);
   if (it.count <= 0) return false;
   it.first = first * a.group + tt * tile;
-  it.len = a.max_len > 0 ? min(max(a.lens[b], 0), a.max_len) : 0;
+  it.len = min(max(len, 0), a.max_len);
   it.token0 = first;
   it.own0 = it.len - n + 1;
   if (w.with_prefix) {  // prefix, then (from the next whole chunk unit on) own keys
@@ -288,50 +289,56 @@ DQ_DEV int first_row(const AttnArgs& a, const Item& it, int key) {
   return max(0, (it.token0 + key + 1 - it.own0) * a.group - it.first);
 }
 
-// The query fragments of rows: lane l has row l % 16 and, of every 32 values, 8 (l / 16) .. + 7. Returns
+// The query fragments of rows: lane l has row l % 16 and, of every 32 values, 8 (l / 16) .. + 7. First their loads,
+// then, once other loads are under way too, the operands; the latter returns
 // the factor from products to scores in powers of two: fp32 rows are scaled to a largest value
 // in [2^14, 2^15), where all of their parts are normal numbers.
-template <int T, int TC, int DP>
-DQ_DEV float load_q(const AttnArgs& a, bool valid, int token, int head, int g, v4u (&q)[kParts<T, TC>][DP / 32]) {
+template <int T, int DP>
+struct RawQ {
+  v4u x[DP / 32][T == DQ_F32 ? 2 : 1];
+};
+template <int T, int DP>
+DQ_DEV void load_q(const AttnArgs& a, bool valid, int token, int head, int g, RawQ<T, DP>& r) {
   const int64_t base = (int64_t)token * a.q_token + (int64_t)head * a.q_head;
-  if constexpr (T != DQ_F32) {
-    const uint16_t* p = static_cast<const uint16_t*>(a.q) + base;
 #pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-      const int d = 32 * s + 8 * g;
+  for (int s = 0; s < DP / 32; ++s) {
+    const int d = 32 * s + 8 * g;
+#pragma unroll
+    for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) {
       v4u x = {0, 0, 0, 0};
       if (valid && d < a.dim) {
-        if (a.q_vec)
-          x = *reinterpret_cast<const v4u*>(p + d);
-        else
+        if constexpr (T == DQ_F32) {
+          const float* p = static_cast<const float*>(a.q) + base + d + 4 * k;
+          if (a.q_vec)
+            x = *reinterpret_cast<const v4u*>(p);
+          else
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = (u32)p[d + 2 * i] | ((u32)p[d + 2 * i + 1] << 16);
-      }
-      q[0][s] = x;
-    }
-    return a.scale_log2;
-  } else {
-    const float* p = static_cast<const float*>(a.q) + base;
-    float x[DP / 32][8];
-    float most = 0;
-#pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-      const int d = 32 * s + 8 * g;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[s][i] = 0;
-      if (valid && d < a.dim) {
-        if (a.q_vec) {
-          const v4f lo = *reinterpret_cast<const v4f*>(p + d), hi = *reinterpret_cast<const v4f*>(p + d + 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[s][i] = lo[i], x[s][4 + i] = hi[i];
+            for (int i = 0; i < 4; ++i) x[i] = as_u(p[i]);
         } else {
+          const uint16_t* p = static_cast<const uint16_t*>(a.q) + base + d;
+          if (a.q_vec)
+            x = *reinterpret_cast<const v4u*>(p);
+          else
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[s][i] = p[d + i];
+            for (int i = 0; i < 4; ++i) x[i] = (u32)p[2 * i] | ((u32)p[2 * i + 1] << 16);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[s][i]));
+      r.x[s][k] = x;
     }
+  }
+}
+template <int T, int TC, int DP>
+DQ_DEV float q_operands(const AttnArgs& a, const RawQ<T, DP>& r, v4u (&q)[kParts<T, TC>][DP / 32]) {
+  if constexpr (T != DQ_F32) {
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) q[0][s] = r.x[s][0];
+    return a.scale_log2;
+  } else {
+    float most = 0;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(as_f(r.x[s][i / 4][i % 4])));
     most = row_max(most);
     const int e = most > 0 && most < INFINITY ? 15 - (__builtin_amdgcn_frexp_expf(most)) : 0;
 #pragma unroll
@@ -339,7 +346,7 @@ DQ_DEV float load_q(const AttnArgs& a, bool valid, int token, int head, int g, v
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         u32 parts[kParts<T, TC>];
-        split<T, TC>(ldexpf(x[s][2 * i], e), ldexpf(x[s][2 * i + 1], e), parts);
+        split<T, TC>(ldexpf(as_f(r.x[s][i / 2][i % 2 * 2]), e), ldexpf(as_f(r.x[s][i / 2][i % 2 * 2 + 1]), e), parts);
 #pragma unroll
         for (int k = 0; k < kParts<T, TC>; ++k) q[k][s][i] = parts[k];
       }
@@ -439,8 +446,10 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
   const int token = row / a.group, qh = it.head * a.group + row % a.group;
   const int own_lim = own_limit(a, it, token);
   const int own_least = own_limit(a, it, it.first / a.group);
+  RawQ<T, DP> raw;
+  load_q<T, DP>(a, valid, token, qh, g, raw);
   v4u q[NP][DP / 32];
-  const float c = load_q<T, TC, DP>(a, valid, token, qh, g, q);
+  float c = 1.f;
 
   RowMax rm;
   float l = 0;
@@ -611,6 +620,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       load(place(tile), r0);
       if (tile + 4 < tiles) next = place(tile + 4);
     }
+    c = q_operands<T, TC, DP>(a, raw, q);
     auto step = [&](KvRegs<DP>& cur, KvRegs<DP>& other) {
       if (tile + 4 < tiles) {
         load(next, other);
@@ -626,12 +636,19 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
     }
   } else {
     Place next;
-    if (tile < tiles) next = place(tile);
-    for (; tile < tiles; tile += 4) {
-      KvRegs<DP> r;
-      load(next, r);
+    KvRegs<DP> r;
+    if (tile < tiles) {
+      load(place(tile), r);
       if (tile + 4 < tiles) next = place(tile + 4);
+    }
+    c = q_operands<T, TC, DP>(a, raw, q);
+    while (tile < tiles) {
       compute(tile, r);
+      tile += 4;
+      if (tile < tiles) {
+        load(next, r);
+        if (tile + 4 < tiles) next = place(tile + 4);
+      }
     }
   }
 
@@ -738,6 +755,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   float c[RT];
   RowMax rm[RT];
   float l[RT];
+  RawQ<T, DP> raw[RT];
   v4u q[RT][NP][DP / 32];
   v4f o[RT][NC];
 #pragma unroll
@@ -746,7 +764,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     const int row = it.first + (valid ? wr + 16 * t + n : 0);
     const int token = row / a.group;
     own_lim[t] = valid ? own_limit(a, it, token) : 0;
-    c[t] = load_q<T, TC, DP>(a, valid, token, it.head * a.group + row % a.group, g, q[t]);
+    load_q<T, DP>(a, valid, token, it.head * a.group + row % a.group, g, raw[t]);
     l[t] = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[t][i] = v4f{0, 0, 0, 0};
@@ -887,6 +905,8 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     issue_values(first, 0);
     if (tiles > 1) issue_keys(next, 1);
   }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) c[t] = q_operands<T, TC, DP>(a, raw[t], q[t]);
   // (waits outside the branch, so that the compiler sees q's loads end here and adds no wait to the loop)
   wait_loads();
   __syncthreads();
@@ -1109,13 +1129,30 @@ DQ_DEV int find_seq(const AttnArgs& a, int t, int lane) {
   return lo >= 1 && lo <= a.batch ? lo - 1 : -1;
 }
 
-// Weights of up to 64 parts at a time lie one to a lane; their sums of v are read 8 at a time.
+// Weights of up to 64 parts at a time lie one to a lane; their sums of v are read 8 at a time, the first 8 before
+// anything is known of the row (a part that was not written is not used).
 template <int T, int TC>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, AttnPart wb) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   const int t = uniform((int)(id / a.heads)), h = uniform((int)(id % a.heads));
   if (t >= a.tokens) return;
+  const int64_t R = (int64_t)a.tokens * a.group, step = R * a.cache.kv_heads;
+  const int64_t at = (int64_t)(h / a.group) * R + (int64_t)t * a.group + h % a.group;
+  const int d = 4 * lane, most = wa.splits + wb.splits;
+  const bool in = d < a.dim;
+  const float* po = a.part_o + at * a.dim + (in ? d : 0);
+  v4f x[8];
+  v2f ml = {-INFINITY, 0};
+  auto read = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const v4f*>(po + min(s0 + i, most - 1) * step * a.dim);
+  };
+  auto read_ml = [&](int s0) {
+    if (s0 + lane < most) ml = *reinterpret_cast<const v2f*>(a.part_ml + (at + (s0 + lane) * step) * 2);
+  };
+  read_ml(0);
+  read(0);
   const int b = find_seq(a, t, lane);
   if (b < 0) return;
   // the own parts that were written: those that begin inside the sequence, and the first
@@ -1123,36 +1160,29 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, Attn
   const int end = wb.with_prefix ? (len > 0 ? wb.own_from + len : a.prefix_len) : len;
   const int own = wb.splits > 0 ? min(wb.splits, max(1, (end + wb.chunk - 1) / wb.chunk)) : 0;
   const int parts = wa.splits + own;
-  const int64_t R = (int64_t)a.tokens * a.group, step = R * a.cache.kv_heads;
-  const int64_t at = (int64_t)(h / a.group) * R + (int64_t)t * a.group + h % a.group;
-  const int d = 4 * lane;
-  const bool in = d < a.dim;
-  const float* po = a.part_o + at * a.dim + (in ? d : 0);
   float mx = -INFINITY, sum = 0;
   v4f y = {0, 0, 0, 0};
   for (int s0 = 0; s0 < parts; s0 += 64) {
     const int n = min(64, parts - s0);
-    v2f ml = {-INFINITY, 0};
-    if (lane < n) ml = *reinterpret_cast<const v2f*>(a.part_ml + (at + (s0 + lane) * step) * 2);
-    float top = ml[0];
+    if (s0 > 0) read_ml(s0);
+    const bool counts = lane < n;
+    float top = counts ? ml[0] : -INFINITY;
 #pragma unroll
     for (int k = 32; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
     top = fmaxf(top, mx);
     const float base = top == -INFINITY ? 0.f : top;
-    const float f = exp2_fast(ml[0] - base), before = exp2_fast(mx - base);
-    float l = ml[1] * f;
+    const float f = counts ? exp2_fast(ml[0] - base) : 0.f, before = exp2_fast(mx - base);
+    float l = counts ? ml[1] * f : 0.f;
 #pragma unroll
     for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k, 64);
     sum = fmaf(sum, before, l);
     y *= before;
     mx = top;
     for (int s = 0; s < n; s += 8) {
-      v4f x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const v4f*>(po + (s0 + min(s + i, n - 1)) * step * a.dim);
+      if (s0 + s > 0) read(s0 + s);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float fi = as_f(__builtin_amdgcn_readlane(as_u(f), (s + i) & 63));  // (past the parts: 0)
+        const float fi = as_f(__builtin_amdgcn_readlane(as_u(f), (s + i) & 63));
         if (s + i < n && fi > 0.f) y += x[i] * fi;
       }
     }

@@ -156,7 +156,7 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workgroups that run at once: two on each of the 256 CUs.
-const int64_t kWorkgroups = getenv("SHT") ? atoi(getenv("SHT")) : 512;
+const int64_t kWorkgroups = getenv("SHT") ? atoi(getenv("SHT")) : 256;
 const int64_t kOwnT = getenv("OWT") ? atoi(getenv("OWT")) : 512;const int64_t kShL = getenv("SHL") ? atoi(getenv("SHL")) : 256;const int64_t kOwL = getenv("OWL") ? atoi(getenv("OWL")) : 256;
 
 // Ranges of `keys` keys for `items` row tiles: as many as fill the card, of at least `least` keys.
