@@ -164,13 +164,12 @@ def _check(rc: int) -> None:
 
 def _ptr(x) -> int | None:
     """Device pointer of a torch tensor / int / None."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
+    try:
         return x.data_ptr()
-    raise TypeError(f"expected a device pointer, got {type(x)!r}")
+    except AttributeError:
+        raise TypeError(f"expected a device pointer, got {type(x)!r}") from None
 
 
 def row_bytes(dtype: int, k: int) -> int:
@@ -356,7 +355,7 @@ class KvCache(C.Structure):
 
 class Attention(C.Structure):
     """dq_attention: one shared_attention call."""
-    _fields_ = [("q", C.POINTER(Heads)), ("out", C.POINTER(Heads)), ("lse", _P), ("tokens", _I64), ("batch", _I64),
+    _fields_ = [("q", _P), ("out", _P), ("lse", _P), ("tokens", _I64), ("batch", _I64),
                 ("q_offsets", _P), ("max_q", _I64), ("prefix_pages", _P), ("prefix_len", _I64), ("pages", _P),
                 ("pages_stride", _I64), ("lens", _P), ("max_len", _I64), ("scale", C.c_float)]
 
@@ -382,7 +381,7 @@ def kv_append(cache: KvCache, tokens: int, k: Heads, v: Heads, slots, k_weight=N
 
 def _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
                max_len, scale) -> Attention:
-    return Attention(C.pointer(q) if q is not None else None, C.pointer(out) if out is not None else None, _ptr(lse), tokens, batch, _ptr(q_offsets), max_q, _ptr(prefix_pages),
+    return Attention(_ref(q), _ref(out), _ptr(lse), tokens, batch, _ptr(q_offsets), max_q, _ptr(prefix_pages),
                      prefix_len, _ptr(pages), pages_stride, _ptr(lens), max_len, scale)
 
 

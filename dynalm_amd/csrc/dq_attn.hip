@@ -27,6 +27,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 
 #define DQ_LDS(T) __attribute__((address_space(3))) T
 
@@ -554,18 +555,22 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       for (int i = 0; i < 4; ++i) x[4 * t + i] = acc[i];
     }
     if (kb + 32 > least || kb + 32 > kend) {
-      bool nf = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
         x[j] = key < lim && key < kend ? x[j] : -INFINITY;
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) {
+        for (int e = 0; e < DP / 32; ++e)
           if (key >= kend) r.v[j][e] = 0;  // places past the keys may hold anything
-          nf |= nonfinite<TC>(r.v[j][e]);
-        }
       }
-      if (__any(nf)) {
+    }
+    if (kb + 32 > least && least < kend) {  // some row does not see all of the tile's keys
+      v2us top = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(v2us, r.v[j][e] & 0x7FFF7FFFu));
+      if (__any(top[0] >= kExp<TC> || top[1] >= kExp<TC>)) {
         if (lane == 0) s_noted = 1;
         u32* tmp = reinterpret_cast<u32*>(&s_o[wave][0][0]) + lane;
 #pragma unroll
@@ -1083,11 +1088,13 @@ union AttnLds<DP, 16> {
 template <int T, int TC, int DP, int RS, int RO>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
-  // The shared items first: one for each CU (the plan makes no more where it can), so that a CU has a
-  // shared item, which computes, beside own ones, which read.
-  const int b = blockIdx.x;
-  const bool stacked = b < shared;
-  const int index = stacked ? xcd_item(b, shared) : xcd_item(b - shared, own);
+  // On every XCD a shared item for each of its 32 CUs, then an own one for each, and so on while both
+  // last: a CU has a shared item, which computes, beside an own one, which reads.
+  const int pairs = min(shared, own) / 256, b = blockIdx.x, turn = b / 256;
+  const bool mixed = turn < 2 * pairs;
+  const bool stacked = mixed ? turn % 2 == 0 : b - 256 * pairs < shared;
+  const int of = mixed ? turn / 2 * 256 + b % 256 : stacked ? b - 256 * pairs : b - shared;
+  const int index = xcd_item(of, stacked ? shared : own);
   if constexpr (RS == RO) {
     AttnPart w;
     w.tiles = stacked ? ws.tiles : wo.tiles;
