@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <cstdlib>
 
 #include "../../include/dynaq.h"
 #include "dq_attn.h"
@@ -137,15 +136,19 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
                          a->q->dtype, a->out->dtype, c->dtype);
   if (a->q->heads != a->out->heads || a->q->heads % c->kv_heads != 0)
     return dq::set_error(DQ_INVALID_ARGUMENT, "%d query heads, %d of out, %d kv heads", a->q->heads, a->out->heads, c->kv_heads);
-  if (int rc = check_tokens(a->tokens, a->q->heads); rc != DQ_OK) return rc;
   if (c->token_stride > (1 << 25)) return dq::set_error(DQ_UNSUPPORTED, "cache: token_stride %lld", (ll)c->token_stride);
-  if (a->batch > INT32_MAX - 1 || a->tokens > INT32_MAX / 2) return dq::set_error(DQ_UNSUPPORTED, "batch %lld, tokens %lld", (ll)a->batch, (ll)a->tokens);
-  if (a->max_q < 1 || a->max_q > INT32_MAX / 2) return dq::set_error(DQ_INVALID_ARGUMENT, "max_q %lld", (ll)a->max_q);
+  // Head rows and work items are counted in 32 bits.
+  if (a->tokens > ((int64_t)1 << 30) / a->q->heads)
+    return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %d heads are too many", (ll)a->tokens, a->q->heads);
+  if (a->max_q < 1) return dq::set_error(DQ_INVALID_ARGUMENT, "max_q %lld", (ll)a->max_q);
+  const int64_t most_q = a->max_q < a->tokens ? a->max_q : a->tokens;
+  if (a->batch > INT32_MAX / 2 / a->q->heads || a->batch * (most_q * (a->q->heads / c->kv_heads) / 16 + 1) > INT32_MAX / 2 / c->kv_heads)
+    return dq::set_error(DQ_UNSUPPORTED, "%lld sequences of up to %lld tokens are too many", (ll)a->batch, (ll)a->max_q);
   if (data && a->q_offsets == nullptr && (a->tokens != a->batch || a->max_q != 1))
     return bad("without q_offsets every sequence has one token");
-  const int64_t most = (int64_t)1 << 30;
+  const int64_t most = (int64_t)1 << 29;
   if (a->prefix_len < 0 || a->prefix_len > most || a->max_len < 0 || a->max_len > most)
-    return dq::set_error(DQ_INVALID_ARGUMENT, "prefix_len %lld, max_len %lld", (ll)a->prefix_len, (ll)a->max_len);
+    return dq::set_error(DQ_INVALID_ARGUMENT, "prefix_len %lld, max_len %lld: 0..2^29 keys", (ll)a->prefix_len, (ll)a->max_len);
   if (a->pages_stride < (a->max_len + c->page_size - 1) / c->page_size || a->pages_stride > most)
     return dq::set_error(DQ_INVALID_ARGUMENT, "pages_stride %lld: max_len %lld needs %lld pages", (ll)a->pages_stride, (ll)a->max_len,
                          (ll)((a->max_len + c->page_size - 1) / c->page_size));
@@ -155,14 +158,20 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Workgroups that run at once: two on each of the 256 CUs.
-const int64_t kWorkgroups = getenv("SHT") ? atoi(getenv("SHT")) : 256;
-const int64_t kOwnT = getenv("OWT") ? atoi(getenv("OWT")) : 512;const int64_t kShL = getenv("SHL") ? atoi(getenv("SHL")) : 256;const int64_t kOwL = getenv("OWL") ? atoi(getenv("OWL")) : 256;
+// Items a launch aims at: two run on each of the 256 CUs at once. Shared ones take the rows of the whole
+// batch and compute for long, own ones beside them read: one shared item for each CU. 64 sequences, 32 / 8
+// bf16 heads of 128, 8,192 shared and up to 512 own keys: 256 shared items 46.8 us, 384 50.7, 512 52.4, 1,024
+// 52.4; 128 sequences, 32 / 4 heads, 32,768 and up to 2,048 keys: 137, 140, 140, 156. Own items of 512
+// against 1,024: 52.4 and 55.1, 140 and 151 (more ranges are more parts to write and to join).
+constexpr int64_t kSharedItems = 256, kOwnItems = 512;
+// Keys that are worth an item of their own (128: 20.2 us against 19.3 on 32 short sequences, 15.9 against
+// 16.4 on 7).
+constexpr int64_t kLeastKeys = 256;
 
-// Ranges of `keys` keys for `items` row tiles: as many as fill the card, of at least `least` keys.
-void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target, int64_t least) {
+// Ranges of `keys` keys for `items` row tiles: as many as bring the items to `target`, of kLeastKeys keys at least.
+void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target) {
   int64_t n = target / items;
-  n = n < ceil_div(keys, least) ? n : ceil_div(keys, least);
+  n = n < ceil_div(keys, kLeastKeys) ? n : ceil_div(keys, kLeastKeys);
   n = n > 1 ? n : 1;
   p->chunk = (int32_t)(ceil_div(ceil_div(keys, n), 128) * 128);
   if (p->chunk == 0) p->chunk = 128;
@@ -180,25 +189,25 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
   const bool f32 = a->q->dtype == DQ_F32;
   auto tile = [&](int64_t n) { return n <= 16 ? 16 : n <= 64 || f32 ? 64 : 128; };
   dq::AttnPlan p;
-  for (int64_t target = kWorkgroups;; target /= 2) {
+  for (int less = 0;; ++less) {  // (fewer parts where they would not fit the workspace; at last none)
     p = dq::AttnPlan{};
     p.own.rows = tile(rows);
     p.own.tiles = (int32_t)ceil_div(rows, p.own.rows);
     p.own.backward = true;
     // The prefix with all sequences' rows, unless one sequence's rows fill tiles by themselves.
-    if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && target > 0) {
-      p.shared.rows = getenv("SHR") ? atoi(getenv("SHR")) : tile(all);
+    if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && (kSharedItems >> less) > 0) {
+      p.shared.rows = tile(all);
       p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
-      split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, target, kShL);
+      split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, kSharedItems >> less);
       if (a->max_len > 0) {
-        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, kOwnT, kOwL);
+        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, kOwnItems >> less);
         p.own.slot = p.shared.splits;
       }
     } else {
       p.own.with_prefix = a->prefix_len > 0;
       p.own.own_from = (int32_t)(ceil_div(a->prefix_len, 128) * 128);
       const int64_t items = a->batch * p.own.tiles * c->kv_heads;
-      split_keys(&p.own, items, p.own.own_from + a->max_len, target > 0 ? target : 1, kOwL);
+      split_keys(&p.own, items, p.own.own_from + a->max_len, kOwnItems >> less);
     }
     const int64_t slots = p.shared.splits + p.own.splits;
     p.slots = slots > 1 ? slots : 0;
@@ -226,7 +235,7 @@ dq::AttnArgs attn_args(const dq_kv_cache* c, const dq_attention* a) {
   r.dim = c->head_dim;
   r.tokens = (int32_t)a->tokens;
   r.batch = (int32_t)a->batch;
-  r.max_q = (int32_t)a->max_q;
+  r.max_q = (int32_t)(a->max_q < a->tokens ? a->max_q : a->tokens);
   r.q_offsets = a->q_offsets;
   r.prefix_pages = a->prefix_pages;
   r.pages = a->pages;

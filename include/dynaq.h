@@ -476,7 +476,7 @@ DQ_API int dq_qk_norm_rope(int64_t tokens, int64_t head_dim, const dq_heads* q, 
                            const float* q_weight, const dq_heads* k, const dq_heads* k_out, const float* k_weight,
                            float eps, const dq_rope* rope, const int32_t* positions, void* stream);
 
-/* A paged cache of keys and values of one layer: place i of page p of head h is the head_dim
+/* A paged cache of keys and values of one layer: place i of page p and head h is the head_dim
  * values from k (v) + p * page_stride + i * token_stride + h * head_stride (strides in values:
  * any order of pages, places and heads; multiples of 8, as k and v are 16-byte aligned). The
  * memory is the caller's. */
@@ -519,7 +519,8 @@ DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads
  * overlap q.
  * The prefix is read once for the whole batch, not once a sequence. A row's bits depend on the call's shape (batch, tokens,
  * max_q, prefix_len, max_len), not on timing. Rows outside every sequence are not written.
- * A row that would read a page number outside [0, n_pages) gets NaN.
+ * A row that would read a page number outside [0, n_pages) gets NaN; so may rows of its sequence beside it (all
+ * rows, for a page of the prefix).
  * workspace: dq_shared_attention_workspace bytes of device memory (16-byte aligned) that the call may overwrite; its
  * contents need not be kept. */
 typedef struct dq_attention {

@@ -102,6 +102,13 @@ def test_attention_refusals():
     refused("unsupported", attend, q=heads(dtype=dq.F16), out=heads())
     refused("unsupported", attend, q=heads(dtype=dq.BF16), out=heads(dtype=dq.BF16))
     refused(bad, attend, c=cache(page_size=8))
+    refused(bad, attend, c=cache(n_pages=0))
+    refused(bad, attend, workspace=None)
+    refused(bad, attend, workspace=AT + 8)
+    refused("resource_exhausted", attend, workspace_bytes=1000)
+    refused("unsupported", attend, c=cache(token_stride=1 << 26))
+    refused("unsupported", attend, tokens=1 << 29, batch=1, max_q=1)
+    refused("unsupported", attend, batch=1 << 30)
 
 
 def test_workspace_needs_no_pointers_and_has_a_bound():

@@ -49,6 +49,11 @@ NORM_ROPE = [
     (6, 2, 2, 128, 0, True, True, "f32", "f32", False, 0),
     (6, 2, 2, 128, 0, True, False, "f32", "bf16", False, 0),
     (1027, 16, 4, 128, 128, True, True, "bf16", "bf16", False, 1024),
+    # two heads a lane group (an odd number of heads among them), and outputs past 32 MB
+    (2500, 13, 3, 64, 32, True, True, "f32", "bf16", False, 8),
+    (7001, 5, 1, 72, 64, False, True, "f16", "f16", False, 0),
+    (9000, 13, 2, 128, 128, True, True, "bf16", "bf16", False, 256),
+    (2300, 13, 2, 256, 128, False, True, "f32", "f32", False, 0),
 ]
 
 
@@ -112,6 +117,7 @@ APPEND = [
     (45, 3, 72, 72, True, False, "bf16", "f16", 80, False, True),
     (513, 4, 64, 64, False, False, "f16", "bf16", 256, True, False),
     (19, 2, 200, 0, True, True, "f32", "f16", 16, False, False),
+    (6000, 3, 96, 48, False, True, "bf16", "bf16", 48, True, False),
 ]
 
 
@@ -138,12 +144,11 @@ def test_append(cuda, tokens, hk, dim, rot, halves, norm, ti, tc, page, heads_fi
                  pos.cuda() if rot else None, stream())
     want_k, bound = B.norm_rope(k.cpu(), w, 1e-5, tables, pos, rot, halves)
     kept = torch.ones(pages * page, dtype=torch.bool)
-    for t in range(tokens):
-        s = int(slots[t])
-        if 0 <= s < pages * page:
-            kept[s] = False
-            B.close(kc[s // page, s % page], want_k[t], bound[t], tc)
-            assert torch.equal(vc[s // page, s % page].cpu(), v[t].cpu().to(B.TYPES[tc]))
+    inside = (slots >= 0) & (slots < pages * page)
+    at = slots[inside]
+    kept[at] = False
+    B.close(kc.cpu()[at // page, at % page], want_k[inside], bound[inside], tc)
+    assert torch.equal(vc.cpu()[at // page, at % page], v.cpu()[inside].to(B.TYPES[tc]))
     for new, old in zip((kc.cpu(), vc.cpu()), before):
         assert torch.equal(new.reshape(pages * page, hk, dim)[kept], old.reshape(pages * page, hk, dim)[kept])
 
@@ -240,6 +245,10 @@ SHAPES = [
     pytest.param([4, 6], [2, 3], 0, 2, 1, 128, 16, False, id="rows that see nothing"),
     pytest.param([70, 33], [70, 200], 50, 4, 2, 128, 16, True, id="prompts behind a prefix"),
     pytest.param([131], [131], 0, 3, 1, 200, 32, False, id="one prompt"),
+    pytest.param([1], [77], 1300, 8, 2, 128, 16, False, id="one sequence behind a prefix"),
+    pytest.param([3], [3], 1023, 15, 3, 96, 48, False, id="one sequence, no own keys before"),
+    pytest.param([40], [300], 900, 4, 2, 256, 32, True, id="one prompt behind a prefix"),
+    pytest.param([6, 2, 5], [700, 2, 300], 260, 10, 2, 128, 64, True, id="own keys in several ranges"),
     pytest.param([64, 1, 17], [64, 500, 17], 100, 8, 8, 64, 64, True, id="prompts and a decode step"),
 ]
 
@@ -330,6 +339,20 @@ def test_attention_gives_the_same_bits_again(cuda, new, lens, prefix):
     first = call(c)
     for _ in range(4):
         assert torch.equal(call(c), first)
+
+
+def test_attention_more_rows_than_the_workspace_holds(cuda):
+    """Parts of 4,100 sequences would take over 128 MB: every sequence then takes the prefix itself."""
+    n, dim = 4100, 256
+    c = build(37, [1] * n, [1 + i % 3 for i in range(n)], 40, 16, 1, dim, "bf16", "bf16", 16)
+    cache, q = B.kv_cache(c["kc"], c["vc"]), B.heads(c["q"])
+    assert dq.shared_attention_workspace(cache, q, q, n, n, 1, 40, 3, 3) == 0
+    assert dq.shared_attention_workspace(cache, q, q, n - 1000, n - 1000, 1, 40, 3, 3) == 2 * (n - 1000) * 16 * (dim + 2) * 4
+    out = call(c)
+    some = list(range(0, n, 97))
+    want, _, bound, _ = B.attention(c["q"].cpu()[some], [c["ks"][i] for i in some], [c["vs"][i] for i in some], [1] * len(some),
+                                    [c["lens"][i] for i in some], 40, c["scale"], "bf16", "bf16")
+    B.close(out[some], want, bound, "bf16")
 
 
 def test_long_cache_offsets(cuda):
