@@ -980,6 +980,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     v4u ring[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ring[i] = key_operand(sk, i);
+    __builtin_amdgcn_s_setprio(1);  // (the other wave of the SIMD is then in its scalar and vector work)
 #pragma unroll
     for (int i = 0; i < F; ++i) {
       const int e = i / (KT / 16), u = i % (KT / 16);
@@ -1006,6 +1007,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
       if (i + kAhead < F) ring[i % kAhead] = value_operand(sv, i + kAhead);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
