@@ -160,13 +160,18 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Items a launch aims at: two run on each of the 256 CUs at once. Shared ones take the rows of the whole
 // batch and compute for long, own ones beside them read: one shared item for each CU. 64 sequences, 32 / 8
-// bf16 heads of 128, 8,192 shared and up to 512 own keys: 256 shared items 46.8 us, 384 50.7, 512 52.4, 1,024
-// 52.4; 128 sequences, 32 / 4 heads, 32,768 and up to 2,048 keys: 137, 140, 140, 156. Own items of 512
-// against 1,024: 52.4 and 55.1, 140 and 151 (more ranges are more parts to write and to join).
+// bf16 heads of 128, 8,192 shared and up to 512 own keys: 128 shared items 54.3 us, 256 44.0, 384 47.6, 512
+// 49.8; 128 sequences, 32 / 4 heads, 32,768 and up to 2,048 keys: 214, 141, 139, 140. Own items of 512
+// against 1,024 on the same: 52.4 and 55.1, 140 and 151 (more ranges are more parts to write and to join).
 constexpr int64_t kSharedItems = 256, kOwnItems = 512;
 // Keys that are worth an item of their own (128: 20.2 us against 19.3 on 32 short sequences, 15.9 against
 // 16.4 on 7).
 constexpr int64_t kLeastKeys = 256;
+
+// Rows times keys (of all kv heads) up to which shared items take 64 rows and not 128: more items, each
+// sooner done. 105 / 128 / 192 / 256 rows on 1,111 / 8,192 / 8,192 / 8,192 keys of 5 / 8 / 8 / 8 heads: 14.1
+// against 16.4, 29.3 against 35.4, 38.0 against 39.1, 43.8 against 46.5 us; 128 rows on 32,768 keys of 8: 57.0 and 53.6.
+constexpr int64_t kSmallShared = 24 << 20;
 
 // Ranges of `keys` keys for `items` row tiles: as many as bring the items to `target`, of kLeastKeys keys at least.
 void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target) {
@@ -196,7 +201,7 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
     p.own.backward = true;
     // The prefix with all sequences' rows, unless one sequence's rows fill tiles by themselves.
     if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && (kSharedItems >> less) > 0) {
-      p.shared.rows = tile(all);
+      p.shared.rows = all > 16 && all * a->prefix_len * c->kv_heads <= kSmallShared ? 64 : tile(all);
       p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
       split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, kSharedItems >> less);
       if (a->max_len > 0) {

@@ -249,6 +249,7 @@ SHAPES = [
     pytest.param([3], [3], 1023, 15, 3, 96, 48, False, id="one sequence, no own keys before"),
     pytest.param([40], [300], 900, 4, 2, 256, 32, True, id="one prompt behind a prefix"),
     pytest.param([6, 2, 5], [700, 2, 300], 260, 10, 2, 128, 64, True, id="own keys in several ranges"),
+    pytest.param([i % 3 for i in range(150)], [i % 3 + i % 40 for i in range(150)], 35, 2, 1, 64, 16, False, id="150 sequences"),
     pytest.param([64, 1, 17], [64, 500, 17], 100, 8, 8, 64, 64, True, id="prompts and a decode step"),
 ]
 
