@@ -616,44 +616,21 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       for (int k = NP - 1; k >= 0; --k) o[i] = mma<TC>(vt, p[k], o[i]);
     }
   };
-  // Two tiles' registers, one loading while the other is used, where the row's operands leave room.
+  // (One tile's registers: two, one loading while the other is used, measured the same.)
   int tile = wave;
-  if constexpr (DP * NP <= 128) {
-    KvRegs<DP> r0, r1;
-    Place next;
+  Place next;
+  KvRegs<DP> r;
+  if (tile < tiles) {
+    load(place(tile), r);
+    if (tile + 4 < tiles) next = place(tile + 4);
+  }
+  c = q_operands<T, TC, DP>(a, raw, q);
+  while (tile < tiles) {
+    compute(tile, r);
+    tile += 4;
     if (tile < tiles) {
-      load(place(tile), r0);
+      load(next, r);
       if (tile + 4 < tiles) next = place(tile + 4);
-    }
-    c = q_operands<T, TC, DP>(a, raw, q);
-    auto step = [&](KvRegs<DP>& cur, KvRegs<DP>& other) {
-      if (tile + 4 < tiles) {
-        load(next, other);
-        if (tile + 8 < tiles) next = place(tile + 8);
-      }
-      compute(tile, cur);
-      tile += 4;
-    };
-    while (tile < tiles) {
-      step(r0, r1);
-      if (tile >= tiles) break;
-      step(r1, r0);
-    }
-  } else {
-    Place next;
-    KvRegs<DP> r;
-    if (tile < tiles) {
-      load(place(tile), r);
-      if (tile + 4 < tiles) next = place(tile + 4);
-    }
-    c = q_operands<T, TC, DP>(a, raw, q);
-    while (tile < tiles) {
-      compute(tile, r);
-      tile += 4;
-      if (tile < tiles) {
-        load(next, r);
-        if (tile + 4 < tiles) next = place(tile + 4);
-      }
     }
   }
 
