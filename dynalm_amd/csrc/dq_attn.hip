@@ -12,6 +12,11 @@
 // `group` query heads times the tokens, so that a key is read once for all of them; the prefix
 // takes the rows of the whole batch together, the own keys those of one sequence. Ranges of a
 // row that run in several items leave (O, m, l) in the workspace and k_attn_join adds them.
+//
+// What bounds it (bf16, head size 128; a copy of 1 GiB reaches 4.8 TB/s here, a matrix product of 8,192^3
+// 1,150 to 1,190 TFLOP/s): the bytes of the keys and values where rows are few, the matrix cores and the vector
+// unit, which share their issue slots, where they are many; the launch and one chain of dependent reads (offsets,
+// page numbers, keys: 7 us) where both are few.
 #include <type_traits>
 
 #include "dq_attn.h"
@@ -410,7 +415,9 @@ DQ_DEV float lse_of(float m, float l, float shift) {
 // the end: a decode step's own keys, where a tile of 16 rows is mostly empty and the keys' bytes
 // are all that counts. Keys and values go straight from memory to registers: a lane's 16 bytes of a key
 // are its A operand as they lie; of the values it takes DP / 16 of 8 keys, which v_perm turns into
-// the operands of DP / 16 tiles.
+// the operands of DP / 16 tiles. Bound by the reads: 128 sequences of up to 2,048 own keys, 4 kv heads of 128
+// (403 MB), 81 us, 4.95 TB/s; 64 of up to 512, 8 kv heads (100 MB), 22 us; a tile of 64 rows in their place
+// 50.7 us against 46.5 for 64 such sequences behind 8,192 shared keys.
 
 template <int DP>
 struct KvRegs {
@@ -688,6 +695,15 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
 // is its number XOR a few bits of its key, which spreads a column of keys over all banks). Keys are
 // read as A operands, values transposed on the way (ds_read_b64_tr_b16: a lane group's 16 lanes
 // read 4 keys x 16 values and each receives one value of the 4 keys).
+//
+// 8 sequences of 257 to 512 new tokens behind 8,192 shared keys, 32 / 8 bf16 heads of 128 (432 GFLOP): 495 to 525 us, 820 to 870
+// TFLOP/s; a prompt of 4,096 in f16 (137 GFLOP, half of the square): 141 to 150 us, 915 to 970. Per wave and tile of 64 keys 64
+// MFMAs (1,024 clocks at their rate) stand beside some 180 vector instructions, 32 of them exponentials:
+// the matrix cores are busy 51% of the time, LDS 26% (no bank conflicts). Timing copies that leave a part out, of
+// 527 us: the loads 65, the exponentials, their sums and rounding 70, the maxima 21, the reads of LDS 50; MFMAs alone
+// 318. Measured and dropped: weights and scores of one tile in turn (555), tiles of 32 keys (605), 64
+// rows a wave with one wave a SIMD (1,028), lines brought into the L2 four tiles ahead (627), maxima looked at
+// after the weights (531).
 
 template <int DP>
 constexpr int kTileKeys = DP <= 128 ? 64 : 32;

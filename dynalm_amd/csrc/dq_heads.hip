@@ -8,7 +8,8 @@
 // Rows that can be read in 16 bytes take up to 16 lanes each, a lane two chunks of 8 values that hold both
 // values of its pairs (chunks j and j + half / 8 for halves, 2j and 2j + 1 for neighbours), so
 // that nothing but the sum of squares crosses lanes; a lane's cosines, sines and weights serve several heads of its token
-// (k_heads). Other rows take a wave each, value by value (k_norm_rope, k_kv_append).
+// (k_heads). Other rows take a wave each, value by value (k_norm_rope, k_kv_append): 235 us in place of 37 for 8,192
+// tokens of 40 heads, 169 in place of 29 for 16,384 tokens appended.
 #include <type_traits>
 
 #include "dq_attn.h"
