@@ -123,10 +123,6 @@ EXPORTS = {
     "dq_plan_defaults": (_I, [_P]),
     "dq_plan_ffn_down": (_I, [_P, _P]),
     "dq_select": (_I, [_P, _P, _P]),
-    "dq_qk_norm_rope": (_I, [_I64, _I64, _P, _P, _P, _P, _P, _P, C.c_float, _P, _P, _P]),
-    "dq_kv_append": (_I, [_P, _I64, _P, _P, _P, _P, C.c_float, _P, _P, _P]),
-    "dq_shared_attention_workspace": (_I64, [_P, _P]),
-    "dq_shared_attention": (_I, [_P, _P, _P, _I64, _P]),
     "dq_matmul_plan": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P]),
 }
 
@@ -360,6 +356,15 @@ class Attention(C.Structure):
                 ("pages_stride", _I64), ("lens", _P), ("max_len", _I64), ("scale", C.c_float)]
 
 
+_HEADS, _ROPE, _CACHE, _ATTENTION = (C.POINTER(t) for t in (Heads, Rope, KvCache, Attention))
+EXPORTS |= {  # (structures are passed as they are, by reference)
+    "dq_qk_norm_rope": (_I, [_I64, _I64, _HEADS, _HEADS, _P, _HEADS, _HEADS, _P, C.c_float, _ROPE, _P, _P]),
+    "dq_kv_append": (_I, [_CACHE, _I64, _HEADS, _HEADS, _P, _P, C.c_float, _ROPE, _P, _P]),
+    "dq_shared_attention_workspace": (_I64, [_CACHE, _ATTENTION]),
+    "dq_shared_attention": (_I, [_CACHE, _ATTENTION, _P, _I64, _P]),
+}
+
+
 def _ref(s):
     return C.addressof(s) if s is not None else None
 
@@ -368,15 +373,18 @@ def qk_norm_rope(tokens: int, head_dim: int, q: Heads, q_out: Heads, q_weight=No
                  k_out: Heads | None = None, k_weight=None, eps: float = 0.0, rope: Rope | None = None, positions=None,
                  stream: int = 0) -> None:
     """q_out = rope(norm(q)), k_out = rope(norm(k)) for each head (dq_qk_norm_rope)."""
-    _check(lib().dq_qk_norm_rope(tokens, head_dim, _ref(q), _ref(q_out), _ptr(q_weight), _ref(k), _ref(k_out),
-                                 _ptr(k_weight), eps, _ref(rope), _ptr(positions), stream))
+    rc = lib().dq_qk_norm_rope(tokens, head_dim, q, q_out, _ptr(q_weight), k, k_out, _ptr(k_weight), eps, rope,
+                               _ptr(positions), stream)
+    if rc:
+        _check(rc)
 
 
 def kv_append(cache: KvCache, tokens: int, k: Heads, v: Heads, slots, k_weight=None, eps: float = 0.0,
               rope: Rope | None = None, positions=None, stream: int = 0) -> None:
     """rope(norm(k)) and v into the cache's slots (dq_kv_append)."""
-    _check(lib().dq_kv_append(_ref(cache), tokens, _ref(k), _ref(v), _ptr(slots), _ptr(k_weight), eps, _ref(rope),
-                              _ptr(positions), stream))
+    rc = lib().dq_kv_append(cache, tokens, k, v, _ptr(slots), _ptr(k_weight), eps, rope, _ptr(positions), stream)
+    if rc:
+        _check(rc)
 
 
 def _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
@@ -389,7 +397,7 @@ def shared_attention_workspace(cache: KvCache, q: Heads, out: Heads, tokens: int
                                prefix_len: int, pages_stride: int, max_len: int, scale: float = 1.0) -> int:
     """Workspace bytes of a shared_attention call of this shape (no GPU needed)."""
     a = _attention(q, out, None, tokens, batch, None, max_q, None, prefix_len, None, pages_stride, None, max_len, scale)
-    n = lib().dq_shared_attention_workspace(_ref(cache), C.addressof(a))
+    n = lib().dq_shared_attention_workspace(cache, a)
     if n < 0:
         raise DqError(1, lib().dq_last_error().decode(errors="replace"))
     return int(n)
@@ -401,7 +409,9 @@ def shared_attention(cache: KvCache, q: Heads, out: Heads, lse, tokens: int, bat
     """out = attention of q over the shared prefix and each sequence's own keys (dq_shared_attention)."""
     a = _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
                    max_len, scale)
-    _check(lib().dq_shared_attention(_ref(cache), C.addressof(a), _ptr(workspace), workspace_bytes, stream))
+    rc = lib().dq_shared_attention(cache, a, _ptr(workspace), workspace_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 # ------------------------------------------------------------------ GGUF files
