@@ -1079,9 +1079,15 @@ union AttnLds<DP, 16> {
   FewLds<DP> few;
 };
 
+// Waves a SIMD that the registers are held down to. Two, but for heads over 128 values where items of few rows
+// would spill: 64 sequences' own keys alone 45.5 us with one and 50.4 with two, fp32 queries 49.6 and
+// 120, behind a prefix of 8,192 117 and 179; bf16 ones behind that prefix 99.4 and 84.6, which takes two.
+template <int T, int DP, int RS, int RO>
+constexpr int kWaves = DP <= 128 || RO == 64 || (RS == 64 && T != DQ_F32) ? 2 : 1;
+
 // RS, RO: rows of the shared and of the own items' tiles.
 template <int T, int TC, int DP, int RS, int RO>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
+__global__ __launch_bounds__(256, kWaves<T, DP, RS, RO>) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
   // On every XCD a shared item for each of its 32 CUs, then an own one for each, and so on while both
   // last: a CU has a shared item, which computes, beside an own one, which reads.
@@ -1210,7 +1216,7 @@ hipError_t launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   if (rs == 16 && ro == 16) e = launch_items<T, TC, DP, 16, 16>(a, p, s);
   if (rs == 64 && ro == 16) e = launch_items<T, TC, DP, 64, 16>(a, p, s);
   if (rs == 64 && ro == 64) e = launch_items<T, TC, DP, 64, 64>(a, p, s);
-  if constexpr (T != DQ_F32) {
+  if constexpr (T != DQ_F32 && DP <= 128) {
     if (rs == 128 && ro == 16) e = launch_items<T, TC, DP, 128, 16>(a, p, s);
     if (rs == 128 && ro == 64) e = launch_items<T, TC, DP, 128, 64>(a, p, s);
     if (rs == 128 && ro == 128) e = launch_items<T, TC, DP, 128, 128>(a, p, s);
