@@ -1087,7 +1087,7 @@ constexpr int kWaves = DP <= 128 || RO == 64 || (RS == 64 && T != DQ_F32) ? 2 : 
 
 // RS, RO: rows of the shared and of the own items' tiles.
 template <int T, int TC, int DP, int RS, int RO>
-__global__ __launch_bounds__(256, kWaves<T, DP, RS, RO>) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
+__global__ __launch_bounds__(256, (kWaves<T, DP, RS, RO>)) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
   // On every XCD a shared item for each of its 32 CUs, then an own one for each, and so on while both
   // last: a CU has a shared item, which computes, beside an own one, which reads.
