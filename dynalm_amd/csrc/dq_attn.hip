@@ -149,6 +149,28 @@ DQ_DEV void load_rows_to_lds(const void* base, const u32 (&off)[N], u32 lds) {
         : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
         : "memory");
 }
+// The same where rows may be less than 1,024 bytes apart: off[i] is the whole offset.
+template <int N>
+DQ_DEV void load_near_rows_to_lds(const void* base, const u32 (&off)[N], u32 lds) {
+  static_assert(N == 2 || N == 4);
+  u32 m0;
+  if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %4\n\ts_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
+        : "memory", "scc");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6\n\ts_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
+        : "memory", "scc");
+}
 DQ_DEV void wait_loads() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -725,10 +747,12 @@ struct TileLds {
   int bad;
 };
 
-template <int T, int TC, int DP, int RT>
+// DP: the values of a key's place in LDS, DC: those that the products run over (the head size, to the next 64, 96, 128, 192
+// or 256).
+template <int T, int TC, int DP, int DC, int RT>
 DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int index, TileLds<DP>& sh) {
   constexpr int NP = kParts<T, TC>;
-  constexpr int NC = DP / 16, KT = kTileKeys<DP>, CH = DP / 8;
+  constexpr int NC = DC / 16, KT = kTileKeys<DP>, CH = DP / 8;
   constexpr int KW = KT / 4, KI = 64 / CH;  // keys a wave loads of a tile, and with one instruction
   auto &s_k = sh.k, &s_v = sh.v;
   auto& s_first = sh.first;
@@ -753,8 +777,8 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   float c[RT];
   RowMax rm[RT];
   float l[RT];
-  RawQ<T, DP> raw[RT];
-  v4u q[RT][NP][DP / 32];
+  RawQ<T, DC> raw[RT];
+  v4u q[RT][NP][DC / 32];
   v4f o[RT][NC];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -762,7 +786,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     const int row = it.first + (valid ? wr + 16 * t + n : 0);
     const int token = row / a.group;
     own_lim[t] = valid ? own_limit(a, it, token) : 0;
-    load_q<T, DP>(a, valid, token, it.head * a.group + row % a.group, g, raw[t]);
+    load_q<T, DC>(a, valid, token, it.head * a.group + row % a.group, g, raw[t]);
     l[t] = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[t][i] = v4f{0, 0, 0, 0};
@@ -785,12 +809,15 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   u32 kload[KW / KI], vload[KW / KI];
 #pragma unroll
   for (int i = 0; i < KW / KI; ++i) {
-    kload[i] = (i * KI + lrow) * token_bytes + kpos(i) - 1024 * i;  // (a whole tile's rows are 1,024 bytes apart at least)
-    vload[i] = (i * KI + lrow) * token_bytes + vpos(i) - 1024 * i;
+    // Heads of DP values lie 1,024 bytes apart from load to load at least. Places past a head of DC < DP values are not
+    // read: the first chunk fills them.
+    const u32 k = kpos(i), v = vpos(i), less = DC == DP ? 1024 * i : 0;
+    kload[i] = (i * KI + lrow) * token_bytes + (k < DC * 2 ? k : 0) - less;
+    vload[i] = (i * KI + lrow) * token_bytes + (v < DC * 2 ? v : 0) - less;
   }
-  u32 kread[DP / 32], vread[NC];
+  u32 kread[DC / 32], vread[NC];
 #pragma unroll
-  for (int e = 0; e < DP / 32; ++e) kread[e] = n * DP + ((4 * e + g) ^ swizzle_k<DP>(n)) * 8;
+  for (int e = 0; e < DC / 32; ++e) kread[e] = n * DP + ((4 * e + g) ^ swizzle_k<DP>(n)) * 8;
   const int vkey = 4 * g + (n >> 2);
 #pragma unroll
   for (int i = 0; i < NC; ++i) vread[i] = vkey * DP + ((2 * i + ((n >> 1) & 1)) ^ swizzle_v<DP>(vkey)) * 8 + (n & 1) * 4;
@@ -832,8 +859,11 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   };
   auto issue = [&](const uint16_t* pool, const Source& r, const u32 (&off)[KW / KI], auto pos_of, u32 to) {
     const uint16_t* from = pool + r.base;
-    if (r.last >= KW - 1 && a.dim == DP) {
-      load_rows_to_lds(from, off, to);
+    if (r.last >= KW - 1 && a.dim == DC) {
+      if constexpr (DC == DP)
+        load_rows_to_lds(from, off, to);
+      else
+        load_near_rows_to_lds(from, off, to);
     } else {
 #pragma unroll
       for (int i = 0; i < KW / KI; ++i) {
@@ -849,7 +879,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   // S^T of a tile
   auto scores = [&](const uint16_t* sk, v4f (&s)[RT][KT / 16]) {
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e)
+    for (int e = 0; e < DC / 32; ++e)
 #pragma unroll
       for (int u = 0; u < KT / 16; ++u) {
         const v4u kf = *reinterpret_cast<const v4u*>(sk + kread[e] + 16 * u * DP);
@@ -904,7 +934,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     if (tiles > 1) issue_keys(next, 1);
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t) c[t] = q_operands<T, TC, DP>(a, raw[t], q[t]);
+  for (int t = 0; t < RT; ++t) c[t] = q_operands<T, TC, DC>(a, raw[t], q[t]);
   // (waits outside the branch, so that the compiler sees q's loads end here and adds no wait to the loop)
   wait_loads();
   __syncthreads();
@@ -967,7 +997,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     }
     // The order below is kept (sched_barrier): operands are read kAhead steps before their products, and
     // the vector work of the weights goes between the products of the next tile's scores.
-    constexpr int F = KT * DP / 512, kAhead = 4, kPairs = RT * KT / 8;
+    constexpr int F = KT * DC / 512, kAhead = 4, kPairs = RT * KT / 8;
     u32 pw[RT][NP][KT / 32][4];
     v4f ahead[RT][KT / 16];  // (after the last tile of what the buffer holds: not used)
     v4u ring[kAhead];
@@ -1061,12 +1091,12 @@ DQ_DEV int xcd_item(int b, int n) {
   return b < 8 * each ? b % 8 * each + b / 8 : b;
 }
 
-template <int T, int TC, int DP, int ROWS, class Lds>
+template <int T, int TC, int DP, int DC, int ROWS, class Lds>
 DQ_DEV void run_item(const AttnArgs& a, const AttnPart& w, bool stacked, int index, Lds& sh) {
   if constexpr (ROWS == 16)
     few_rows<T, TC, DP>(a, w, stacked, index, sh.few);
   else
-    many_rows<T, TC, DP, ROWS / 64>(a, w, stacked, index, sh.tile);
+    many_rows<T, TC, DP, DC, ROWS / 64>(a, w, stacked, index, sh.tile);
 }
 
 template <int DP, int MOST>
@@ -1086,7 +1116,7 @@ template <int T, int DP, int RS, int RO>
 constexpr int kWaves = DP <= 128 || RO == 64 || (RS == 64 && T != DQ_F32) ? 2 : 1;
 
 // RS, RO: rows of the shared and of the own items' tiles.
-template <int T, int TC, int DP, int RS, int RO>
+template <int T, int TC, int DP, int DC, int RS, int RO>
 __global__ __launch_bounds__(256, (kWaves<T, DP, RS, RO>)) void k_attn(AttnArgs a, AttnPart ws, AttnPart wo, int shared, int own) {
   __shared__ __align__(16) AttnLds<DP, RS> sh;
   // On every XCD a shared item for each of its 32 CUs, then an own one for each, and so on while both
@@ -1105,11 +1135,11 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, RS, RO>)) void k_attn(AttnArgs 
     w.own_from = wo.own_from;
     w.with_prefix = wo.with_prefix;
     w.backward = wo.backward;
-    run_item<T, TC, DP, RS>(a, w, stacked, index, sh);
+    run_item<T, TC, DP, DC, RS>(a, w, stacked, index, sh);
   } else if (stacked) {
-    run_item<T, TC, DP, RS>(a, ws, true, index, sh);
+    run_item<T, TC, DP, DC, RS>(a, ws, true, index, sh);
   } else {
-    run_item<T, TC, DP, RO>(a, wo, false, index, sh);
+    run_item<T, TC, DP, DC, RO>(a, wo, false, index, sh);
   }
 }
 
@@ -1200,26 +1230,26 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, Attn
   if (a.lse != nullptr && lane == 0) a.lse[(int64_t)t * a.heads + h] = lse_of(mx, sum, kShift<TC>);
 }
 
-template <int T, int TC, int DP, int RS, int RO>
+template <int T, int TC, int DP, int DC, int RS, int RO>
 hipError_t launch_items(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   const int64_t shared = (int64_t)p.shared.tiles * a.cache.kv_heads * p.shared.splits;
   const int64_t own = (int64_t)p.own.tiles * a.cache.kv_heads * p.own.splits * a.batch;
-  hipLaunchKernelGGL((k_attn<T, TC, DP, RS, RO>), dim3((uint32_t)(shared + own)), dim3(256), 0, s, a, p.shared, p.own,
+  hipLaunchKernelGGL((k_attn<T, TC, DP, DC, RS, RO>), dim3((uint32_t)(shared + own)), dim3(256), 0, s, a, p.shared, p.own,
                      (int)shared, (int)own);
   return hipGetLastError();
 }
 
-template <int T, int TC, int DP>
+template <int T, int TC, int DP, int DC = DP>
 hipError_t launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   const int rs = p.shared.splits > 0 ? p.shared.rows : p.own.rows, ro = p.own.rows;
   hipError_t e = hipErrorInvalidValue;
-  if (rs == 16 && ro == 16) e = launch_items<T, TC, DP, 16, 16>(a, p, s);
-  if (rs == 64 && ro == 16) e = launch_items<T, TC, DP, 64, 16>(a, p, s);
-  if (rs == 64 && ro == 64) e = launch_items<T, TC, DP, 64, 64>(a, p, s);
+  if (rs == 16 && ro == 16) e = launch_items<T, TC, DP, DP, 16, 16>(a, p, s);
+  if (rs == 64 && ro == 16) e = launch_items<T, TC, DP, DC, 64, 16>(a, p, s);
+  if (rs == 64 && ro == 64) e = launch_items<T, TC, DP, DC, 64, 64>(a, p, s);
   if constexpr (T != DQ_F32 && DP <= 128) {
-    if (rs == 128 && ro == 16) e = launch_items<T, TC, DP, 128, 16>(a, p, s);
-    if (rs == 128 && ro == 64) e = launch_items<T, TC, DP, 128, 64>(a, p, s);
-    if (rs == 128 && ro == 128) e = launch_items<T, TC, DP, 128, 128>(a, p, s);
+    if (rs == 128 && ro == 16) e = launch_items<T, TC, DP, DC, 128, 16>(a, p, s);
+    if (rs == 128 && ro == 64) e = launch_items<T, TC, DP, DC, 128, 64>(a, p, s);
+    if (rs == 128 && ro == 128) e = launch_items<T, TC, DP, DC, 128, 128>(a, p, s);
   }
   if (e != hipSuccess || a.part_o == nullptr) return e;
   hipLaunchKernelGGL((k_attn_join<T, TC>), dim3((uint32_t)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(256), 0, s, a, p.shared,
@@ -1230,7 +1260,9 @@ hipError_t launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
 template <int T, int TC>
 hipError_t by_dim(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   if (a.dim <= 64) return launch<T, TC, 64>(a, p, s);
+  if (a.dim <= 96) return launch<T, TC, 128, 96>(a, p, s);
   if (a.dim <= 128) return launch<T, TC, 128>(a, p, s);
+  if (a.dim <= 192) return launch<T, TC, 256, 192>(a, p, s);
   return launch<T, TC, 256>(a, p, s);
 }
 

@@ -250,6 +250,9 @@ SHAPES = [
     pytest.param([40], [300], 900, 4, 2, 256, 32, True, id="one prompt behind a prefix"),
     pytest.param([6, 2, 5], [700, 2, 300], 260, 10, 2, 128, 64, True, id="own keys in several ranges"),
     pytest.param([i % 3 for i in range(150)], [i % 3 + i % 40 for i in range(150)], 35, 2, 1, 64, 16, False, id="150 sequences"),
+    pytest.param([33, 40], [90, 70], 140, 4, 2, 192, 16, True, id="heads of 192"),
+    pytest.param([33, 40], [90, 70], 140, 4, 2, 160, 32, False, id="heads of 160"),
+    pytest.param([33, 40], [90, 170], 140, 8, 2, 96, 16, True, id="prompts in heads of 96"),
     pytest.param([64, 1, 17], [64, 500, 17], 100, 8, 8, 64, 64, True, id="prompts and a decode step"),
 ]
 
