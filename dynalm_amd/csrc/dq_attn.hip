@@ -1169,6 +1169,8 @@ DQ_DEV int find_seq(const AttnArgs& a, int t, int lane) {
 
 // Weights of up to 64 parts at a time lie one to a lane; their sums of v are read 8 at a time, the first 8 before
 // anything is known of the row (a part that was not written is not used).
+// Bound by two or three rounds of reads: 6.2 us for 2,048 rows of 9 parts of 128 values, 8.7 for 4,096 of 17 (36
+// MB), 4 for a few rows; 16 parts at a time 1 us more.
 template <int T, int TC>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, AttnPart wb) {
   const int lane = threadIdx.x & 63;

@@ -521,6 +521,8 @@ DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads
  * max_q, prefix_len, max_len), not on timing. Rows outside every sequence are not written.
  * A row that would read a page number outside [0, n_pages) gets NaN; so may rows of its sequence beside it (all
  * rows, for a page of the prefix).
+ * A cache without pages is refused where there are keys; keys and head rows are counted in 32 bits (up to 2^29
+ * keys of a kind, 2^30 head rows), places of a page lie up to 2^25 values apart.
  * workspace: dq_shared_attention_workspace bytes of device memory (16-byte aligned) that the call may overwrite; its
  * contents need not be kept. */
 typedef struct dq_attention {
