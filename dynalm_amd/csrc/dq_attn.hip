@@ -940,10 +940,8 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   __syncthreads();
   if (tiles > 0) scores(s_k[0], s);
   for (int tile = 0; tile < tiles; ++tile) {
-    if (tile > 0) {
-      wait_loads();     // this wave's part of the tile's values and of the next one's keys is in LDS
-      __syncthreads();  // everyone's is, and the other buffers are read out
-    }
+    if (tile > 0) wait_loads();  // this wave's part of the tile's values and of the next one's keys is in LDS
+    __syncthreads();             // everyone's is, and the buffers loaded below are read out (tile 0: its keys, just above)
     if (tile + 1 < tiles) issue_values(next, (tile + 1) & 1);
     if (tile + 2 < tiles) {
       next = resolve(after);

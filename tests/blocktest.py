@@ -106,3 +106,37 @@ def attention(q, ks, vs, lens_q, lens, prefix: int, scale: float, type: str, cac
                 lse_bound[start + i, h] = d + (64 + seen / 8) * F32U + 2 * F32U * abs(z.item())
         start += n
     return out, lse, bound, lse_bound
+
+
+def attention_by_heads(q, ks, vs, lens_q, lens, prefix: int, scale: float, type: str, cache_type: str):
+    """`attention` for many rows: the same values and bounds, a sequence's head at a time, on q's device."""
+    tokens, nh, dim = q.shape
+    out = torch.zeros((tokens, nh, dim), dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    lse = torch.full((tokens, nh), -math.inf, dtype=torch.float64, device=q.device)
+    lse_bound = torch.zeros_like(lse)
+    start = 0
+    ut = 0.0 if type == "f32" else U[cache_type]
+    for b, n in enumerate(lens_q):
+        k, v = ks[b].to(q.device).double(), vs[b].to(q.device).double()
+        group = nh // k.shape[1]
+        seen = prefix + torch.clamp(lens[b] - n + 1 + torch.arange(n, device=q.device), 0, lens[b])
+        hidden = torch.arange(k.shape[0], device=q.device)[None, :] >= seen[:, None]
+        some = seen > 0
+        rows = slice(start, start + n)
+        for h in range(nh if n and k.shape[0] else 0):
+            kk, vv, qq = k[:, h // group], v[:, h // group], q[rows, h].double()
+            s = (qq @ kk.t().contiguous() * scale).masked_fill(hidden, -math.inf)
+            z = torch.logsumexp(s, 1)
+            p = torch.where(some[:, None], torch.exp(s - z[:, None]), 0.0)
+            size = p @ vv.abs()
+            most = (qq.abs() @ kk.abs().t().contiguous()).masked_fill(hidden, 0.0).amax(1)
+            d = (dim + 16) * 2 * F32U * most * scale + 4 * F32U * (s.masked_fill(hidden, 0.0).abs().amax(1) + 16)
+            steps = (64 + seen / 8) * F32U
+            low = 2.0**-25 * ((~hidden).double() @ vv.abs()) * p.amax(1, keepdim=True) if type == "f16" else 0.0
+            out[rows, h] = p @ vv
+            bound[rows, h] = (2 * d + steps + ut)[:, None] * size + low
+            lse[rows, h] = z
+            lse_bound[rows, h] = torch.where(some, d + steps + 2 * F32U * z.abs(), 0.0)
+        start += n
+    return out.cpu(), lse.cpu(), bound.cpu(), lse_bound.cpu()

@@ -431,3 +431,24 @@ def test_block_in_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
+
+
+def check_by_heads(c, repeats=0, **kw):
+    """`check` for calls of many rows; every further call gives the same bits."""
+    lse = torch.full((c["tokens"], c["q"].shape[1]), 33.0, device="cuda")
+    out = call(c, lse=lse, **kw)
+    want, want_lse, bound, lse_bound = B.attention_by_heads(c["q"], c["ks"], c["vs"], c["new"], c["lens"], c["prefix"], c["scale"],
+                                                            c["type"], c["cache"])
+    B.close(out, want, bound, c["type"])
+    B.close(lse, want_lse, lse_bound, "f32")
+    for _ in range(repeats):
+        assert torch.equal(call(c, **kw), out)
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("new,lens,prefix", [([256] * 8, [300] * 8, 200), ([1] * 96, [130] * 96, 2000)], ids=["prompts", "decode"])
+def test_attention_with_every_cu_taken(cuda, type, cache, dim, new, lens, prefix):
+    """Tiles of several keys' worth on all CUs, two workgroups each, whose waves run apart: keys are loaded over
+    those of two tiles before only once all waves have read them."""
+    check_by_heads(build(41, new, lens, prefix, 32, 8, dim, type, cache, 16, True), repeats=10)
