@@ -428,6 +428,14 @@ DQ_DEV void store4(const AttnArgs& a, int64_t at, int d, v4f y) {
   }
 }
 
+// The finished values of a row: zeros where no weight was above zero (whatever infinite or NaN values it saw).
+DQ_DEV v4f finish(v4f o, float sum, float inv) {
+  v4f y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = sum == 0.f ? 0.f : o[i] * inv;
+  return y;
+}
+
 DQ_DEV float lse_of(float m, float l, float shift) {
   return l == 0.f ? -INFINITY : (float)(((double)(m - shift) + (double)__log2f(l)) * 0.693147180559945309);
 }
@@ -699,8 +707,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
     const int rw = it.first + r, tk = rw / a.group, h = it.head * a.group + rw % a.group;
     if (a.part_o == nullptr) {
       if (it.b < 0 && a.q_offsets != nullptr && (tk < a.q_offsets[0] || tk >= a.q_offsets[a.batch])) continue;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      store4<T>(a, (int64_t)tk * a.out_token + (int64_t)h * a.out_head, 4 * d4, y * inv);
+      store4<T>(a, (int64_t)tk * a.out_token + (int64_t)h * a.out_head, 4 * d4, finish(y, sum, 1.f / sum));
       if (a.lse != nullptr && d4 == 0) a.lse[(int64_t)tk * a.heads + h] = lse_of(mx, sum, kShift<TC>);
     } else {
       const int64_t at = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group + rw;
@@ -1037,6 +1044,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   if (bad) s_bad = 1;
   __syncthreads();
   const bool nan = s_bad != 0;
+  float* s_sum = reinterpret_cast<float*>(&s_k[0][0]);  // (the keys have been read)
   const int64_t part = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group;
   auto covered = [&](int token) {
     return it.b >= 0 || a.q_offsets == nullptr || (token >= a.q_offsets[0] && token < a.q_offsets[a.batch]);
@@ -1049,12 +1057,13 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
     const int row = it.first + wr + 16 * t + n, token = row / a.group, h = it.head * a.group + row % a.group;
     if (a.part_o == nullptr) {
       if (!covered(token)) continue;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = 1.f / sum;
       const int64_t at = (int64_t)token * a.out_token + (int64_t)h * a.out_head;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (16 * i + 4 * g < a.dim) store4<T>(a, at, 16 * i + 4 * g, o[t][i] * inv);
+        if (16 * i + 4 * g < a.dim) store4<T>(a, at, 16 * i + 4 * g, finish(o[t][i], sum, inv));
       if (a.lse != nullptr && g == 0) a.lse[(int64_t)token * a.heads + h] = lse_of(rm[t].m, sum, kShift<TC>);
+      if (noting && g == 0) s_sum[wr + 16 * t + n] = sum;
     } else {
       const int64_t at = part + row;
 #pragma unroll
@@ -1072,7 +1081,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
       const int token = row / a.group;
       if (a.part_o != nullptr) {
         a.part_o[(part + row) * a.dim + d] += y;
-      } else if (covered(token)) {
+      } else if (covered(token) && s_sum[r] != 0.f) {
         const int64_t at = (int64_t)token * a.out_token + (int64_t)(it.head * a.group + row % a.group) * a.out_head + d;
         store1<T>(a.out, at, load1<T>(a.out, at) + y);
       }
@@ -1225,8 +1234,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, Attn
       }
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (in) store4<T>(a, (int64_t)t * a.out_token + (int64_t)h * a.out_head, d, y * inv);
+  if (in) store4<T>(a, (int64_t)t * a.out_token + (int64_t)h * a.out_head, d, finish(y, sum, 1.f / sum));
   if (a.lse != nullptr && lane == 0) a.lse[(int64_t)t * a.heads + h] = lse_of(mx, sum, kShift<TC>);
 }
 

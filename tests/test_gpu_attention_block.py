@@ -452,3 +452,34 @@ def test_attention_with_every_cu_taken(cuda, type, cache, dim, new, lens, prefix
     """Tiles of several keys' worth on all CUs, two workgroups each, whose waves run apart: keys are loaded over
     those of two tiles before only once all waves have read them."""
     check_by_heads(build(41, new, lens, prefix, 32, 8, dim, type, cache, 16, True), repeats=10)
+
+
+def put(c, pool, b, j, head, column, value):
+    """Sets a value of key j (the prefix's before the own ones) of sequence b in the cache."""
+    page = pool.shape[1]
+    if j < c["prefix"]:
+        pool[int(c["prefix_pages"][j // page]), j % page, head, column] = value
+    else:
+        j -= c["prefix"]
+        pool[int(c["table"][b, j // page]), j % page, head, column] = value
+
+
+# (few rows and tiles, with and without a prefix, one item a row and several)
+SPLITS = [([1], [700], 600), ([3, 2], [40, 30], 900), ([90], [1500], 0), ([12] * 3, [60] * 3, 1100)]
+IDS = ["few rows", "prefix shared", "tiles", "prefix shared by tiles"]
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lens,prefix", SPLITS + [([2], [20], 0), ([70], [70], 0)], ids=IDS + ["few rows, one item", "tiles, one item"])
+def test_rows_whose_scores_are_all_minus_infinity(cuda, type, new, lens, prefix):
+    """They get zeros whatever the values, as rows without keys do."""
+    c = build(47, new, lens, prefix, 2, 1, 64, type, type, 16)
+    keys = torch.isfinite(c["kc"][..., 0])
+    c["kc"][..., 0] = torch.where(keys, -math.inf, c["kc"][..., 0])
+    c["q"][:, :, 0] = c["q"][:, :, 0].abs() + 1
+    lse = torch.full((c["tokens"], 2), 33.0, device="cuda")
+    for value in (0.5, math.inf, math.nan):
+        for j in {0, prefix // 2, prefix + lens[0] - new[0], prefix + lens[0] - 1}:
+            put(c, c["vc"], 0, j, 0, 9, value)
+        assert torch.all(call(c, lse=lse) == 0), value
+        assert torch.all(lse == -math.inf)
