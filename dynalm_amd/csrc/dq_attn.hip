@@ -699,7 +699,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       const float mk = s_ml[k][r][0];
       const float f = mk == -INFINITY ? 0.f : exp2_fast(mk - mx);
       sum = fmaf(s_ml[k][r][1], f, sum);
-      if (mk != -INFINITY) y += s_o[k][r][d4] * f;
+      y += s_o[k][r][d4] * f;
     }
     if (s_bad) sum = __builtin_nanf("");
     if (s_noted)
@@ -1230,7 +1230,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, Attn
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float fi = as_f(__builtin_amdgcn_readlane(as_u(f), (s + i) & 63));
-        if (s + i < n && fi > 0.f) y += x[i] * fi;
+        if (s + i < n) y += x[i] * fi;  // (a factor of 0 too: what is infinite or NaN stays to be seen)
       }
     }
   }

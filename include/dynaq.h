@@ -517,6 +517,9 @@ DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads
  * to that type before the second product, or DQ_F32, where queries and weights are split so that
  * products keep fp32's precision; sums, maxima and the softmax are fp32 always. out must not
  * overlap q.
+ * An infinite or NaN value of a key makes its column infinite or NaN in every row that sees the key, however
+ * small the key's weight, and reaches no other row. With fp32 q an infinite query or key may give NaN where its scores
+ * are infinite (products are summed in parts).
  * The prefix is read once for the whole batch, not once a sequence. A row's bits depend on the call's shape (batch, tokens,
  * max_q, prefix_len, max_len), not on timing. Rows outside every sequence are not written.
  * A row that would read a page number outside [0, n_pages) gets NaN; so may rows of its sequence beside it (all

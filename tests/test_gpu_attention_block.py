@@ -483,3 +483,25 @@ def test_rows_whose_scores_are_all_minus_infinity(cuda, type, new, lens, prefix)
             put(c, c["vc"], 0, j, 0, 9, value)
         assert torch.all(call(c, lse=lse) == 0), value
         assert torch.all(lse == -math.inf)
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("new,lens,prefix", SPLITS, ids=IDS)
+def test_a_nan_value_is_seen_whatever_its_weight(cuda, type, cache, new, lens, prefix):
+    """A visible key's NaN makes its column NaN, also where the key's weight rounds to 0 beside another
+    range's: it does not depend on how the keys are split."""
+    c = build(43, new, lens, prefix, 2, 1, 64, type, cache, 16)
+    c["q"][:, :, 0] = 40.0
+    last = prefix + lens[0] - new[0]
+    for b in range(len(new)):
+        put(c, c["kc"], b, prefix + lens[b] - new[b], 0, 0, 120.0)  # 600 above all others, seen by all rows
+    clean = call(c)
+    assert torch.isfinite(clean).all()
+    for at in {0, last // 2, last - 1}:
+        c2 = c | {"vc": c["vc"].clone()}
+        put(c2, c2["vc"], 0, at, 0, 5, math.nan)
+        out = call(c2)
+        want = torch.zeros_like(out, dtype=torch.bool)
+        want[: new[0] if at >= prefix else None, :, 5] = True
+        assert torch.equal(torch.isnan(out), want), at
+        assert torch.equal(out[~want], clean[~want])
