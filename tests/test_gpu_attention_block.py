@@ -505,3 +505,31 @@ def test_a_nan_value_is_seen_whatever_its_weight(cuda, type, cache, new, lens, p
         want[: new[0] if at >= prefix else None, :, 5] = True
         assert torch.equal(torch.isnan(out), want), at
         assert torch.equal(out[~want], clean[~want])
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("dim", [64, 80, 96, 128, 192, 256])
+@pytest.mark.parametrize("new,lens,prefix", SPLITS + [([5], [40], 20), ([90], [90], 0), ([40, 50], [70, 50], 64), ([70], [200], 130)])
+def test_infinite_values_reach_the_rows_that_see_them(cuda, type, cache, dim, new, lens, prefix):
+    """Values alone are infinite or NaN, the keys finite: their columns in the rows that see them are what the
+    sum makes of them, everything else keeps its bits."""
+    heads, kv = 4, 2
+    c = build(53 + dim, new, lens, prefix, heads, kv, dim, type, cache, 16)
+    clean = call(c)
+    n, own = new[0], prefix + lens[0] - new[0]  # own: the key of row 0
+    want = torch.zeros((c["tokens"], heads, dim), dtype=torch.float64)
+    bad = [(own + n - 1, 0, 0, math.inf), (own + n - 1, 1, dim - 1, -math.inf), (own + n // 2, 0, 3, math.nan), (own + n // 2, 1, 1, math.inf),
+           (own + n - 1, 1, 1, -math.inf), (own, 0, dim - 2, -math.inf), (own + n // 3, 0, dim // 2 + 1, math.inf),
+           (max(0, own - 1), 1, dim // 2, math.inf), (0, 1, 7, -math.inf), (prefix // 2, 0, 7, math.nan)]
+    for (j, head, column), value in {b[:3]: b[3] for b in bad}.items():
+        put(c, c["vc"], 0, j, head, column, value)
+        rows = slice(None) if j < prefix else slice(max(0, j - own), n)
+        want[rows, 2 * head : 2 * head + 2, column] += value
+    out = call(c).cpu()
+    same = want == 0
+    assert torch.equal(out[same], clean.cpu()[same])
+    if type == "f32":  # (a weight's parts times an infinity: of both signs, or NaN)
+        assert not torch.isfinite(out[~same]).any()
+    else:
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out[torch.isinf(want)].double(), want[torch.isinf(want)])
