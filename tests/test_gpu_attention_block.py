@@ -433,14 +433,18 @@ def test_block_in_a_graph(cuda):
         assert torch.equal(out, want), i
 
 
-def check_by_heads(c, repeats=0, **kw):
-    """`check` for calls of many rows; every further call gives the same bits."""
+def check_by_heads(c, repeats=0, every=1, **kw):
+    """`check` for calls of many rows (every `every`th sequence of them); every further call gives the same bits."""
     lse = torch.full((c["tokens"], c["q"].shape[1]), 33.0, device="cuda")
     out = call(c, lse=lse, **kw)
-    want, want_lse, bound, lse_bound = B.attention_by_heads(c["q"], c["ks"], c["vs"], c["new"], c["lens"], c["prefix"], c["scale"],
-                                                            c["type"], c["cache"])
-    B.close(out, want, bound, c["type"])
-    B.close(lse, want_lse, lse_bound, "f32")
+    at, start = [], 0
+    for b, n in enumerate(c["new"]):
+        at += range(start, start + n) if b % every == 0 else ()
+        start += n
+    want, want_lse, bound, lse_bound = B.attention_by_heads(c["q"][at], c["ks"][::every], c["vs"][::every], c["new"][::every],
+                                                            c["lens"][::every], c["prefix"], c["scale"], c["type"], c["cache"])
+    B.close(out[at], want, bound, c["type"])
+    B.close(lse[at], want_lse, lse_bound, "f32")
     for _ in range(repeats):
         assert torch.equal(call(c, **kw), out)
 
@@ -533,3 +537,12 @@ def test_infinite_values_reach_the_rows_that_see_them(cuda, type, cache, dim, ne
     else:
         assert torch.equal(torch.isnan(out), torch.isnan(want))
         assert torch.equal(out[torch.isinf(want)].double(), want[torch.isinf(want)])
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 80, 96, 128])
+@pytest.mark.parametrize("new,lens", [([1] * 40, [1 + 9 * i % 200 for i in range(40)]), ([3 - i % 3 for i in range(20)], [3 + 31 * i for i in range(20)])],
+                         ids=["one token", "proposed tokens"])
+def test_shared_tiles_of_128_rows(cuda, type, dim, new, lens):
+    """A prefix so long that its items take 128 rows, own keys beside them in tiles of 16 and of 64 rows."""
+    check_by_heads(build(59, new, lens, 10001, 64, 8, dim, type, type, 16, dim == 96), repeats=2, every=7)
