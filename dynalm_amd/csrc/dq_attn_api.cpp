@@ -116,11 +116,12 @@ dq::HeadRows rows(const dq_heads* in, const dq_heads* out, const float* w) {
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int64_t kMaxRows = (int64_t)1 << 31;  // head rows of a launch (a grid's workgroups)
+constexpr int64_t kMaxRows = (int64_t)1 << 31;   // head rows of a call: they are counted in 32 bits
+constexpr int64_t kMaxHeads = (int64_t)1 << 25;  // heads of a token: its rows run in one launch
 
 int check_tokens(int64_t tokens, int64_t heads) {
   if (tokens < 0) return bad("tokens must be >= 0");
-  if (tokens > kMaxRows / heads) return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %lld heads are too many", (ll)tokens, (ll)heads);
+  if (tokens > kMaxRows / heads || heads > kMaxHeads) return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %lld heads are too many", (ll)tokens, (ll)heads);
   return DQ_OK;
 }
 

@@ -321,6 +321,26 @@ hipError_t launch_heads(int64_t tokens, int dim, const HeadRows& a, const HeadRo
   return hipGetLastError();
 }
 
+// A dispatch counts its threads in 32 bits: launches of kLaunchRows head rows at most, of whole tokens, one after
+// another (a wave a row, 2^31 threads).
+constexpr int64_t kLaunchRows = (int64_t)1 << 25;
+
+// The rows from token t0 on.
+HeadRows from_token(HeadRows r, int in_type, int out_type, int64_t t0) {
+  r.in = static_cast<const char*>(r.in) + t0 * r.in_token * (in_type == DQ_F32 ? 4 : 2);
+  if (r.out != nullptr) r.out = static_cast<char*>(r.out) + t0 * r.out_token * (out_type == DQ_F32 ? 4 : 2);
+  return r;
+}
+
+// f(first token, tokens) for each launch.
+template <class F>
+hipError_t by_launch(int64_t tokens, int64_t heads, F&& f) {
+  const int64_t most = heads < kLaunchRows ? kLaunchRows / heads : 1;
+  for (int64_t t0 = 0; t0 < tokens; t0 += most)
+    if (const hipError_t e = f(t0, tokens - t0 < most ? tokens - t0 : most); e != hipSuccess) return e;
+  return hipSuccess;
+}
+
 template <class F>
 hipError_t by_type(int type, F&& f) {
   switch (type) {
@@ -340,14 +360,19 @@ hipError_t by_cache_type(int type, F&& f) {
 
 hipError_t launch_norm_rope(int in_type, int out_type, int64_t tokens, int dim, const HeadRows& a, const HeadRows& b,
                             float eps, const RopeArgs& rope, hipStream_t s) {
-  const int64_t blocks = (tokens * (a.heads + b.heads) + 3) / 4;
+  const int64_t heads = (int64_t)a.heads + b.heads;
   const bool chunks = in_chunks(in_type, out_type, a, b, rope);
-  return by_type(in_type, [&](auto ti) {
-    return by_type(out_type, [&](auto to) {
-      if (chunks) return launch_heads<ti(), to(), false>(tokens, dim, a, b, CacheArgs{}, nullptr, eps, rope, s);
-      hipLaunchKernelGGL((k_norm_rope<ti(), to()>), dim3((uint32_t)blocks), dim3(256), 0, s, tokens, dim, a, b, eps,
-                         rope);
-      return hipGetLastError();
+  return by_launch(tokens, heads, [&](int64_t t0, int64_t n) {
+    const HeadRows at = from_token(a, in_type, out_type, t0), bt = from_token(b, in_type, out_type, t0);
+    RopeArgs rt = rope;
+    if (rt.positions != nullptr) rt.positions += t0;
+    return by_type(in_type, [&](auto ti) {
+      return by_type(out_type, [&](auto to) {
+        if (chunks) return launch_heads<ti(), to(), false>(n, dim, at, bt, CacheArgs{}, nullptr, eps, rt, s);
+        hipLaunchKernelGGL((k_norm_rope<ti(), to()>), dim3((uint32_t)((n * heads + 3) / 4)), dim3(256), 0, s, n, dim, at,
+                           bt, eps, rt);
+        return hipGetLastError();
+      });
     });
   });
 }
@@ -355,14 +380,19 @@ hipError_t launch_norm_rope(int in_type, int out_type, int64_t tokens, int dim, 
 hipError_t launch_kv_append(int in_type, int cache_type, int64_t tokens, int dim, const HeadRows& k, const HeadRows& v,
                             const CacheArgs& cache, const int64_t* slots, float eps, const RopeArgs& rope,
                             hipStream_t s) {
-  const int64_t blocks = (tokens * 2 * cache.kv_heads + 3) / 4;
+  const int64_t heads = 2 * (int64_t)cache.kv_heads;
   const bool chunks = in_chunks(in_type, cache_type, k, v, rope);  // (the cache's places are 16-byte aligned always)
-  return by_type(in_type, [&](auto ti) {
-    return by_cache_type(cache_type, [&](auto tc) {
-      if (chunks) return launch_heads<ti(), tc(), true>(tokens, dim, k, v, cache, slots, eps, rope, s);
-      hipLaunchKernelGGL((k_kv_append<ti(), tc()>), dim3((uint32_t)blocks), dim3(256), 0, s, tokens, dim, k, v, cache,
-                         slots, eps, rope);
-      return hipGetLastError();
+  return by_launch(tokens, heads, [&](int64_t t0, int64_t n) {
+    const HeadRows kt = from_token(k, in_type, cache_type, t0), vt = from_token(v, in_type, cache_type, t0);
+    RopeArgs rt = rope;
+    if (rt.positions != nullptr) rt.positions += t0;
+    return by_type(in_type, [&](auto ti) {
+      return by_cache_type(cache_type, [&](auto tc) {
+        if (chunks) return launch_heads<ti(), tc(), true>(n, dim, kt, vt, cache, slots + t0, eps, rt, s);
+        hipLaunchKernelGGL((k_kv_append<ti(), tc()>), dim3((uint32_t)((n * heads + 3) / 4)), dim3(256), 0, s, n, dim, kt,
+                           vt, cache, slots + t0, eps, rt);
+        return hipGetLastError();
+      });
     });
   });
 }

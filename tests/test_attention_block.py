@@ -122,3 +122,11 @@ def test_workspace_needs_no_pointers_and_has_a_bound():
                     assert 0 <= n <= dq.ATTENTION_WORKSPACE_BYTES
     with pytest.raises(dq.DqError):
         dq.shared_attention_workspace(cache(), heads(), heads(), 1, 1, 0, 0, 1, 1)
+
+
+def test_heads_of_a_token_run_in_one_launch():
+    """A launch counts its threads in 32 bits: 2^26 heads of one token are over that, refused and not tried."""
+    many = {"heads": 1 << 26, "token_stride": 64 << 26}
+    refused("unsupported", dq.qk_norm_rope, 1, 64, heads(**many), heads(**many))
+    kv = heads(**{"heads": 1 << 25, "token_stride": 64 << 25})
+    refused("unsupported", dq.kv_append, cache(kv_heads=1 << 25, token_stride=64 << 25, page_stride=64 << 29), 1, kv, kv, AT)

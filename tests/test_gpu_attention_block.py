@@ -546,3 +546,27 @@ def test_infinite_values_reach_the_rows_that_see_them(cuda, type, cache, dim, ne
 def test_shared_tiles_of_128_rows(cuda, type, dim, new, lens):
     """A prefix so long that its items take 128 rows, own keys beside them in tiles of 16 and of 64 rows."""
     check_by_heads(build(59, new, lens, 10001, 64, 8, dim, type, type, 16, dim == 96), repeats=2, every=7)
+
+
+@pytest.mark.parametrize("rot", [0, 2])
+def test_more_rows_than_a_launch_has_threads_for(cuda, rot):
+    """2^26 head rows and some, a wave each: in several launches, the same bits as in calls of fewer tokens. (Half of a
+    rotation of 2 is less than a chunk of 8 values; heads at odd values are no chunks either.)"""
+    tokens, heads, dim, part = (1 << 23) + 5, 8, 8, 1 << 20
+    x = torch.randn(tokens * heads * dim + 1, device="cuda", dtype=torch.float16)[1:].view(tokens, heads, dim)
+    td = [t.cuda() for t in B.rope_table(64, 2)]
+    rope = dq.Rope(td[0].data_ptr(), td[1].data_ptr(), 64, 2, dq.ROPE_HALVES) if rot else None
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda") % 64
+    w = 1 + torch.rand(dim, device="cuda")
+    out = torch.full_like(x, math.nan)
+    dq.qk_norm_rope(tokens, dim, B.heads(x), B.heads(out), w, eps=1e-5, rope=rope, positions=pos, stream=stream())
+    for t0 in range(0, tokens, part):
+        n = min(part, tokens - t0)
+        want = torch.full_like(x[t0 : t0 + n], 55.0)
+        dq.qk_norm_rope(n, dim, B.heads(x[t0 : t0 + n]), B.heads(want), w, eps=1e-5, rope=rope, positions=pos[t0 : t0 + n], stream=stream())
+        assert torch.equal(out[t0 : t0 + n], want), t0
+    pages = (tokens + 15) // 16
+    k, v = (torch.zeros((pages, 16, heads, dim), device="cuda", dtype=torch.float16) for _ in range(2))
+    slots = tokens - 1 - torch.arange(tokens, device="cuda")
+    dq.kv_append(B.kv_cache(k, v), tokens, B.heads(x), B.heads(x), slots, w, 1e-5, rope, pos, stream())
+    assert torch.equal(k.view(-1, heads, dim)[:tokens].flip(0), out) and torch.equal(v.view(-1, heads, dim)[:tokens].flip(0), x)
