@@ -2,6 +2,7 @@
 // checks with dynacore's status codes, then the launches. Nothing is allocated or kept.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/dynaq.h"
@@ -91,6 +92,39 @@ int check_cache(const dq_kv_cache* c, bool data) {
   if (data && c->n_pages > 0) {
     if (c->k == nullptr || c->v == nullptr) return bad("cache: null pointer");
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0) return bad("cache: k and v must be 16-byte aligned");
+  }
+  return DQ_OK;
+}
+
+// A cache's places that are written must not run into each other, nor its keys into its values.
+int check_cache_apart(const dq_kv_cache* c) {
+  if (c->n_pages == 0) return DQ_OK;
+  struct Axis {
+    int64_t stride, n;
+  } x[3] = {{c->page_stride, c->n_pages}, {c->token_stride, c->page_size}, {c->head_stride, c->kv_heads}};
+  for (Axis& a : x)
+    if (a.n == 1) a.stride = 0;
+  std::sort(x, x + 3, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+  int64_t end = c->head_dim;  // of the values that the shorter strides reach
+  for (const Axis& a : x) {
+    if (a.n > 1 && a.stride < end)
+      return dq::set_error(DQ_INVALID_ARGUMENT, "cache: places overlap (page_stride %lld, token_stride %lld, head_stride %lld)",
+                           (ll)c->page_stride, (ll)c->token_stride, (ll)c->head_stride);
+    end += (a.n - 1) * a.stride;
+  }
+  // Apart by d values, a key's place meets a value's if d is less than a head away from a difference of two places;
+  // of each axis, longest stride first, only the two multiples next to d can come that near.
+  const int64_t d = (reinterpret_cast<intptr_t>(c->v) - reinterpret_cast<intptr_t>(c->k)) / 2;
+  for (int pick = 0; pick < 8; ++pick) {
+    int64_t rest = d < 0 ? -d : d;
+    for (int i = 2; i >= 0; --i) {
+      if (x[i].n == 1) continue;
+      int64_t m = rest / x[i].stride + (pick >> i & 1);
+      if (rest < 0) m = -(-rest / x[i].stride) - (pick >> i & 1);
+      m = std::min(std::max(m, -(x[i].n - 1)), x[i].n - 1);
+      rest -= m * x[i].stride;
+    }
+    if (rest < c->head_dim && -rest < c->head_dim) return bad("cache: keys and values overlap");
   }
   return DQ_OK;
 }
@@ -311,6 +345,7 @@ int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, co
   dq::RopeArgs ra;
   if (int rc = check_rope(rope, positions, cache->head_dim, tokens, &ra); rc != DQ_OK) return rc;
   if (tokens == 0) return DQ_OK;
+  if (int rc = check_cache_apart(cache); rc != DQ_OK) return rc;
   if (slots == nullptr) return bad("slots: null argument");
   if (int rc = check_data("k", k); rc != DQ_OK) return rc;
   if (int rc = check_data("v", v); rc != DQ_OK) return rc;

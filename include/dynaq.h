@@ -496,7 +496,8 @@ typedef struct dq_kv_cache {
 /* Appends token t's keys rope(norm(k[t])) and values v[t] (kv_heads heads of the cache's
  * head_dim each) at slots[t] = page * page_size + place. A slot outside [0, n_pages *
  * page_size) leaves its token out (padding: -1); a slot that is given twice holds one of the
- * two tokens' heads. k_weight, eps, rope and positions are dq_qk_norm_rope's; without a norm
+ * two tokens' heads. A cache whose places overlap, or whose keys overlap its values, is refused.
+ * k_weight, eps, rope and positions are dq_qk_norm_rope's; without a norm
  * and a rotation keys are converted as values are (to nearest even). */
 DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, const dq_heads* v,
                         const int64_t* slots, const float* k_weight, float eps, const dq_rope* rope,

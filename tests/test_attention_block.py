@@ -130,3 +130,27 @@ def test_heads_of_a_token_run_in_one_launch():
     refused("unsupported", dq.qk_norm_rope, 1, 64, heads(**many), heads(**many))
     kv = heads(**{"heads": 1 << 25, "token_stride": 64 << 25})
     refused("unsupported", dq.kv_append, cache(kv_heads=1 << 25, token_stride=64 << 25, page_stride=64 << 29), 1, kv, kv, AT)
+
+
+def test_append_refuses_caches_whose_places_overlap():
+    """Two rows would be written to one address; which layouts are apart is counted place by place."""
+
+    def apart(c):
+        base = [c.k // 2 + p * c.page_stride + i * c.token_stride + h * c.head_stride
+                for p in range(c.n_pages) for i in range(c.page_size) for h in range(c.kv_heads)]
+        at = sorted(base + [x + (c.v - c.k) // 2 for x in base])
+        return all(b - a >= c.head_dim for a, b in zip(at, at[1:]))
+
+    n, kinds = 3 * 16 * 2 * 64, set()
+    for kv, page, token, head in ((2, 16 * 128, 128, 64), (2, 16 * 128, 64, 1024), (2, 64, 3 * 128, 3 * 64), (2, 64, 192, 192 * 16),
+                                  (2, 2048, 64, 64), (2, 1024, 128, 64), (2, 16 * 128, 96, 64), (1, 16 * 64, 64, 8), (1, 16 * 64, 64, 64),
+                                  (2, 16 * 256, 256, 64), (2, 16 * 256, 256, 128), (2, 64, 64, 64), (2, 2040, 128, 64), (2, 2 * 2048, 128, 64)):
+        for d in (n, 2 * n + 8, 0, 8, 56, 64, 128, 2048, -2048, 1024, -64, -n, 2048 + 64, 4 * n, 192):
+            c = cache(v=AT + 2 * d, kv_heads=kv, n_pages=3, page_stride=page, token_stride=token, head_stride=head)
+            rows = heads(heads=kv, token_stride=128)
+            with pytest.raises(dq.DqError) as e:
+                dq.kv_append(c, 1, rows, rows, None)  # (a layout that passes is refused for its slots)
+            assert ("slots" if apart(c) else "overlap") in str(e.value), (page, token, head, d)
+            assert e.value.status == "invalid_argument"
+            kinds.add(apart(c))
+    assert kinds == {True, False}
