@@ -59,6 +59,8 @@ struct AttnArgs {
   int32_t tokens = 0;
   int32_t batch = 0;
   int32_t max_q = 0;
+  int32_t part_tokens = 0;  // tokens of this launch's sequences (at most)
+  bool sliced = false;      // not the call's first sequences, or not all: their rows begin at q_offsets[0]
   const int32_t* q_offsets = nullptr;  // nullptr: one token a sequence
   const int32_t* prefix_pages = nullptr;
   const int32_t* pages = nullptr;
@@ -84,9 +86,10 @@ struct AttnPart {
   bool backward = false;  // the last rows, which see most keys, first
 };
 
-// How a call's work is split: `shared` items take the prefix with the rows of all sequences,
+// How a call's work is split: launches of `batch` sequences, one after another; `shared` items take the prefix with the rows of all sequences,
 // `own` ones a sequence's own keys (with the prefix before them where there are no shared items).
 struct AttnPlan {
+  int64_t batch = 0;
   AttnPart shared, own;
   int64_t slots = 0;  // parts of a row (0: none, every item finishes its rows)
 };

@@ -252,7 +252,11 @@ struct Item {
   int pk0, pk1;      // range of the prefix
   int ok0, ok1;      // range of the own keys
   int slot;
+  int part0;         // the row that the workspace's parts begin with
 };
+
+// The first token of a launch's sequences.
+DQ_DEV int first_token(const AttnArgs& a) { return a.sliced ? min(max(a.q_offsets[0], 0), a.tokens) : 0; }
 
 // This workgroup's item; false where there is none. `tile`: rows of a tile.
 DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int index, int tile, Item& it) {
@@ -264,15 +268,17 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   const int split = rest % w.splits;
   it.slot = w.slot + split;
   const int k0 = split * w.chunk, k1 = k0 + w.chunk;
+  const int t0 = first_token(a), end = min(a.tokens, t0 + a.part_tokens);
+  it.part0 = t0 * a.group;
   it.pk0 = it.pk1 = it.ok0 = it.ok1 = 0;
   if (stacked) {
     it.b = -1;
-    it.first = t * tile;
-    it.count = min(tile, a.tokens * a.group - it.first);
+    it.first = t0 * a.group + t * tile;
+    it.count = min(tile, end * a.group - it.first);
     it.token0 = it.own0 = it.len = 0;
     it.pk0 = k0;
     it.pk1 = min(k1, a.prefix_len);
-    return true;
+    return it.count > 0;
   }
   const int b = rest / w.splits;
   it.b = b;
@@ -280,8 +286,8 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   const int hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
   const int len = a.max_len > 0 ? a.lens[b] : 0;  // (all three under way together)
   // (whatever the offsets hold, rows stay inside the tensors)
-  const int first = min(max(lo, 0), a.tokens);
-  const int n = min(min(max(hi, first), a.tokens) - first, a.max_q);
+  const int first = min(max(lo, t0), end);
+  const int n = min(min(max(hi, first), end) - first, a.max_q);
   const int tt = w.backward ? w.tiles - 1 - t : t;
   it.count = min(tile, n * a.group - tt * tile);
   if (it.count <= 0) return false;
@@ -710,7 +716,7 @@ DQ_DEV void few_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int ind
       store4<T>(a, (int64_t)tk * a.out_token + (int64_t)h * a.out_head, 4 * d4, finish(y, sum, 1.f / sum));
       if (a.lse != nullptr && d4 == 0) a.lse[(int64_t)tk * a.heads + h] = lse_of(mx, sum, kShift<TC>);
     } else {
-      const int64_t at = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group + rw;
+      const int64_t at = ((int64_t)it.slot * ca.kv_heads + it.head) * a.part_tokens * a.group + rw - it.part0;
       *reinterpret_cast<v4f*>(a.part_o + at * a.dim + 4 * d4) = y;
       if (d4 == 0) *reinterpret_cast<v2f*>(a.part_ml + at * 2) = v2f{mx, sum};
     }
@@ -1045,7 +1051,7 @@ DQ_DEV void many_rows(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   __syncthreads();
   const bool nan = s_bad != 0;
   float* s_sum = reinterpret_cast<float*>(&s_k[0][0]);  // (the keys have been read)
-  const int64_t part = ((int64_t)it.slot * ca.kv_heads + it.head) * a.tokens * a.group;
+  const int64_t part = ((int64_t)it.slot * ca.kv_heads + it.head) * a.part_tokens * a.group - it.part0;
   auto covered = [&](int token) {
     return it.b >= 0 || a.q_offsets == nullptr || (token >= a.q_offsets[0] && token < a.q_offsets[a.batch]);
   };
@@ -1182,10 +1188,11 @@ template <int T, int TC>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, AttnPart wa, AttnPart wb) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  const int t = uniform((int)(id / a.heads)), h = uniform((int)(id % a.heads));
-  if (t >= a.tokens) return;
-  const int64_t R = (int64_t)a.tokens * a.group, step = R * a.cache.kv_heads;
-  const int64_t at = (int64_t)(h / a.group) * R + (int64_t)t * a.group + h % a.group;
+  const int of = uniform((int)(id / a.heads)), h = uniform((int)(id % a.heads));
+  const int t = first_token(a) + of;
+  if (of >= a.part_tokens || t >= a.tokens) return;
+  const int64_t R = (int64_t)a.part_tokens * a.group, step = R * a.cache.kv_heads;
+  const int64_t at = (int64_t)(h / a.group) * R + (int64_t)of * a.group + h % a.group;
   const int d = 4 * lane, most = wa.splits + wb.splits;
   const bool in = d < a.dim;
   const float* po = a.part_o + at * a.dim + (in ? d : 0);
@@ -1260,7 +1267,7 @@ hipError_t launch(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (rs == 128 && ro == 128) e = launch_items<T, TC, DP, DC, 128, 128>(a, p, s);
   }
   if (e != hipSuccess || a.part_o == nullptr) return e;
-  hipLaunchKernelGGL((k_attn_join<T, TC>), dim3((uint32_t)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(256), 0, s, a, p.shared,
+  hipLaunchKernelGGL((k_attn_join<T, TC>), dim3((uint32_t)(((int64_t)a.part_tokens * a.heads + 3) / 4)), dim3(256), 0, s, a, p.shared,
                      p.own);
   return hipGetLastError();
 }

@@ -203,6 +203,14 @@ constexpr int64_t kSharedItems = 256, kOwnItems = 512;
 // 16.4 on 7).
 constexpr int64_t kLeastKeys = 256;
 
+// Rows of a sequence that fill tiles by themselves: from here on it reads the prefix for itself.
+constexpr int64_t kFullRows = 64;
+
+// Keys of a prefix from which on a batch too large for the workspace runs in slices that share it. 4,100 / 8,192 sequences, 32 / 8
+// bf16 heads of 128, slices against every sequence's own reading: 128 keys 429 / 964 against 306 / 744 us, 256 keys 439 /
+// 981 against 403 / 941, 512 keys 448 / 992 against 652 / 1,460, 1,024 keys 473 / 1,044 against 1,212 / 2,599.
+constexpr int64_t kSliceKeys = 288;
+
 // Rows times keys (of all kv heads) up to which shared items take 64 rows and not 128: more items, each
 // sooner done. 105 / 128 / 192 / 256 rows on 1,111 / 8,192 / 8,192 / 8,192 keys of 5 / 8 / 8 / 8 heads: 14.1
 // against 16.4, 29.3 against 35.4, 38.0 against 39.1, 43.8 against 46.5 us; 128 rows on 32,768 keys of 8: 57.0 and 53.6.
@@ -218,14 +226,21 @@ void split_keys(dq::AttnPart* p, int64_t items, int64_t keys, int64_t target) {
   p->splits = (int32_t)(keys > 0 ? ceil_div(keys, p->chunk) : 1);
 }
 
-// Bytes of the parts: O and (m, l) of every slot.
-int64_t part_bytes(const dq_kv_cache* c, const dq_attention* a, int64_t slots) {
-  return slots * a->tokens * a->q->heads * (c->head_dim + 2) * 4;
+// The most tokens that a sequence, that `batch` of them can have.
+int64_t most_tokens(const dq_attention* a, int64_t batch) {
+  const int64_t max_q = std::min(a->max_q, a->tokens);
+  return max_q > a->tokens / batch ? a->tokens : std::min(a->tokens, batch * max_q);
 }
 
-dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
-  const int64_t group = a->q->heads / c->kv_heads, all = a->tokens * group;
-  const int64_t max_q = a->max_q < a->tokens ? a->max_q : a->tokens, rows = max_q * group;
+// Bytes of the parts: O and (m, l) of every slot.
+int64_t part_bytes(const dq_kv_cache* c, const dq_attention* a, int64_t tokens, int64_t slots) {
+  return slots * tokens * a->q->heads * (c->head_dim + 2) * 4;
+}
+
+// The plan of a launch of `batch` sequences.
+dq::AttnPlan plan_launch(const dq_kv_cache* c, const dq_attention* a, int64_t batch) {
+  const int64_t group = a->q->heads / c->kv_heads, tokens = most_tokens(a, batch), all = tokens * group;
+  const int64_t rows = std::min(a->max_q, a->tokens) * group;
   const bool f32 = a->q->dtype == DQ_F32;
   // (128 rows of fp32 or of heads over 128 values would leave one wave a SIMD: 432 GFLOP of prompts behind a prefix in
   // heads of 256, 1,173 us with 64 rows against 1,776)
@@ -234,28 +249,63 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
   dq::AttnPlan p;
   for (int less = 0;; ++less) {  // (fewer parts where they would not fit the workspace; at last none)
     p = dq::AttnPlan{};
+    p.batch = batch;
     p.own.rows = tile(rows);
     p.own.tiles = (int32_t)ceil_div(rows, p.own.rows);
     p.own.backward = true;
     // The prefix with all sequences' rows, unless one sequence's rows fill tiles by themselves.
-    if (a->prefix_len > 0 && a->batch > 1 && rows < 64 && (kSharedItems >> less) > 0) {
+    if (a->prefix_len > 0 && batch > 1 && rows < kFullRows && (kSharedItems >> less) > 0) {
       p.shared.rows = all > 16 && all * a->prefix_len * c->kv_heads <= kSmallShared ? 64 : tile(all);
       p.shared.tiles = (int32_t)ceil_div(all, p.shared.rows);
       split_keys(&p.shared, p.shared.tiles * c->kv_heads, a->prefix_len, kSharedItems >> less);
       if (a->max_len > 0) {
-        split_keys(&p.own, a->batch * p.own.tiles * c->kv_heads, a->max_len, kOwnItems >> less);
+        split_keys(&p.own, batch * p.own.tiles * c->kv_heads, a->max_len, kOwnItems >> less);
         p.own.slot = p.shared.splits;
       }
     } else {
       p.own.with_prefix = a->prefix_len > 0;
       p.own.own_from = (int32_t)(ceil_div(a->prefix_len, 128) * 128);
-      const int64_t items = a->batch * p.own.tiles * c->kv_heads;
+      const int64_t items = batch * p.own.tiles * c->kv_heads;
       split_keys(&p.own, items, p.own.own_from + a->max_len, kOwnItems >> less);
     }
     const int64_t slots = p.shared.splits + p.own.splits;
     p.slots = slots > 1 ? slots : 0;
-    if (part_bytes(c, a, p.slots) <= (int64_t)DQ_ATTENTION_WORKSPACE_BYTES) return p;
+    if (part_bytes(c, a, tokens, p.slots) <= (int64_t)DQ_ATTENTION_WORKSPACE_BYTES) return p;
   }
+}
+
+// A batch whose rows leave more than the workspace in two parts each (a shared one and an own one) runs in slices of
+// whole sequences, so that the prefix is read once a slice and not once a sequence; a prefix of less than
+// kSliceKeys keys is read by every sequence then.
+dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
+  int64_t batch = a->batch;
+  const int64_t max_q = std::min(a->max_q, a->tokens);
+  if (a->prefix_len >= kSliceKeys && a->max_len > 0 && batch > 1 && max_q * (a->q->heads / c->kv_heads) < kFullRows) {
+    const int64_t fit = (int64_t)DQ_ATTENTION_WORKSPACE_BYTES / part_bytes(c, a, 1, 2);
+    if (a->tokens > fit && fit >= 2 * max_q) batch = ceil_div(batch, ceil_div(batch, fit / max_q));
+  }
+  return plan_launch(c, a, batch);
+}
+
+// The launch of `batch` sequences from sequence b on, of a call in launches of p.batch.
+hipError_t launch_slice(const dq_kv_cache* c, const dq_attention* a, const dq::AttnPlan& p, dq::AttnArgs r, int64_t b, hipStream_t s) {
+  const int64_t batch = std::min(p.batch, a->batch - b);
+  r.batch = (int32_t)batch;
+  r.part_tokens = (int32_t)most_tokens(a, batch);
+  r.lens = a->max_len > 0 ? a->lens + b : nullptr;
+  r.pages = a->max_len > 0 ? a->pages + b * a->pages_stride : nullptr;
+  if (a->q_offsets != nullptr) {
+    r.q_offsets = a->q_offsets + b;
+    r.tokens = (int32_t)a->tokens;
+    r.sliced = batch < a->batch;
+  } else {  // one token each
+    const int64_t bytes = float_bytes(a->q->dtype);
+    r.tokens = (int32_t)batch;
+    r.q = static_cast<const char*>(r.q) + b * r.q_token * bytes;
+    r.out = static_cast<char*>(r.out) + b * r.out_token * bytes;
+    if (r.lse != nullptr) r.lse += b * r.heads;
+  }
+  return dq::launch_attention(a->q->dtype, c->dtype, r, p, s);
 }
 
 bool aligned(const dq_heads* r, size_t bytes) {
@@ -276,13 +326,8 @@ dq::AttnArgs attn_args(const dq_kv_cache* c, const dq_attention* a) {
   r.heads = a->q->heads;
   r.group = a->q->heads / c->kv_heads;
   r.dim = c->head_dim;
-  r.tokens = (int32_t)a->tokens;
-  r.batch = (int32_t)a->batch;
-  r.max_q = (int32_t)(a->max_q < a->tokens ? a->max_q : a->tokens);
-  r.q_offsets = a->q_offsets;
+  r.max_q = (int32_t)std::min(a->max_q, a->tokens);
   r.prefix_pages = a->prefix_pages;
-  r.pages = a->pages;
-  r.lens = a->lens;
   r.pages_stride = a->pages_stride;
   r.prefix_len = (int32_t)a->prefix_len;
   r.max_len = (int32_t)a->max_len;
@@ -359,7 +404,8 @@ int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, co
 int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a) {
   if (check_attention(cache, a, false) != DQ_OK) return -1;
   if (a->tokens == 0 || a->batch == 0) return 0;
-  return part_bytes(cache, a, plan(cache, a).slots);
+  const dq::AttnPlan p = plan(cache, a);
+  return part_bytes(cache, a, most_tokens(a, p.batch), p.slots);
 }
 
 int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace, int64_t workspace_bytes,
@@ -374,16 +420,18 @@ int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* w
   const dq::AttnPlan p = plan(cache, a);
   dq::AttnArgs args = attn_args(cache, a);
   if (p.slots > 0) {
-    const int64_t need = part_bytes(cache, a, p.slots);
+    const int64_t tokens = most_tokens(a, p.batch), need = part_bytes(cache, a, tokens, p.slots);
     if (workspace == nullptr) return bad("workspace: null argument");
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return bad("workspace: must be 16-byte aligned");
     if (workspace_bytes < need)
       return dq::set_error(DQ_RESOURCE_EXHAUSTED, "workspace: %lld bytes, the call needs %lld", (ll)workspace_bytes, (ll)need);
     args.part_o = static_cast<float*>(workspace);
-    args.part_ml = args.part_o + p.slots * a->tokens * a->q->heads * cache->head_dim;
+    args.part_ml = args.part_o + p.slots * tokens * a->q->heads * cache->head_dim;
   }
-  const hipError_t e = dq::launch_attention(a->q->dtype, cache->dtype, args, p, static_cast<hipStream_t>(stream));
-  return e == hipSuccess ? DQ_OK : hip_fail(e, "shared_attention launch");
+  for (int64_t b = 0; b < a->batch; b += p.batch)
+    if (const hipError_t e = launch_slice(cache, a, p, args, b, static_cast<hipStream_t>(stream)); e != hipSuccess)
+      return hip_fail(e, "shared_attention launch");
+  return DQ_OK;
 }
 
 }  // extern "C"

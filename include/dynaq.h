@@ -521,7 +521,10 @@ DQ_API int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads
  * An infinite or NaN value of a key makes its column infinite or NaN in every row that sees the key, however
  * small the key's weight, and reaches no other row. With fp32 q an infinite query or key may give NaN where its scores
  * are infinite (products are summed in parts).
- * The prefix is read once for the whole batch, not once a sequence. A row's bits depend on the call's shape (batch, tokens,
+ * While a sequence has fewer than 64 rows of a kv head (max_q * q heads / kv heads) the prefix is read once for the rows
+ * of all sequences together; from 64 on, where a sequence's rows fill tiles by themselves, each sequence reads it. A batch
+ * too large for DQ_ATTENTION_WORKSPACE_BYTES runs in slices of whole sequences, each of which reads the prefix once (a prefix
+ * of less than some 300 keys is read by every sequence then). A row's bits depend on the call's shape (batch, tokens,
  * max_q, prefix_len, max_len), not on timing. Rows outside every sequence are not written.
  * A row that would read a page number outside [0, n_pages) gets NaN; so may rows of its sequence beside it (all
  * rows, for a page of the prefix).

@@ -154,3 +154,14 @@ def test_append_refuses_caches_whose_places_overlap():
             assert e.value.status == "invalid_argument"
             kinds.add(apart(c))
     assert kinds == {True, False}
+
+
+def test_large_batches_go_on_sharing_the_prefix():
+    """More rows than the workspace holds parts of: the batch runs in slices, whose parts are counted here (32 / 8 heads
+    of 128; two parts a row of 32 x 130 floats)."""
+    c = cache(k=None, v=None, kv_heads=8, head_dim=128, token_stride=1024, head_stride=128, page_stride=1 << 14)
+    q = heads(p=None, dtype=dq.F16, heads=32, token_stride=4096, head_stride=128)
+    for tokens, batch, max_q, a_slice in ((4000, 4000, 1, 4000), (4096, 4096, 1, 2048), (4096, 1024, 4, 2048), (4096, 512, 8, 2048),
+                                          (20000, 20000, 1, 4000), (5000, 1500, 7, 500 * 7)):
+        n = dq.shared_attention_workspace(c, q, q, tokens, batch, max_q, 8192, 64, 512)
+        assert n == 2 * a_slice * 32 * 130 * 4 <= dq.ATTENTION_WORKSPACE_BYTES, (tokens, batch, max_q, n)

@@ -570,3 +570,26 @@ def test_more_rows_than_a_launch_has_threads_for(cuda, rot):
     slots = tokens - 1 - torch.arange(tokens, device="cuda")
     dq.kv_append(B.kv_cache(k, v), tokens, B.heads(x), B.heads(x), slots, w, 1e-5, rope, pos, stream())
     assert torch.equal(k.view(-1, heads, dim)[:tokens].flip(0), out) and torch.equal(v.view(-1, heads, dim)[:tokens].flip(0), x)
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("new,hq,hk,dim,tail", [([1] * 4100, 32, 8, 128, 0), ([i % 9 for i in range(1300)], 16, 4, 256, 3), ([1] * 8200, 16, 16, 128, 0)],
+                         ids=["one token", "up to 8 tokens", "one token, 3 slices"])
+def test_large_batches_run_in_slices(cuda, type, cache, new, hq, hk, dim, tail):
+    """More rows than the workspace holds parts of: slices of the batch share the prefix, each row is its sequence's."""
+    lens = [n + i % 5 for i, n in enumerate(new)]
+    c = build(61, new, lens, 300, hq, hk, dim, type, cache, 16, tail=tail)
+    out, lse = torch.full_like(c["q"], 55.0), torch.full((c["tokens"], hq), 33.0, device="cuda")
+    call(c, out=out, lse=lse)
+    n, at, start = sum(new), [], 0
+    every = len(new) // 23
+    for b, k in enumerate(new):
+        at += range(start, start + k) if b % every == 0 else ()
+        start += k
+    want, want_lse, bound, lse_bound = B.attention_by_heads(c["q"][at], c["ks"][::every], c["vs"][::every], new[::every], lens[::every], 300,
+                                                            c["scale"], type, cache)
+    B.close(out[at], want, bound, type)
+    B.close(lse[at], want_lse, lse_bound, "f32")
+    assert torch.all(out[n:] == 55.0) and torch.all(lse[n:] == 33.0) and torch.isfinite(out).all() and torch.isfinite(lse).all()
+    if max(new) == 1:
+        assert torch.equal(call(c, out=torch.empty_like(out), no_offsets=True), out)
