@@ -153,6 +153,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int64_t kMaxRows = (int64_t)1 << 31;   // head rows of a call: they are counted in 32 bits
 constexpr int64_t kMaxHeads = (int64_t)1 << 25;  // heads of a token: its rows run in one launch
 
+// Workgroups of an attention launch stay below this: a dispatch counts its threads, 256 a workgroup, in 32 bits.
+constexpr int64_t kMaxGroups = (int64_t)1 << 24;
+// Rows of a sequence that fill tiles by themselves: from here on it reads the prefix for itself.
+constexpr int64_t kFullRows = 64;
+
 int check_tokens(int64_t tokens, int64_t heads) {
   if (tokens < 0) return bad("tokens must be >= 0");
   if (tokens > kMaxRows / heads || heads > kMaxHeads) return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %lld heads are too many", (ll)tokens, (ll)heads);
@@ -179,6 +184,8 @@ int check_attention(const dq_kv_cache* c, const dq_attention* a, bool data) {
   const int64_t most_q = a->max_q < a->tokens ? a->max_q : a->tokens;
   if (a->batch > INT32_MAX / 2 / a->q->heads || a->batch * (most_q * (a->q->heads / c->kv_heads) / 16 + 1) > INT32_MAX / 2 / c->kv_heads)
     return dq::set_error(DQ_UNSUPPORTED, "%lld sequences of up to %lld tokens are too many", (ll)a->batch, (ll)a->max_q);
+  if ((most_q * (a->q->heads / c->kv_heads) / kFullRows + 1) * c->kv_heads >= kMaxGroups)  // (of one sequence)
+    return dq::set_error(DQ_UNSUPPORTED, "%lld tokens of %d heads are too many for a launch", (ll)most_q, a->q->heads);
   if (data && a->q_offsets == nullptr && (a->tokens != a->batch || a->max_q != 1))
     return bad("without q_offsets every sequence has one token");
   const int64_t most = (int64_t)1 << 29;
@@ -202,9 +209,6 @@ constexpr int64_t kSharedItems = 256, kOwnItems = 512;
 // Keys that are worth an item of their own (128: 20.2 us against 19.3 on 32 short sequences, 15.9 against
 // 16.4 on 7).
 constexpr int64_t kLeastKeys = 256;
-
-// Rows of a sequence that fill tiles by themselves: from here on it reads the prefix for itself.
-constexpr int64_t kFullRows = 64;
 
 // Keys of a prefix from which on a batch too large for the workspace runs in slices that share it. 4,100 / 8,192 sequences, 32 / 8
 // bf16 heads of 128, slices against every sequence's own reading: 128 keys 429 / 964 against 306 / 744 us, 256 keys 439 /
@@ -274,9 +278,13 @@ dq::AttnPlan plan_launch(const dq_kv_cache* c, const dq_attention* a, int64_t ba
   }
 }
 
-// A batch whose rows leave more than the workspace in two parts each (a shared one and an own one) runs in slices of
-// whole sequences, so that the prefix is read once a slice and not once a sequence; a prefix of less than
-// kSliceKeys keys is read by every sequence then.
+int64_t workgroups(const dq_kv_cache* c, const dq::AttnPlan& p) {
+  return ((int64_t)p.shared.tiles * p.shared.splits + (int64_t)p.own.tiles * p.own.splits * p.batch) * c->kv_heads;
+}
+
+// A batch of more items than a launch takes runs in slices of whole sequences, and so does one whose rows leave more than the
+// workspace in two parts each (a shared one and an own one), so that the prefix is read once a slice and not once a
+// sequence; a prefix of less than kSliceKeys keys is read by every sequence then.
 dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
   int64_t batch = a->batch;
   const int64_t max_q = std::min(a->max_q, a->tokens);
@@ -284,7 +292,9 @@ dq::AttnPlan plan(const dq_kv_cache* c, const dq_attention* a) {
     const int64_t fit = (int64_t)DQ_ATTENTION_WORKSPACE_BYTES / part_bytes(c, a, 1, 2);
     if (a->tokens > fit && fit >= 2 * max_q) batch = ceil_div(batch, ceil_div(batch, fit / max_q));
   }
-  return plan_launch(c, a, batch);
+  dq::AttnPlan p = plan_launch(c, a, batch);
+  while (batch > 1 && workgroups(c, p) >= kMaxGroups) p = plan_launch(c, a, batch = ceil_div(batch, 2));
+  return p;
 }
 
 // The launch of `batch` sequences from sequence b on, of a call in launches of p.batch.

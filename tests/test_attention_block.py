@@ -165,3 +165,12 @@ def test_large_batches_go_on_sharing_the_prefix():
                                           (20000, 20000, 1, 4000), (5000, 1500, 7, 500 * 7)):
         n = dq.shared_attention_workspace(c, q, q, tokens, batch, max_q, 8192, 64, 512)
         assert n == 2 * a_slice * 32 * 130 * 4 <= dq.ATTENTION_WORKSPACE_BYTES, (tokens, batch, max_q, n)
+
+
+def test_a_sequence_runs_in_one_launch():
+    """2^24 workgroups have more threads than a launch counts: 128 tokens of 2^23 kv heads are refused, not tried."""
+    kv = 1 << 23
+    c = cache(kv_heads=kv, token_stride=64, head_stride=1024, page_stride=1024 * kv)
+    q = heads(dtype=dq.F16, heads=kv, token_stride=64 * kv)
+    with pytest.raises(dq.DqError, match="too many for a launch"):
+        dq.shared_attention_workspace(c, q, q, 128, 1, 128, 0, 8, 128)

@@ -593,3 +593,16 @@ def test_large_batches_run_in_slices(cuda, type, cache, new, hq, hk, dim, tail):
     assert torch.all(out[n:] == 55.0) and torch.all(lse[n:] == 33.0) and torch.isfinite(out).all() and torch.isfinite(lse).all()
     if max(new) == 1:
         assert torch.equal(call(c, out=torch.empty_like(out), no_offsets=True), out)
+
+
+@pytest.mark.parametrize("offsets", [True, False])
+def test_more_items_than_a_launch_has_threads_for(cuda, offsets):
+    """2^24 items and some, in several launches: each of 2^21 sequences has one key, whose value it gets as it is."""
+    n, heads, dim, page = (1 << 21) + 3, 8, 8, 16
+    k, v = (torch.randn((64, page, heads, dim), device="cuda").half() for _ in range(2))
+    q = torch.randn((n, heads, dim), device="cuda").half()
+    out, lens = torch.full_like(q, math.nan), torch.ones(n, dtype=torch.int32, device="cuda")
+    pages = torch.randint(0, 64, (n, 1), dtype=torch.int32, device="cuda")
+    at = torch.arange(n + 1, dtype=torch.int32, device="cuda") if offsets else None
+    dq.shared_attention(B.kv_cache(k, v), B.heads(q), B.heads(out), None, n, n, at, 1, None, 0, pages, 1, lens, 1, 1.0, None, 0, stream())
+    assert torch.equal(out, v[pages[:, 0].long(), 0])
