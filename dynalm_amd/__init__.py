@@ -399,7 +399,7 @@ def shared_attention_workspace(cache: KvCache, q: Heads, out: Heads, tokens: int
     a = _attention(q, out, None, tokens, batch, None, max_q, None, prefix_len, None, pages_stride, None, max_len, scale)
     n = lib().dq_shared_attention_workspace(cache, a)
     if n < 0:
-        raise DqError(1, lib().dq_last_error().decode(errors="replace"))
+        _check(-n)
     return int(n)
 
 

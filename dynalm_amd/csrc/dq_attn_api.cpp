@@ -412,7 +412,7 @@ int dq_kv_append(const dq_kv_cache* cache, int64_t tokens, const dq_heads* k, co
 }
 
 int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a) {
-  if (check_attention(cache, a, false) != DQ_OK) return -1;
+  if (int rc = check_attention(cache, a, false); rc != DQ_OK) return -rc;
   if (a->tokens == 0 || a->batch == 0) return 0;
   const dq::AttnPlan p = plan(cache, a);
   return part_bytes(cache, a, most_tokens(a, p.batch), p.slots);

@@ -552,8 +552,8 @@ typedef struct dq_attention {
 /* Bytes that any dq_shared_attention call can do with. */
 #define DQ_ATTENTION_WORKSPACE_BYTES (128u << 20)
 
-/* Workspace bytes of a call (0: none; -1 with dq_last_error() set if the arguments are
- * refused). A function of the shape only: the device pointers in it may be NULL. */
+/* Workspace bytes of a call (0: none; minus the status, with dq_last_error() set, if the
+ * arguments are refused). A function of the shape only: the device pointers in it may be NULL. */
 DQ_API int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_attention* a);
 DQ_API int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace,
                                int64_t workspace_bytes, void* stream);

@@ -174,3 +174,12 @@ def test_a_sequence_runs_in_one_launch():
     q = heads(dtype=dq.F16, heads=kv, token_stride=64 * kv)
     with pytest.raises(dq.DqError, match="too many for a launch"):
         dq.shared_attention_workspace(c, q, q, 128, 1, 128, 0, 8, 128)
+
+
+def test_the_workspace_query_is_refused_with_the_calls_status():
+    def ask(q=heads(), most=16):
+        return dq.shared_attention_workspace(cache(), q, q, 1, 1, 1, 0, 1, most)
+
+    assert ask() == 0
+    refused("invalid_argument", ask, most=17)
+    refused("unsupported", ask, q=heads(dtype=7))
