@@ -246,8 +246,8 @@ dq::AttnPlan plan_launch(const dq_kv_cache* c, const dq_attention* a, int64_t ba
   const int64_t group = a->q->heads / c->kv_heads, tokens = most_tokens(a, batch), all = tokens * group;
   const int64_t rows = std::min(a->max_q, a->tokens) * group;
   const bool f32 = a->q->dtype == DQ_F32;
-  // (128 rows of fp32 or of heads over 128 values would leave one wave a SIMD: 432 GFLOP of prompts behind a prefix in
-  // heads of 256, 1,173 us with 64 rows against 1,776)
+  // (128 rows of fp32 or of heads over 128 values would leave one wave a SIMD: 864 GFLOP of prompts behind a prefix in
+  // heads of 256, 1,143 to 1,174 us with 64 rows against 1,776)
   const bool wide = !f32 && c->head_dim <= 128;
   auto tile = [&](int64_t n) { return n <= 16 ? 16 : n <= 64 || !wide ? 64 : 128; };
   dq::AttnPlan p;

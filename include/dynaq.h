@@ -454,7 +454,7 @@ typedef enum dq_rope_style {
  * cosine and sine are cos[p * rot_dim / 2 + i] and sin[p * rot_dim / 2 + i] (device memory,
  * max_pos rows each); values from rot_dim on stay as they are. The tables carry whatever
  * frequency scaling the model uses. A token whose position is not in [0, max_pos) gets NaN
- * in place of its rotated heads. */
+ * in the first rot_dim values of its heads. */
 typedef struct dq_rope {
   const float* cos;
   const float* sin;
