@@ -268,17 +268,18 @@ DQ_DEV bool find_item(const AttnArgs& a, const AttnPart& w, bool stacked, int in
   const int split = rest % w.splits;
   it.slot = w.slot + split;
   const int k0 = split * w.chunk, k1 = k0 + w.chunk;
-  const int t0 = first_token(a), end = min(a.tokens, t0 + a.part_tokens);
+  const int t0 = first_token(a), end = t0 + min(a.part_tokens, a.tokens - t0);
   it.part0 = t0 * a.group;
   it.pk0 = it.pk1 = it.ok0 = it.ok1 = 0;
   if (stacked) {
     it.b = -1;
+    it.count = min(tile, (end - t0) * a.group - t * tile);
+    if (it.count <= 0) return false;
     it.first = t0 * a.group + t * tile;
-    it.count = min(tile, end * a.group - it.first);
     it.token0 = it.own0 = it.len = 0;
     it.pk0 = k0;
     it.pk1 = min(k1, a.prefix_len);
-    return it.count > 0;
+    return true;
   }
   const int b = rest / w.splits;
   it.b = b;

@@ -606,3 +606,21 @@ def test_more_items_than_a_launch_has_threads_for(cuda, offsets):
     at = torch.arange(n + 1, dtype=torch.int32, device="cuda") if offsets else None
     dq.shared_attention(B.kv_cache(k, v), B.heads(q), B.heads(out), None, n, n, at, 1, None, 0, pages, 1, lens, 1, 1.0, None, 0, stream())
     assert torch.equal(out, v[pages[:, 0].long(), 0])
+
+
+@pytest.mark.parametrize("new,max_q", [([3, 0, 5, 1, 2, 4, 2], 6), ([40, 33, 20, 1, 2, 4, 30], 64), ([1 + i % 2 for i in range(3000)], 2)],
+                         ids=["few rows", "tiles", "slices"])
+def test_offsets_of_any_values_stay_inside_the_tensors(cuda, new, max_q):
+    """Offsets that decrease or leave the tokens: rows past the tensors' ends and the workspace's are not touched."""
+    c = build(67, new, [n + 20 for n in new], 300, 32, 8, 128, "bf16", "bf16", 16)
+    gen = torch.Generator().manual_seed(5)
+    wide = torch.full((c["tokens"] + 20, 32, 128), 55.0, dtype=torch.bfloat16, device="cuda")
+    lse = torch.full((c["tokens"] + 20, 32), 33.0, device="cuda")
+    q = torch.zeros_like(wide)
+    q[10:-10] = c["q"]
+    c["q"] = q[10:-10]
+    for low, high in ((-(2**31), 2**31 - 1), (-5, c["tokens"] + 5)):
+        c["offsets"] = torch.randint(low, high, (len(new) + 1,), generator=gen).to(torch.int32).cuda()
+        call(c, out=wide[10:-10], lse=lse[10:-10], max_q=max_q)
+        for x, value in ((wide, 55.0), (lse, 33.0)):
+            assert torch.all(x[:10] == value) and torch.all(x[-10:] == value)
