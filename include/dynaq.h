@@ -471,7 +471,7 @@ typedef struct dq_rope {
  * norm). rope NULL: no rotation (positions is not read), else positions has one entry a token.
  * k and k_out may be NULL (both): queries alone. All arithmetic is fp32, rounded once to the
  * output's type (to nearest even). An output may be its input (the same pointer, type and
- * strides), and must not overlap an input otherwise. */
+ * strides), and must not overlap an input otherwise, nor the other output. Up to 2^31 head rows, 2^25 heads a token. */
 DQ_API int dq_qk_norm_rope(int64_t tokens, int64_t head_dim, const dq_heads* q, const dq_heads* q_out,
                            const float* q_weight, const dq_heads* k, const dq_heads* k_out, const float* k_weight,
                            float eps, const dq_rope* rope, const int32_t* positions, void* stream);
