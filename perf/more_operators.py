@@ -232,7 +232,8 @@ def _run_own(s: dict):
                         stream)
         return s["chosen"]
     if kind == "mass":
-        dq.attention_mass(cache, seqs, q, s["lse"], s["scale"], c["decay"], s["mass"], *s["mass"].stride()[:2], stream)
+        dq.attention_mass(cache, seqs, q, s["lse"], s["scale"], c["decay"], s["mass"], *s["mass"].stride()[:2], s["workspace"],
+                          WORKSPACE_BYTES, stream)
         return s["mass"]
     out = dq.Heads(s["out"].data_ptr(), kinds[s["out"].dtype], c["heads"], s["out"].stride(0), s["out"].stride(1))
     dq.page_attention(cache, seqs, q, out, s["lse"], s["chosen"], c["count"], s["scale"], s["workspace"], WORKSPACE_BYTES, stream)
