@@ -42,6 +42,8 @@ __all__ = [
     "SILU", "GELU", "GELU_TANH", "act_mul", "matmul_gated", "GgufFile", "GgufTensor", "EXPORTS",
     "F32", "F16", "BF16", "ROPE_HALVES", "ROPE_PAIRS", "MAX_HEAD_DIM", "Heads", "Rope", "KvCache", "Attention", "qk_norm_rope",
     "kv_append", "shared_attention", "shared_attention_workspace", "ATTENTION_WORKSPACE_BYTES",
+    "Sequences", "page_bounds", "choose_pages", "choose_pages_workspace", "page_attention", "page_attention_workspace",
+    "attention_mass", "attention_mass_workspace", "kv_keep", "kv_compact",
     "MatmulShape", "External", "matmul_noalloc", "NOALLOC_SCRATCH_BYTES", "Plan", "Selection",
     "plan_defaults", "plan_ffn_down", "select", "matmul_plan", "KERNEL_NAMES", "KERNEL_QMM_GEMM", "KERNEL_QMM_GEMV",
 ]
@@ -410,6 +412,99 @@ def shared_attention(cache: KvCache, q: Heads, out: Heads, lse, tokens: int, bat
     a = _attention(q, out, lse, tokens, batch, q_offsets, max_q, prefix_pages, prefix_len, pages, pages_stride, lens,
                    max_len, scale)
     rc = lib().dq_shared_attention(cache, a, _ptr(workspace), workspace_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+# ---------------------------------------------------------------- long caches
+
+
+class Sequences(C.Structure):
+    """dq_sequences: a batch's rows and keys, Sequences(batch, tokens, q_offsets, max_q, pages, pages_stride, lens, max_len)."""
+    _fields_ = [("batch", _I64), ("tokens", _I64), ("q_offsets", _P), ("max_q", _I64), ("pages", _P), ("pages_stride", _I64),
+                ("lens", _P), ("max_len", _I64)]
+
+
+_SEQUENCES = C.POINTER(Sequences)
+EXPORTS |= {
+    "dq_page_bounds": (_I, [_CACHE, _SEQUENCES, _P, _I64, _P, _P]),
+    "dq_choose_pages_workspace": (_I64, [_CACHE, _SEQUENCES]),
+    "dq_choose_pages": (_I, [_CACHE, _SEQUENCES, _HEADS, _P, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "dq_page_attention_workspace": (_I64, [_CACHE, _SEQUENCES, _HEADS, _I64]),
+    "dq_page_attention": (_I, [_CACHE, _SEQUENCES, _HEADS, _HEADS, _P, _P, _I64, C.c_float, _P, _I64, _P]),
+    "dq_attention_mass_workspace": (_I64, [_CACHE, _SEQUENCES, _HEADS]),
+    "dq_attention_mass": (_I, [_CACHE, _SEQUENCES, _HEADS, _P, C.c_float, C.c_float, _P, _I64, _I64, _P, _I64, _P]),
+    "dq_kv_keep": (_I, [_SEQUENCES, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "dq_kv_compact": (_I, [_CACHE, _SEQUENCES, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P]),
+}
+
+
+def _bytes(n: int) -> int:
+    if n < 0:
+        _check(-n)
+    return int(n)
+
+
+def page_bounds(cache: KvCache, seqs: Sequences, from_, max_new: int, bounds, stream: int = 0) -> None:
+    """Each channel's smallest and largest value over the pages of the keys from from_[b] on (None: of all keys) (dq_page_bounds)."""
+    rc = lib().dq_page_bounds(cache, seqs, _ptr(from_), max_new, _ptr(bounds), stream)
+    if rc:
+        _check(rc)
+
+
+def choose_pages_workspace(cache: KvCache, seqs: Sequences) -> int:
+    """Workspace bytes of a choose_pages call of this shape (no GPU needed)."""
+    return _bytes(lib().dq_choose_pages_workspace(cache, seqs))
+
+
+def choose_pages(cache: KvCache, seqs: Sequences, q: Heads, bounds, first: int, last: int, count: int, chosen, workspace,
+                 workspace_bytes: int, stream: int = 0) -> None:
+    """The `count` pages that each row reads in each kv head, by their bounds (dq_choose_pages)."""
+    rc = lib().dq_choose_pages(cache, seqs, q, _ptr(bounds), first, last, count, _ptr(chosen), _ptr(workspace), workspace_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def page_attention_workspace(cache: KvCache, seqs: Sequences, q: Heads, count: int) -> int:
+    """Workspace bytes of a page_attention call of this shape (no GPU needed)."""
+    return _bytes(lib().dq_page_attention_workspace(cache, seqs, q, count))
+
+
+def page_attention(cache: KvCache, seqs: Sequences, q: Heads, out: Heads, lse, chosen, count: int, scale: float, workspace,
+                   workspace_bytes: int, stream: int = 0) -> None:
+    """out = attention of q over the keys of each row's chosen pages (dq_page_attention)."""
+    rc = lib().dq_page_attention(cache, seqs, q, out, _ptr(lse), _ptr(chosen), count, scale, _ptr(workspace), workspace_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def attention_mass_workspace(cache: KvCache, seqs: Sequences, q: Heads) -> int:
+    """Workspace bytes of an attention_mass call of this shape (no GPU needed)."""
+    return _bytes(lib().dq_attention_mass_workspace(cache, seqs, q))
+
+
+def attention_mass(cache: KvCache, seqs: Sequences, q: Heads, lse, scale: float, decay: float, mass, seq_stride: int,
+                   head_stride: int, workspace, workspace_bytes: int, stream: int = 0) -> None:
+    """mass = decay * mass + the attention weight that each key gathers from the rows (dq_attention_mass)."""
+    rc = lib().dq_attention_mass(cache, seqs, q, _ptr(lse), scale, decay, _ptr(mass), seq_stride, head_stride, _ptr(workspace),
+                                 workspace_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def kv_keep(seqs: Sequences, kv_heads: int, mass, seq_stride: int, head_stride: int, first: int, last: int, budget: int, kept,
+            kept_lens=None, stream: int = 0) -> None:
+    """The places of the `budget` keys that stay in each kv head, by their mass (dq_kv_keep)."""
+    rc = lib().dq_kv_keep(seqs, kv_heads, _ptr(mass), seq_stride, head_stride, first, last, budget, _ptr(kept), _ptr(kept_lens), stream)
+    if rc:
+        _check(rc)
+
+
+def kv_compact(cache: KvCache, seqs: Sequences, kept, budget: int, to_pages=None, to_stride: int = 0, mass=None, mass_out=None,
+               seq_stride: int = 0, head_stride: int = 0, stream: int = 0) -> None:
+    """The kept keys and values (and masses) to the front of to_pages, or of the sequences' own (dq_kv_compact)."""
+    rc = lib().dq_kv_compact(cache, seqs, _ptr(kept), budget, _ptr(to_pages), to_stride, _ptr(mass), _ptr(mass_out), seq_stride,
+                             head_stride, stream)
     if rc:
         _check(rc)
 

@@ -558,6 +558,98 @@ DQ_API int64_t dq_shared_attention_workspace(const dq_kv_cache* cache, const dq_
 DQ_API int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* ---- long caches: the pages that a query reads, the keys that stay ----------
+ * Beside dense attention over the pages of a cache: a decode step that reads the pages on
+ * which its queries may score high, and nothing else (dq_page_bounds after an append,
+ * dq_choose_pages, dq_page_attention); and a cache that keeps the keys which attention has
+ * weighed most (dq_attention_mass after an attention that wrote lse, dq_kv_keep and
+ * dq_kv_compact now and then; dq_page_bounds again). What is said of the attention block's
+ * calls holds for these: the current device, the given stream, no memory of the library's;
+ * lengths, offsets, page numbers, chosen pages and kept places are device memory, and
+ * whatever they hold, no access leaves the buffers that the arguments describe. */
+
+/* The keys and the query rows of a batch. Sequence b's keys are the lens[b] (at most max_len)
+ * first places of the pages pages[b * pages_stride], ...; its rows are the tokens [q_offsets[b],
+ * q_offsets[b + 1]) of all rows (batch + 1 entries from 0 on, not decreasing, at most max_q apart;
+ * NULL: one row each), the last of its keys are theirs: row i of n sees the keys j <= lens[b] - n +
+ * i. Rows outside every sequence are not written. */
+typedef struct dq_sequences {
+  int64_t batch;
+  int64_t tokens;
+  const int32_t* q_offsets;
+  int64_t max_q;
+  const int32_t* pages;
+  int64_t pages_stride;
+  const int32_t* lens;
+  int64_t max_len;
+} dq_sequences;
+
+/* The smallest and the largest value of each channel over a page's keys:
+ *     bounds[p][h][0][d] = min_j k_j[d],  bounds[p][h][1][d] = max_j k_j[d]
+ * (n_pages x kv_heads x 2 x head_dim values of the cache's type, 16-byte aligned), for the pages that hold one
+ * of sequence b's keys from[b], from[b] + 1, ..., lens[b] - 1 (at most max_new of them; from NULL: all keys, max_new
+ * is not read); bounds take all of such a page's keys below lens[b]. Other pages' are left as they are. A NaN
+ * among the values makes both NaN. Of the zeros -0 is the smaller. A page that several sequences list gets the bounds of one of
+ * them. The rows of `s` (tokens, q_offsets, max_q) are not read. */
+DQ_API int dq_page_bounds(const dq_kv_cache* cache, const dq_sequences* s, const int32_t* from, int64_t max_new,
+                          void* bounds, void* stream);
+
+/* The pages that each row reads in each kv head, by an upper bound of what it can score on a page:
+ *     s_p = max over the query heads h of the kv head of sum_d q[t, h, d] (q[t, h, d] > 0 ? hi_p[d] : lo_p[d])
+ * with the bounds of dq_page_bounds; sums are 64 bits wide. Of the pages that hold keys which row t sees: the
+ * first `first`, the last `last` (1 at least), and of the others those of largest s_p (of equal ones the
+ * lower; a NaN is above all numbers) until there are `count`. chosen[t][g][i] (tokens x kv_heads x count) is the i-th such page,
+ * as an index into the sequence's pages, ascending; -1 where there are no more. A page number outside [0, n_pages) counts as
+ * a score of NaN. The cache's k and v are not read and may be NULL. q: fp32 or the cache's type.
+ * first + last <= count.
+ * workspace: dq_choose_pages_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
+DQ_API int64_t dq_choose_pages_workspace(const dq_kv_cache* cache, const dq_sequences* s);
+DQ_API int dq_choose_pages(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, const void* bounds,
+                           int64_t first, int64_t last, int64_t count, int32_t* chosen, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* dq_shared_attention's rows over the keys of chosen pages alone:
+ *     out[t, h] = sum_j p_j v_j,  p = softmax over the visible j on a chosen page of scale * q[t, h] . k_j
+ * chosen is dq_choose_pages' list, or any other of that form: tokens x kv_heads x count indices into a sequence's pages, in any
+ * order; entries outside the pages that hold visible keys are left out, a page that is given twice counts twice. Types, rounding, lse, infinite and NaN
+ * values, rows without keys and page numbers outside the cache (of a chosen page) are as there.
+ * workspace: dq_page_attention_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
+DQ_API int64_t dq_page_attention_workspace(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, int64_t count);
+DQ_API int dq_page_attention(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, const dq_heads* out,
+                             float* lse, const int32_t* chosen, int64_t count, float scale, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* The attention weight that each key gathers in each kv head, over the rows and the query heads of the kv head:
+ *     mass[b][g][j] = decay * mass[b][g][j] + sum of exp(scale * q[t, h] . k_j - lse[t, h]) over b's rows t that see j
+ * for j < lens[b]; the keys of the rows themselves (the last n) have no earlier mass, and with decay 0 no key has: then
+ * mass is not read. lse: tokens x q heads floats, as dq_shared_attention writes it; a row whose lse is -inf adds nothing, one
+ * whose lse is NaN makes the mass of the keys that it sees NaN.
+ * mass[b][g][j] is at mass + b * seq_stride + g * head_stride + j; from lens[b] on it is left as it is. Sums are fp32
+ * and do not depend on timing. q: fp32 or the cache's type; the cache's v is not read and may be NULL. A key on a page number
+ * outside the cache gets NaN. 0 <= decay <= 1.
+ * workspace: dq_attention_mass_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
+DQ_API int64_t dq_attention_mass_workspace(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q);
+DQ_API int dq_attention_mass(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, const float* lse,
+                             float scale, float decay, float* mass, int64_t seq_stride, int64_t head_stride,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The places of the keys that stay, in each kv head by itself: of sequence b's lens[b] keys the first `first`, the last
+ * `last`, and of the others those of largest mass (of equal ones the lower; a NaN is below all numbers) until there are `budget`.
+ * kept[b][g][i] (batch x kv_heads x budget) is the i-th such place, ascending; -1 where there are no more.
+ * kept_lens[b] = min(lens[b], budget) (NULL: not written). first + last <= budget. Of `s` batch, lens and max_len
+ * are read. */
+DQ_API int dq_kv_keep(const dq_sequences* s, int64_t kv_heads, const float* mass, int64_t seq_stride, int64_t head_stride,
+                      int64_t first, int64_t last, int64_t budget, int32_t* kept, int32_t* kept_lens, void* stream);
+
+/* Moves the keys and values of places kept[b][g][i] of sequence b to places i, in each kv head by itself, of the pages
+ * to_pages[b * to_stride], ... (NULL: of the sequence's own, in place; then kept must ascend, as dq_kv_keep's does). Entries
+ * outside [0, lens[b]) and pages outside the cache are left out. With mass and mass_out (both or neither), mass_out[b][g][i] is
+ * mass[b][g][kept[b][g][i]] too, at the same strides; mass_out may be mass. Pages that are written to must be of one sequence and
+ * (to_pages) be read by none. Keys have been rotated to their positions when they were appended: those that stay keep them. */
+DQ_API int dq_kv_compact(const dq_kv_cache* cache, const dq_sequences* s, const int32_t* kept, int64_t budget,
+                         const int32_t* to_pages, int64_t to_stride, const float* mass, float* mass_out, int64_t seq_stride,
+                         int64_t head_stride, void* stream);
+
 /* ---- GGUF files ----------------------------------------------------------
  * A GGUF v2 / v3 model mapped read-only (mmap): header, metadata and tensor
  * directory parsed with every length and offset checked against the file
