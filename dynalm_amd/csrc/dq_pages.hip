@@ -1,6 +1,6 @@
 // dq_pages.hip -- the pages that a query reads: each page's bounds of its keys' channels, the choice of pages
 // by an upper bound of a row's scores on them, and attention over the chosen pages alone.
-#include <type_traits>
+#include <algorithm>
 
 #include "dq_attn_device.h"
 #include "dq_pages.h"
@@ -95,9 +95,13 @@ __global__ __launch_bounds__(256) void k_page_bounds(AttnArgs a, const int32_t* 
 }
 
 // ---- the choice of pages ----------------------------------------------------
-// Scores decide which pages are read, so two that differ must not tie for a rounding: sums are 64 bits wide
-// (products of 16 or 24-bit values are exact in them). They go to the workspace as whole numbers that
-// order as they do.
+// A row's score of a page is S = sum_d q+_d hi_d + q-_d lo_d, with q's positive values in q+ and the others in q-: a
+// matrix product over 2 dim values, on the 16-bit matrix cores (an fp32 q in two parts). Two scores that differ must not tie for
+// a rounding, so the choice is one of 64-bit sums; but of these it needs few. Beside S the same instructions give
+// A = sum |q_d| max(|lo_d|, |hi_d|), with it a bound on S's error, and from both an interval that holds the 64-bit sum. A row's
+// pages are certain where their intervals say so; only those that meet at the border of the choice (two or three of 512), and those whose sums
+// are not finite, are summed again in 64 bits. 64-bit sums of all of them: 479 us for 512 tokens of 32 heads
+// on 512 pages of 4 kv heads of 128.
 
 constexpr uint64_t kAlways = ~0ull, kNanKey = ~0ull - 1;
 
@@ -105,6 +109,139 @@ DQ_DEV uint64_t order_key(double x) {
   if (x != x) return kNanKey;
   const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);  // (-0 is 0)
   return b >> 63 ? ~b : b | 1ull << 63;
+}
+DQ_DEV u32 order_key(float x) {
+  const u32 b = as_u(x + 0.f);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+template <int kCtrl>
+DQ_DEV float dpp_f(float x) {
+  return as_f((u32)dpp<kCtrl>((int)as_u(x)));
+}
+// The largest over each aligned group of `lanes` (1, 2, 4, 8, 16).
+DQ_DEV float lanes_max(float x, int lanes) {
+  if (lanes > 1) x = fmaxf(x, dpp_f<kQuadXor1>(x));
+  if (lanes > 2) x = fmaxf(x, dpp_f<kQuadXor2>(x));
+  if (lanes > 4) x = fmaxf(x, dpp_f<kHalfMirror>(x));
+  if (lanes > 8) x = fmaxf(x, dpp_f<kRowRor8>(x));
+  return x;
+}
+
+template <int T>
+constexpr int kScoreParts = T == DQ_F32 ? 2 : 1;
+
+// What S may be off by, of A: a rounding (or a cut) of each of the 2 dim sums and of those of the parts, an fp32 q's third part,
+// A's own error, the interval's ends.
+template <int T, int TC>
+DQ_DEV float score_error(int dim) {
+  return (2 * kScoreParts<T> * dim + 64) * 0x1p-23f + (T != DQ_F32 ? 0.f : TC == DQ_F16 ? 0x1p-20f : 0x1p-16f);
+}
+
+// A wave takes 16 pages of a kv head, whose bounds it holds, and of a sequence's rows a range, 16 at a time: `slots` tokens
+// of `lanes` lanes, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
+template <int T, int TC, int DP>
+__global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int lanes, int ranges, int range_tokens,
+                                                     int64_t items) {
+  constexpr int NS = DP / 32, NP = kScoreParts<T>;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (item >= items) return;
+  const int hk = a.cache.kv_heads, page_tiles = (c.pages + 15) / 16;
+  const int h = (int)(item % hk), p0 = (int)(item / hk % page_tiles) * 16;
+  const int range = (int)(item / hk / page_tiles % ranges), b = (int)(item / hk / page_tiles / ranges);
+  // the range's tokens, of the launch's
+  const int64_t lo = a.q_offsets != nullptr ? a.q_offsets[b] : b, hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
+  const int64_t end = min(min(hi, (int64_t)a.tokens), (int64_t)token0 + c.tokens);
+  const int64_t first = max(lo, (int64_t)token0) + (int64_t)range * range_tokens, last = min(first + range_tokens, end);
+  const int pages = (seq_len(a, b) + a.cache.page_size - 1) / a.cache.page_size;
+  if (p0 >= pages || first >= last) return;
+
+  // the bounds as A operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values
+  const int id = p0 + n < pages ? a.pages[b * a.pages_stride + p0 + n] : 0;
+  const bool bad = (u32)id >= (u32)a.cache.n_pages;
+  const uint16_t* near = c.bounds + ((int64_t)(bad ? 0 : id) * hk + h) * 2 * a.dim;
+  v4u x[2][NS], most[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int d = 32 * s + 8 * g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i][s] = d < a.dim ? *reinterpret_cast<const v4u*>(near + i * a.dim + d) : v4u{0, 0, 0, 0};
+  }
+  // of the four pages whose products the lane holds
+  const uint64_t bads = __ballot(bad);
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const v2us u = __builtin_bit_cast(v2us, x[0][s][e] & 0x7FFF7FFFu), v = __builtin_bit_cast(v2us, x[1][s][e] & 0x7FFF7FFFu);
+      most[s][e] = __builtin_bit_cast(u32, __builtin_elementwise_max(u, v));
+    }
+  const float error = score_error<T, TC>(a.dim);
+  const int slots = 16 / lanes, slot = n / lanes, blocks = (a.group + 15) / 16;
+  for (int64_t t0 = first; t0 < last; t0 += slots) {
+    const int t = (int)min(t0 + slot, last - 1);
+    float low[4], high[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
+    for (int block = 0; block < blocks; ++block) {  // (a lane past the heads takes the last again)
+      RawQ<T, DP> raw;
+      load_q<T, DP>(a, true, t, h * a.group + min(16 * block + n % lanes, a.group - 1), g, raw);
+      int e2 = 0;
+      if constexpr (T == DQ_F32 && TC == DQ_F16) {  // scaled to a largest value in [2^14, 2^15)
+        float top = 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(as_f(raw.x[s][i / 4][i % 4])));
+        top = row_max(top);
+        e2 = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+      }
+      v4f sum = {0, 0, 0, 0}, size = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        v4u part[NP], down, mag;  // down: the halves of values that are not above 0
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (T == DQ_F32) {
+            const float y0 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2]), e2), y1 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2 + 1]), e2);
+            u32 p = pack<TC>(y0, y1);
+            part[0][e] = p;
+            part[1][e] = pack<TC>(y0 - widen<TC>(p), y1 - widen_hi<TC>(p));
+            down[e] = (y0 > 0 ? 0u : 0xFFFFu) | (y1 > 0 ? 0u : 0xFFFF0000u);
+            // (what the parts leave out is less than 2^-20 (2^-16) of the value, or of the least magnitude that counts here)
+            constexpr float kLeast = TC == DQ_F16 ? 0x1p-4f : 0x1p-100f;
+            mag[e] = pack<TC>(y0 != y0 ? y0 : fmaxf(fabsf(y0), kLeast), y1 != y1 ? y1 : fmaxf(fabsf(y1), kLeast));
+          } else {
+            const u32 y = raw.x[s][0][e];
+            part[0][e] = y;
+            down[e] = __builtin_bit_cast(u32, __builtin_bit_cast(v2s, y) >> 15);
+            mag[e] = y & 0x7FFF7FFFu;
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          sum = mma<TC>(x[1][s], part[p] & ~down, sum);
+          sum = mma<TC>(x[0][s], part[p] & down, sum);
+        }
+        size = mma<TC>(most[s], mag, size);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float d = fmaf(error, size[i], 0x1p-118f);
+        const bool fine = d < INFINITY && fabsf(sum[i]) < INFINITY && !(bads >> (4 * g + i) & 1);
+        low[i] = fmaxf(low[i], fine ? ldexpf(sum[i] - d, -e2) : -INFINITY);
+        high[i] = fmaxf(high[i], fine ? ldexpf(sum[i] + d, -e2) : INFINITY);
+      }
+    }
+    uint64_t* out = c.keys + ((t - token0) * (int64_t)hk + h) * c.pages + p0 + 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      low[i] = lanes_max(low[i], lanes);
+      high[i] = lanes_max(high[i], lanes);
+      if (n % lanes == 0 && t0 + slot < last && p0 + 4 * g + i < pages) *reinterpret_cast<v2f*>(out + i) = v2f{low[i], high[i]};
+    }
+  }
 }
 
 template <int kCtrl>
@@ -123,134 +260,225 @@ DQ_DEV double lanes_sum(double x, int log2) {
   return x;
 }
 
-// A wave scores kRun pages of a row's kv head: 64 / lanes of them at a time, a lane 8 channels of one.
-constexpr int kRun = 64;
-
+// The 64-bit score of row t on a page, as a whole number that orders as it does: a wave's work, 2^log2 lanes a query head.
 template <int T, int TC>
-__global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int64_t token0, int lanes_log2, int64_t items) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  if (item >= items) return;
-  const int runs = (c.pages + kRun - 1) / kRun, hk = a.cache.kv_heads;
-  const int run = (int)(item % runs), h = (int)(item / runs % hk);
-  const int64_t row = item / runs / hk;
-  const int t = (int)(token0 + row);
-  const int b = find_seq(a, t, lane);
-  if (b < 0) return;
-  const int pages = (row_sees(a, b, t, seq_len(a, b)) + a.cache.page_size - 1) / a.cache.page_size;
-  if (run * kRun >= pages) return;
-  const int32_t* list = a.pages + b * a.pages_stride;
-  const int lanes = 1 << lanes_log2, step = 64 >> lanes_log2, d = 8 * (lane & (lanes - 1));
+DQ_DEV uint64_t exact_key(const AttnArgs& a, const ChooseArgs& c, int t, int h, int id, int log2, int lane) {
+  if ((u32)id >= (u32)a.cache.n_pages) return kNanKey;
+  const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), heads = 64 >> log2;
   const bool in = d < a.dim;
-  uint64_t* out = c.keys + (row * hk + h) * c.pages;
-  const int end = min(pages, (run + 1) * kRun);
-  for (int p0 = run * kRun; p0 < end; p0 += 2 * step) {
-    v4u lo[2], hi[2];
-    int id[2];
+  const uint16_t* near = c.bounds + ((int64_t)id * a.cache.kv_heads + h) * 2 * a.dim + (in ? d : 0);
+  const v4u lo = *reinterpret_cast<const v4u*>(near), hi = *reinterpret_cast<const v4u*>(near + a.dim);
+  uint64_t best = 0;
+  for (int i0 = 0; i0 < a.group; i0 += heads) {  // (a lane past the heads takes the last again)
+    const int head = h * a.group + min(i0 + (lane >> log2), a.group - 1);
+    const int64_t at = (int64_t)t * a.q_token + (int64_t)head * a.q_head + d;
+    double s = 0;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int p = min(p0 + u * step + (lane >> lanes_log2), end - 1);
-      id[u] = list[p];
-      const bool ok = (u32)id[u] < (u32)a.cache.n_pages;
-      const uint16_t* x = c.bounds + ((int64_t)(ok ? id[u] : 0) * hk + h) * 2 * a.dim + (in ? d : 0);
-      lo[u] = *reinterpret_cast<const v4u*>(x);
-      hi[u] = *reinterpret_cast<const v4u*>(x + a.dim);
-      id[u] = ok;
+    for (int e = 0; e < 8; ++e) {
+      const float q = in ? load1<T>(a.q, at + e) : 0.f;
+      const u32 x = q > 0 ? hi[e / 2] : lo[e / 2];
+      s = fma((double)q, (double)(e % 2 ? widen_hi<TC>(x) : widen<TC>(x)), s);
     }
-    uint64_t best[2] = {0, 0};
-    for (int i = 0; i < a.group; ++i) {
-      const int64_t at = (int64_t)t * a.q_token + (int64_t)(h * a.group + i) * a.q_head + d;
-      float q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = in ? load1<T>(a.q, at + e) : 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        double s = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const u32 x = q[e] > 0 ? hi[u][e / 2] : lo[u][e / 2];
-          s = fma((double)q[e], (double)(e % 2 ? widen_hi<TC>(x) : widen<TC>(x)), s);
-        }
-        s = lanes_sum(in ? s : 0.0, lanes_log2);
-        const uint64_t key = order_key(s);
-        best[u] = key > best[u] ? key : best[u];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int p = p0 + u * step + (lane >> lanes_log2);
-      if (p < end && (lane & (lanes - 1)) == 0) out[p] = id[u] ? best[u] : kNanKey;
-    }
+    const uint64_t key = order_key(lanes_sum(in ? s : 0.0, log2));
+    best = key > best ? key : best;
   }
+  for (int m = lanes; m < 64; m <<= 1) {
+    const uint64_t o = __shfl_xor(best, m, 64);
+    best = o > best ? o : best;
+  }
+  return best;
 }
 
-// The choice: a wave takes a row's kv head, and finds the count-th largest key bit by bit.
-// kHeld: all of a row's keys lie in registers, N to a lane; else they are read again for every bit.
-template <int N, bool kHeld>
-__global__ __launch_bounds__(256) void k_page_choice(AttnArgs a, ChooseArgs c, int64_t token0, int64_t rows) {
+// Keys of all of a row's pages in 64 bits, where too many meet at the border: they take the intervals' place.
+DQ_DEV uint64_t load_key(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+DQ_DEV void store_key(uint64_t* p, uint64_t x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The choice: W waves take a row's kv head (W 1: four rows a workgroup). The count-th largest of the intervals' ends is found bit
+// by bit, on whole numbers that order as they do. kHeld: a row's intervals lie in registers, N to a lane, else they are read again for every
+// bit. Wave w takes a run of the pages, so that the list comes out ascending.
+template <int T, int TC, int N, int W, bool kHeld>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs a, ChooseArgs c, int token0, int64_t rows, int log2) {
+  constexpr int R = W == 1 ? 4 : 1;  // rows of a workgroup
+  __shared__ int s_counts[2][W], s_list[R][64];
+  __shared__ uint64_t s_key[R][64];
   const int lane = threadIdx.x & 63, hk = a.cache.kv_heads;
-  const int64_t row = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  const int in_group = uniform(threadIdx.x >> 6), w = W == 1 ? 0 : in_group, r = W == 1 ? in_group : 0;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
   if (row >= rows) return;
-  const int t = (int)(token0 + row / hk);
+  const int t = token0 + (int)(row / hk), h = (int)(row % hk);
   const int b = find_seq(a, t, lane);
   if (b < 0) return;
   const int pages = (row_sees(a, b, t, seq_len(a, b)) + a.cache.page_size - 1) / a.cache.page_size;
-  int32_t* out = c.chosen + ((int64_t)t * hk + row % hk) * c.count;
-  const int count = (int)min(c.count, (int64_t)pages);
-  for (int64_t i = count + lane; i < c.count; i += 64) out[i] = -1;
+  int32_t* out = c.chosen + ((int64_t)t * hk + h) * c.count;
+  const int count = (int)min(c.count, (int64_t)pages), tid = w * 64 + lane;
+  for (int64_t i = count + tid; i < c.count; i += 64 * W) out[i] = -1;
   if (pages <= c.count) {
-    for (int i = lane; i < pages; i += 64) out[i] = i;
+    for (int i = tid; i < pages; i += 64 * W) out[i] = i;
     return;
   }
-  const uint64_t* keys = c.keys + row * c.pages;
-  auto key_at = [&](int p) {
-    if (p >= pages) return (uint64_t)0;  // (below every score)
-    return p < c.first || p >= pages - c.last ? kAlways : keys[p];
+  const int32_t* list = a.pages + b * a.pages_stride;
+  uint64_t* keys = c.keys + row * c.pages;
+  const int rounds = kHeld ? N : (pages + 64 * W - 1) / (64 * W), base = w * rounds * 64;
+  auto interval = [&](int i, u32& low, u32& high) {
+    const int p = base + i * 64 + lane;
+    low = high = p < pages ? ~0u : 0u;  // (0: no page)
+    if (p < c.first || p >= pages - c.last) return;
+    const v2f x = *reinterpret_cast<const v2f*>(keys + p);
+    low = order_key(x[0]);
+    high = order_key(x[1]);
   };
-  uint64_t k[N];
+  u32 low[N], high[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) k[i] = kHeld ? key_at(i * 64 + lane) : 0;
-  const int rounds = kHeld ? N : (pages + 63) / 64;
-  uint64_t least = 0;
-  int taken = 0;  // keys >= least, once they are `count`
-#pragma unroll 1
-  for (int bit = 63; bit >= 0 && taken != count; --bit) {
-    const uint64_t mid = least | 1ull << bit;
-    int n = 0;
+  for (int i = 0; i < N; ++i)
+    if (kHeld) interval(i, low[i], high[i]);
+  // the sum over the row's waves
+  int turn = 0;
+  auto all_waves = [&](int n) {
+    if constexpr (W == 1) return n;
+    turn ^= 1;
+    if (lane == 0) s_counts[turn][w] = n;
+    __syncthreads();  // (a turn's counts are read before the next one's barrier, written after it)
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) sum += s_counts[turn][i];
+    return sum;
+  };
+  // f(round, low, high) for the wave's pages
+  auto each = [&](auto&& f) {
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) n += __popcll(__ballot(k[i] >= mid));
+      for (int i = 0; i < N; ++i) f(i, low[i], high[i]);
     } else {
-      for (int i = 0; i < rounds; ++i) n += __popcll(__ballot(key_at(i * 64 + lane) >= mid));
+      for (int i = 0; i < rounds; ++i) {
+        u32 l, u;
+        interval(i, l, u);
+        f(i, l, u);
+      }
     }
-    if (n >= count) {
-      least = mid;
-      taken = n;
-    }
-  }
-  // those above `least`, and of those at it the first ones
-  int above = 0;
-  if constexpr (kHeld) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) above += __popcll(__ballot(k[i] > least));
-  } else {
-    for (int i = 0; i < rounds; ++i) above += __popcll(__ballot(key_at(i * 64 + lane) > least));
-  }
-  int equal = count - above, at = 0;
-  auto put = [&](int i, uint64_t key) {
-    const uint64_t before = (1ull << lane) - 1, ties = __ballot(key == least);
-    const bool mine = key > least || (key == least && __popcll(ties & before) < equal);
-    const uint64_t all = __ballot(mine);
-    if (mine) out[at + __popcll(all & before)] = i * 64 + lane;
-    at += __popcll(all);
-    equal -= min(equal, __popcll(ties));
   };
-  if constexpr (kHeld) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) put(i, k[i]);
-  } else {
-    for (int i = 0; i < rounds; ++i) put(i, key_at(i * 64 + lane));
+  // the n-th largest; early: or a lower one with the same n above it or at it
+  auto nth = [&](int n, bool highs, bool early) {
+    u32 least = 0;
+    int taken = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0 && !(early && taken == n); --bit) {
+      const u32 mid = least | 1u << bit;
+      int k = 0;
+      each([&](int, u32 l, u32 u) { k += __popcll(__ballot((highs ? u : l) >= mid)); });
+      k = all_waves(k);
+      if (k >= n) {
+        least = mid;
+        taken = k;
+      }
+    }
+    return least;
+  };
+  // A page whose high end is below the count-th largest low end is out; one whose low end is above the next high
+  // end after the count-th is in; the others are looked at again.
+  const u32 floor = nth(count, false, true);
+  int able = 0;
+  each([&](int, u32, u32 u) { able += __popcll(__ballot(u >= floor)); });
+  able = all_waves(able);
+  const u32 ceiling = able > count ? nth(count + 1, true, false) : 0u;
+  const bool all_in = able == count;
+  int open = 0;
+  if (!all_in) each([&](int, u32 l, u32 u) { open += __popcll(__ballot(u >= floor && l <= ceiling)); });
+  open = all_waves(open);
+  int before = 0;  // open ones of the waves before
+  if constexpr (W > 1)
+    for (int i = 0; i < w; ++i) before += s_counts[turn][i];
+  const int room = count - (able - open);  // for open ones
+  uint64_t taken = 0;  // of the open ones, in their order
+  if (open > 0 && open <= 64) {
+    int at = before;
+    each([&](int i, u32 l, u32 u) {
+      const bool mine = u >= floor && l <= ceiling;
+      const uint64_t m = __ballot(mine);
+      if (mine) s_list[r][at + __popcll(m & ((1ull << lane) - 1))] = list[base + i * 64 + lane];
+      at += __popcll(m);
+    });
+    if constexpr (W > 1) __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    for (int j = w; j < open; j += W) {
+      const uint64_t key = exact_key<T, TC>(a, c, t, h, s_list[r][j], log2, lane);
+      if (lane == 0) s_key[r][j] = key;
+    }
+    if constexpr (W > 1) __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    const uint64_t key = lane < open ? s_key[r][lane] : 0;
+    int rank = 0;
+    for (int j = 0; j < open; ++j) {
+      const uint64_t o = s_key[r][j];
+      rank += o > key || (o == key && j < lane);
+    }
+    taken = __ballot(lane < open && rank < room);
+  } else if (open > 64) {
+    for (int p = w; p < pages; p += W) {
+      const uint64_t key = p < c.first || p >= pages - c.last ? kAlways : exact_key<T, TC>(a, c, t, h, list[p], log2, lane);
+      if (lane == 0) store_key(keys + p, key);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "agent");
+    if constexpr (W > 1) __syncthreads();
+    auto key_at = [&](int i) {
+      const int p = base + i * 64 + lane;
+      return p < pages ? load_key(keys + p) : 0;
+    };
+    uint64_t least = 0;
+    int k = 0;
+#pragma unroll 1
+    for (int bit = 63; bit >= 0 && k != count; --bit) {
+      const uint64_t mid = least | 1ull << bit;
+      int m = 0;
+      for (int i = 0; i < rounds; ++i) m += __popcll(__ballot(key_at(i) >= mid));
+      m = all_waves(m);
+      if (m >= count) {
+        least = mid;
+        k = m;
+      }
+    }
+    int above = 0, ties = 0;
+    for (int i = 0; i < rounds; ++i) {
+      above += __popcll(__ballot(key_at(i) > least));
+      ties += __popcll(__ballot(key_at(i) == least));
+    }
+    const int all_above = all_waves(above);
+    int at = 0, left = count - all_above, ties_before = 0;
+    if constexpr (W > 1) {
+      for (int i = 0; i < w; ++i) at += s_counts[turn][i];
+      all_waves(ties);
+      for (int i = 0; i < w; ++i) ties_before += s_counts[turn][i];
+    }
+    at += min(ties_before, left);
+    left = max(left - ties_before, 0);
+    for (int i = 0; i < rounds; ++i) {
+      const uint64_t key = key_at(i), tie = __ballot(key == least), lower = (1ull << lane) - 1;
+      const bool mine = key > least || (key == least && __popcll(tie & lower) < left);
+      const uint64_t m = __ballot(mine);
+      if (mine) out[at + __popcll(m & lower)] = base + i * 64 + lane;
+      at += __popcll(m);
+      left -= min(left, __popcll(tie));
+    }
+    return;
   }
+  // certain ones and taken ones, in their order
+  int sure = 0;
+  each([&](int, u32 l, u32 u) { sure += __popcll(__ballot(u >= floor && (all_in || l > ceiling))); });
+  int at = before < 64 ? __popcll(taken & ((1ull << before) - 1)) : __popcll(taken), seen = before;
+  if constexpr (W > 1) {
+    all_waves(sure);
+    for (int i = 0; i < w; ++i) at += s_counts[turn][i];
+  }
+  each([&](int i, u32 l, u32 u) {
+    const uint64_t lower = (1ull << lane) - 1;
+    const bool isopen = !all_in && u >= floor && l <= ceiling;
+    const uint64_t mo = __ballot(isopen);
+    const int index = seen + __popcll(mo & lower);
+    const bool mine = isopen ? taken >> index & 1 : u >= floor;
+    const uint64_t m = __ballot(mine);
+    if (mine) out[at + __popcll(m & lower)] = base + i * 64 + lane;
+    at += __popcll(m);
+    seen += __popcll(mo);
+  });
 }
 
 // ---- attention over chosen pages ---------------------------------------------
@@ -483,6 +711,9 @@ __global__ __launch_bounds__(256) void k_page_attn(AttnArgs a, const int32_t* ch
   }
 }
 
+// Waves that a launch of scores aims at.
+constexpr int64_t kScoreWaves = 4096;
+
 // lanes that hold a head's values, 8 each: their number's logarithm
 int lanes_log2(int dim) {
   int log2 = 0;
@@ -507,25 +738,35 @@ hipError_t launch_page_bounds(int cache_type, const AttnArgs& a, const int32_t* 
 }
 
 hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, const ChooseArgs& c, hipStream_t s) {
-  const int64_t runs = (c.pages + kRun - 1) / kRun;
+  int lanes = 1;
+  while (lanes < a.group && lanes < 16) lanes *= 2;
+  const int slots = 16 / lanes;
   for (int64_t t = 0; t < a.tokens; t += c.tokens) {
-    const int64_t rows = (a.tokens - t < c.tokens ? a.tokens - t : c.tokens) * a.cache.kv_heads, items = rows * runs;
-    if (c.pages > c.count) {  // (else every page is read)
-      const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
-        hipLaunchKernelGGL((k_page_scores<tq(), tc()>), dim3((uint32_t)((items + 3) / 4)), dim3(256), 0, s, a, c, t,
-                           lanes_log2(a.dim), items);
-        return hipGetLastError();
-      });
-      if (e != hipSuccess) return e;
-    }
-    const dim3 grid((uint32_t)((rows + 3) / 4));
-    if (c.pages <= 8 * 64)
-      hipLaunchKernelGGL((k_page_choice<8, true>), grid, dim3(256), 0, s, a, c, t, rows);
-    else if (c.pages <= 32 * 64)
-      hipLaunchKernelGGL((k_page_choice<32, true>), grid, dim3(256), 0, s, a, c, t, rows);
-    else
-      hipLaunchKernelGGL((k_page_choice<1, false>), grid, dim3(256), 0, s, a, c, t, rows);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const int64_t rows = (a.tokens - t < c.tokens ? a.tokens - t : c.tokens) * a.cache.kv_heads;
+    const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
+      if (c.pages > c.count) {  // (else every page is read)
+        const int64_t tiles = (a.max_q + slots - 1) / slots, waves = (int64_t)a.batch * a.cache.kv_heads * ((c.pages + 15) / 16);
+        const int64_t ranges = std::max<int64_t>(1, std::min(tiles, kScoreWaves / waves)), per = (tiles + ranges - 1) / ranges * slots;
+        const int64_t items = waves * ranges;
+        const dim3 grid((uint32_t)((items + 3) / 4));
+        if (a.dim <= 64)
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 64>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+        else if (a.dim <= 128)
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 128>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+        else
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+      }
+      const int log2 = lanes_log2(a.dim);
+      if (c.pages <= 8 * 64)
+        hipLaunchKernelGGL((k_page_choice<tq(), tc(), 8, 1, true>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, c, (int)t, rows, log2);
+      else if (c.pages <= 8 * 16 * 64)
+        hipLaunchKernelGGL((k_page_choice<tq(), tc(), 8, 16, true>), dim3((uint32_t)rows), dim3(1024), 0, s, a, c, (int)t, rows, log2);
+      else
+        hipLaunchKernelGGL((k_page_choice<tq(), tc(), 1, 16, false>), dim3((uint32_t)rows), dim3(1024), 0, s, a, c, (int)t, rows, log2);
+      return hipGetLastError();
+    });
+    if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }

@@ -129,11 +129,11 @@ AttnArgs query_args(const dq_kv_cache* c, const dq_sequences* s, const dq_heads*
 
 // ---- plans: functions of the shape ----
 
-// Tokens whose scores a launch of dq_choose_pages writes.
+// Tokens whose scores a launch of dq_choose_pages writes (0: one's are too many).
 int64_t choose_tokens(const dq_kv_cache* c, const dq_sequences* s, bool scores) {
-  const int64_t pages = ceil_div(s->max_len, c->page_size), runs = ceil_div(pages, 64);
-  int64_t n = kMaxGroups / c->kv_heads;
-  if (scores) n = std::min(kWorkspace / (8 * pages * c->kv_heads), kMaxGroups / (runs * c->kv_heads));
+  const int64_t pages = ceil_div(s->max_len, c->page_size);
+  int64_t n = kMaxGroups / 4 / c->kv_heads;  // (a workgroup of 1,024 threads a row at most)
+  if (scores) n = std::min(n, kWorkspace / 8 / pages / c->kv_heads);
   return std::min(n, s->tokens);
 }
 
@@ -141,7 +141,9 @@ int check_choose(const dq_kv_cache* c, const dq_sequences* s) {
   if (int rc = check_cache(c, false); rc != DQ_OK) return rc;
   if (int rc = check_sequences(s, c->page_size); rc != DQ_OK) return rc;
   if (s->tokens < 0) return bad("tokens must be >= 0");
-  if (s->tokens > 0 && s->max_len > 0 && choose_tokens(c, s, true) == 0) return too_many("pages and heads");
+  if (s->tokens > 0 && s->max_len > 0 &&
+      (choose_tokens(c, s, true) == 0 || s->batch > 4 * kMaxGroups / (ceil_div(ceil_div(s->max_len, c->page_size), 16) * c->kv_heads)))
+    return too_many("pages and heads");
   return DQ_OK;
 }
 
@@ -243,7 +245,6 @@ int dq_choose_pages(const dq_kv_cache* cache, const dq_sequences* s, const dq_he
     return set_error(DQ_INVALID_ARGUMENT, "first %lld and last %lld of %lld pages: last is 1 or more, their sum at most count", (ll)first,
                      (ll)last, (ll)count);
   if (s->tokens == 0 || s->batch == 0) return DQ_OK;
-  if (cache->kv_heads > kMaxGroups) return too_many("heads");
   if (int rc = check_sequence_data(s, cache); rc != DQ_OK) return rc;
   if (int rc = check_data("q", q); rc != DQ_OK) return rc;
   if (chosen == nullptr) return bad("chosen: null argument");

@@ -96,6 +96,46 @@ def test_choice_of_equal_scores(cuda):
             assert torch.equal(L.run_choose(c, bounds, 1, 1, count).cpu(), L.choose(c, bounds, 1, 1, count))
 
 
+@pytest.mark.parametrize("pages,count", [(200, 70), (700, 65), (9000, 1000)])
+@pytest.mark.parametrize("type,cache", KINDS)
+def test_choice_where_many_pages_meet_at_the_border(cuda, pages, count, type, cache):
+    """Hundreds of pages with one score, or with two, and some apart: all are told apart exactly, ties go to the lower ones."""
+    c = Call(61, [1, 1], [pages * 16, pages * 16 - 300], 2, 1, 16, type, cache, 16)
+    gen = torch.Generator().manual_seed(pages)
+    bounds = torch.zeros((c.kc.shape[0], 1, 2, 16), dtype=c.kc.dtype, device="cuda")
+    # (NaN keys elsewhere would make intervals without ends: the bounds alone count here)
+    for kind in range(4):
+        if kind == 0:
+            c.q.zero_()
+        else:
+            c.q.copy_(torch.randn(c.q.shape, generator=gen))
+            bounds.copy_(torch.randn((1, 1, 1, 16), generator=gen).expand(bounds.shape))
+        if kind == 2:
+            bounds[torch.rand(bounds.shape[0], generator=gen).cuda() < 0.5] *= 1.0078125
+        if kind == 3:
+            some = torch.rand(bounds.shape[0], generator=gen).cuda() < 0.02
+            bounds[some] = torch.randn((int(some.sum()), 1, 2, 16), generator=gen).to(bounds.dtype).cuda() * 3
+            bounds[int(c.table[0, 5]), 0, 1, 3] = math.inf
+            bounds[int(c.table[0, 9]), 0, 0, 2] = math.nan
+        assert torch.equal(L.run_choose(c, bounds, 2, 3, count).cpu(), L.choose(c, bounds, 2, 3, count)), kind
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e30])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_choice_of_queries_of_any_size(cuda, type, cache, size, mixed):
+    """Large and small queries, and heads whose values lie many orders of magnitude apart."""
+    if type == "f16":
+        size = min(max(size, 1e-6), 1e3)
+    c = Call(62, [1, 2], [300 * 16, 250 * 16], 6, 2, 64, type, cache, 16)
+    bounds = L.run_bounds(c)
+    scale = torch.full((64,), size)
+    if mixed:
+        scale = scale * 2.0 ** -torch.randint(0, 12 if type == "f16" else 40, (64,), generator=torch.Generator().manual_seed(1))
+    c.q.copy_((c.q.float().cpu() * scale).to(c.q.dtype))
+    assert torch.equal(L.run_choose(c, bounds, 1, 1, 20).cpu(), L.choose(c, bounds, 1, 1, 20))
+
+
 def test_choice_tells_scores_apart_that_differ_by_little(cuda):
     """Scores that differ by 2^-40 of their size are no tie."""
     c = Call(5, [1], [64 * 16], 1, 1, 64, "f32", "bf16", 16)
