@@ -96,6 +96,18 @@ DQ_DEV float row_sum(float x) {
   return as_f(b[0]) + as_f(b[1]);
 }
 
+// The least over a wave.
+DQ_DEV u32 wave_least(u32 x) {
+  x = min(x, (u32)dpp<kQuadXor1>((int)x));
+  x = min(x, (u32)dpp<kQuadXor2>((int)x));
+  x = min(x, (u32)dpp<kHalfMirror>((int)x));
+  x = min(x, (u32)dpp<kRowRor8>((int)x));
+  auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = min((u32)a[0], (u32)a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return min((u32)b[0], (u32)b[1]);
+}
+
 // Every load of the wave has come.
 DQ_DEV void wait_loads() {
   asm volatile("" ::: "memory");

@@ -24,6 +24,57 @@ DQ_DEV void seq_rows(const AttnArgs& a, int b, int& first, int& n) {
 constexpr int kMassTiles = 4;                       // of 16 keys: a wave's
 constexpr int kMassKeys = 4 * 16 * kMassTiles;      // a workgroup's
 
+// z = lse log2 e as a float and the power of two of what that leaves out.
+DQ_DEV void split_lse(float lse, float& hi, float& f) {
+  const double z = (double)lse * 1.4426950408889634074;
+  hi = (float)z;
+  f = exp2_fast((float)((double)hi - z));
+  if (fabsf(hi) == INFINITY) {
+    hi = fabsf(lse) == INFINITY ? INFINITY : copysignf(FLT_MAX, lse);  // (a row whose lse is -inf has no weights)
+    f = 1.f;
+  }
+}
+
+// A wave's keys as B operands: lane n of a group has key n, 8 (lane / 16) .. + 7 of every 32 values.
+template <int DP>
+DQ_DEV void load_keys(const AttnArgs& a, int b, int head, int k0, int len, int n, int g, v4u (&k)[kMassTiles][DP / 32], bool (&bad)[kMassTiles]) {
+  const CacheArgs& ca = a.cache;
+  const int32_t* list = a.pages + b * a.pages_stride;
+  const u32 token_bytes = (u32)ca.token * 2;
+#pragma unroll
+  for (int i = 0; i < kMassTiles; ++i) {
+    const int key = k0 + 16 * i, p = min(key, len - 1) / ca.page_size;
+    int id = page_at(list, p);
+    bad[i] = (u32)id >= (u32)ca.n_pages;
+    if (bad[i]) id = 0;
+    const int in = key < len ? key - p * ca.page_size : 0;
+    const auto kr = rsrc(ca.k + id * ca.page + in * ca.token + head * ca.head, 0x7FFFFFFFu);
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s)
+      k[i][s] = ld16(kr, key < len && 32 * s + 8 * g < a.dim ? n * token_bytes + (32 * s + 8 * g) * 2 : 0x80000000u);
+  }
+}
+
+// The sums over a wave's rows into the weights, or into the range's part.
+DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int range, int k0, int len, int old, int n, int g, float (&sum)[kMassTiles],
+                     const bool (&bad)[kMassTiles]) {
+  const CacheArgs& ca = a.cache;
+#pragma unroll
+  for (int i = 0; i < kMassTiles; ++i) sum[i] = row_sum(sum[i]);
+  // lane group i writes tile i
+  static_assert(kMassTiles == 4);
+  float x = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
+  if (g == 0 ? bad[0] : g == 1 ? bad[1] : g == 2 ? bad[2] : bad[3]) x = __builtin_nanf("");
+  const int key = k0 + 16 * g + n;
+  if (key >= len) return;
+  if (m.part != nullptr) {
+    m.part[(((int64_t)range * a.batch + b) * ca.kv_heads + head) * a.max_len + key] = x;
+    return;
+  }
+  float* out = m.mass + b * m.seq + head * m.head + key;
+  *out = m.decay != 0 && key < old ? fmaf(m.decay, *out, x) : x;
+}
+
 template <int T, int TC, int DP>
 __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_tiles) {
   constexpr int NP = kParts<T, TC>;
@@ -42,23 +93,9 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
   seq_rows(a, b, first, count);
   const int old = len - count;  // keys before the rows' own
 
-  // the wave's keys as B operands: lane n of a group has key n, 8 (lane / 16) .. + 7 of every 32 values
   v4u k[kMassTiles][DP / 32];
   bool bad[kMassTiles];
-  const int32_t* list = a.pages + b * a.pages_stride;
-  const u32 token_bytes = (u32)ca.token * 2;
-#pragma unroll
-  for (int i = 0; i < kMassTiles; ++i) {
-    const int key = k0 + 16 * i, p = min(key, len - 1) / ca.page_size;
-    int id = page_at(list, p);
-    bad[i] = (u32)id >= (u32)ca.n_pages;
-    if (bad[i]) id = 0;
-    const int in = key < len ? key - p * ca.page_size : 0;
-    const auto kr = rsrc(ca.k + id * ca.page + in * ca.token + head * ca.head, 0x7FFFFFFFu);
-#pragma unroll
-    for (int s = 0; s < DP / 32; ++s)
-      k[i][s] = ld16(kr, key < len && 32 * s + 8 * g < a.dim ? n * token_bytes + (32 * s + 8 * g) * 2 : 0x80000000u);
-  }
+  load_keys<DP>(a, b, head, k0, len, n, g, k, bad);
 
   float sum[kMassTiles];
 #pragma unroll
@@ -76,13 +113,9 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
     const float lse = m.lse[(int64_t)token * a.heads + qh];
     v4u q[NP][DP / 32];
     const float c = q_operands<T, TC, DP>(a, raw, q);
-    const double z = (double)lse * 1.4426950408889634074;
-    float hi = (float)z, f = exp2_fast((float)((double)hi - z));
-    int limit = valid ? old + (token - first) + 1 : 0;
-    if (fabsf(hi) == INFINITY) {
-      hi = fabsf(lse) == INFINITY ? INFINITY : copysignf(FLT_MAX, lse);  // (a row whose lse is -inf has no weights)
-      f = 1.f;
-    }
+    float hi, f;
+    split_lse(lse, hi, f);
+    const int limit = valid ? old + (token - first) + 1 : 0;
     // of the four rows whose products the lane holds
     float c4[4], hi4[4], f4[4];
     int limit4[4];
@@ -108,20 +141,176 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
       }
     }
   }
+  put_mass(a, m, b, head, range, k0, len, old, n, g, sum, bad);
+}
+
+// Many rows: the same with the rows' queries through LDS, kMassRows at a time and two buffers deep, for the four waves
+// together; a row's 16-byte chunks lie at their number XOR some bits of the row's, which spreads a column of rows over the banks.
+
+template <int T>
+constexpr int kMassRows = T == DQ_F32 ? 32 : 64;
+
+template <int T, int TC, int DP>
+struct MassLds {
+  uint16_t q[2][kParts<T, TC>][kMassRows<T> * DP];
+  float hi[2][kMassRows<T>], f[2][kMassRows<T>], c[2][kMassRows<T>];
+  int limit[2][kMassRows<T>];
+};
+
+template <int T, int TC, int DP>
+__global__ __launch_bounds__(256) void k_mass_many(AttnArgs a, MassArgs m, int key_tiles) {
+  constexpr int NP = kParts<T, TC>, QR = kMassRows<T>;
+  constexpr int kChunks = DP / 8, kPasses = QR * kChunks / 256, kPassRows = 256 / kChunks;
+  __shared__ MassLds<T, TC, DP> sh;
+  const CacheArgs& ca = a.cache;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  u32 item = blockIdx.x;
+  const int head = item % ca.kv_heads;
+  item /= ca.kv_heads;
+  const int kt = item % key_tiles;
+  item /= key_tiles;
+  const int range = item % m.splits, b = item / m.splits;
+  const int len = seq_len(a, b);
+  if (kt * kMassKeys >= len) return;
+  const int k0 = kt * kMassKeys + wave * 16 * kMassTiles;
+  int first, count;
+  seq_rows(a, b, first, count);
+  const int old = len - count;
+  const int rows = count * a.group;
+  const int r_end = (int)min((int64_t)rows, m.splits > 1 ? (int64_t)(range + 1) * m.rows : (int64_t)rows);
+  // rows before the first that sees one of the workgroup's keys add nothing
+  const int r_begin = (int)max((int64_t)range * m.rows, max((int64_t)0, (int64_t)(kt * kMassKeys - old) * a.group) / QR * QR);
+
+  // a thread's 16 bytes (fp32: 32) of a row, kPasses rows of a tile
+  const int chunk = threadIdx.x % kChunks, pass_row = threadIdx.x / kChunks;
+  v4u raw[kPasses][T == DQ_F32 ? 2 : 1];
+  float lse = 0;
+  auto read = [&](int r0) {
 #pragma unroll
-  for (int i = 0; i < kMassTiles; ++i) sum[i] = row_sum(sum[i]);
-  // lane group i writes tile i
-  static_assert(kMassTiles == 4);
-  float x = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
-  if (g == 0 ? bad[0] : g == 1 ? bad[1] : g == 2 ? bad[2] : bad[3]) x = __builtin_nanf("");
-  const int key = k0 + 16 * g + n;
-  if (key >= len) return;
-  if (m.part != nullptr) {
-    m.part[(((int64_t)range * a.batch + b) * ca.kv_heads + head) * a.max_len + key] = x;
-    return;
+    for (int p = 0; p < kPasses; ++p) {
+      const int r = r0 + p * kPassRows + pass_row;
+      const bool in = r < r_end && 8 * chunk < a.dim;
+      const int64_t at = (int64_t)(first + r / a.group) * a.q_token + (int64_t)(head * a.group + r % a.group) * a.q_head + 8 * chunk;
+#pragma unroll
+      for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) {
+        v4u x = {0, 0, 0, 0};
+        if (in) {
+          if constexpr (T == DQ_F32) {
+            const float* src = static_cast<const float*>(a.q) + at + 4 * k;
+            if (a.q_vec)
+              x = *reinterpret_cast<const v4u*>(src);
+            else
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = as_u(src[i]);
+          } else {
+            const uint16_t* src = static_cast<const uint16_t*>(a.q) + at;
+            if (a.q_vec)
+              x = *reinterpret_cast<const v4u*>(src);
+            else
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = (u32)src[2 * i] | ((u32)src[2 * i + 1] << 16);
+          }
+        }
+        raw[p][k] = x;
+      }
+    }
+    const int r = r0 + (int)threadIdx.x;
+    if (threadIdx.x < QR && r < r_end) lse = m.lse[(int64_t)(first + r / a.group) * a.heads + head * a.group + r % a.group];
+  };
+  auto place = [&](int row, int ch) { return row * DP + 8 * (ch ^ (DP == 64 ? (row >> 1) & 7 : row & 15)); };
+  auto write = [&](int r0, int buf) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * kPassRows + pass_row;
+      if constexpr (T != DQ_F32) {
+        *reinterpret_cast<v4u*>(&sh.q[buf][0][place(row, chunk)]) = raw[p][0];
+      } else {
+        // scaled to a largest value in [2^14, 2^15), where all parts are normal numbers
+        float most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(as_f(raw[p][i / 4][i % 4])));
+#pragma unroll
+        for (int s = kChunks / 2; s >= 1; s >>= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
+        const int e = most > 0 && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+        v4u part[NP];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32 x[NP];
+          split<T, TC>(ldexpf(as_f(raw[p][i / 2][i % 2 * 2]), e), ldexpf(as_f(raw[p][i / 2][i % 2 * 2 + 1]), e), x);
+#pragma unroll
+          for (int k = 0; k < NP; ++k) part[k][i] = x[k];
+        }
+#pragma unroll
+        for (int k = 0; k < NP; ++k) *reinterpret_cast<v4u*>(&sh.q[buf][k][place(row, chunk)]) = part[k];
+        if (chunk == 0) sh.c[buf][row] = fmaxf(ldexpf(a.scale_log2, -e), 1.2e-38f);
+      }
+    }
+    if (threadIdx.x < QR) {
+      const int r = r0 + (int)threadIdx.x;
+      float hi, f;
+      split_lse(lse, hi, f);
+      sh.hi[buf][threadIdx.x] = hi;
+      sh.f[buf][threadIdx.x] = f;
+      sh.limit[buf][threadIdx.x] = r < r_end ? old + r / a.group + 1 : 0;
+    }
+  };
+
+  if (r_begin < r_end) read(r_begin);
+  v4u k[kMassTiles][DP / 32];
+  bool bad[kMassTiles];
+  load_keys<DP>(a, b, head, k0, len, n, g, k, bad);
+  float sum[kMassTiles];
+#pragma unroll
+  for (int i = 0; i < kMassTiles; ++i) sum[i] = 0;
+  if (r_begin < r_end) write(r_begin, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = r_begin; r0 < r_end; r0 += QR, buf ^= 1) {
+    const bool more = r0 + QR < r_end;
+    if (more) read(r0 + QR);
+    // (the rows' first sees the least)
+    const bool all_see = r0 + QR <= r_end && k0 + 16 * kMassTiles <= old + r0 / a.group + 1;
+    const bool none_sees = k0 >= old + (min(r0 + QR, r_end) - 1) / a.group + 1;
+    auto tile = [&](auto masked) {
+#pragma unroll 1
+      for (int q0 = 0; q0 < QR; q0 += 16) {
+        v4u q[NP][DP / 32];
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int s = 0; s < DP / 32; ++s) q[p][s] = *reinterpret_cast<const v4u*>(&sh.q[buf][p][place(q0 + n, 4 * s + g)]);
+        const v4f hi = *reinterpret_cast<const v4f*>(&sh.hi[buf][q0 + 4 * g]), f = *reinterpret_cast<const v4f*>(&sh.f[buf][q0 + 4 * g]);
+        v4f c = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+        if constexpr (T == DQ_F32) c = *reinterpret_cast<const v4f*>(&sh.c[buf][q0 + 4 * g]);
+        v4i limit = {0, 0, 0, 0};
+        if constexpr (masked()) limit = *reinterpret_cast<const v4i*>(&sh.limit[buf][q0 + 4 * g]);
+#pragma unroll
+        for (int i = 0; i < kMassTiles; ++i) {
+          v4f acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+            for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(q[p][s], k[i][s], acc);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float w = exp2_fast(fmaf(acc[e], c[e], -hi[e]));
+            if constexpr (masked())
+              sum[i] += k0 + 16 * i + n < limit[e] ? w * f[e] : 0.f;
+            else
+              sum[i] = fmaf(w, f[e], sum[i]);
+          }
+        }
+      }
+    };
+    if (all_see)
+      tile(std::false_type{});
+    else if (!none_sees)
+      tile(std::true_type{});
+    if (more) write(r0 + QR, buf ^ 1);
+    __syncthreads();
   }
-  float* out = m.mass + b * m.seq + head * m.head + key;
-  *out = m.decay != 0 && key < old ? fmaf(m.decay, *out, x) : x;
+  put_mass(a, m, b, head, range, k0, len, old, n, g, sum, bad);
 }
 
 // Adds the ranges of rows that were summed apart.
@@ -140,10 +329,14 @@ __global__ __launch_bounds__(256) void k_mass_join(AttnArgs a, MassArgs m, int64
 }
 
 // ---- the keys that stay ---------------------------------------------------------
-// A workgroup takes a sequence's kv head and finds the budget-th largest weight bit by bit, of whole numbers that
-// order as the weights do. Wave w holds (or, kHeld false, reads again for each bit) a run of the places, so that the list comes out ascending.
+// A workgroup takes a sequence's kv head. The budget-th largest weight is found on whole numbers that order as the weights do:
+// a histogram of kBins bins between their least and largest says in which bin it lies, another one of that bin's
+// numbers where in it, until a bin is one number, or taken as a whole: three passes at most. Wave w holds (or, kHeld false, reads again for each
+// pass) a run of the places, so that the list comes out ascending. Bit by bit, with a barrier each: 20 to 29 us in place of XXX
+// for 16,384 places.
 
 constexpr int kKeepWaves = 16;
+constexpr int kBinsLog2 = 11, kBins = 1 << kBinsLog2;
 
 // (NaN 1, below all numbers; -inf 0x7FFFFF, +inf 0xFF800000; 0 is no key's)
 DQ_DEV u32 weight_key(float x) {
@@ -152,9 +345,24 @@ DQ_DEV u32 weight_key(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
+// The sum over the lanes before this one, and over all.
+DQ_DEV int lanes_before(int x, int lane, int& all) {
+  int sum = x;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int y = __shfl_up(sum, m, 64);
+    if (lane >= m) sum += y;
+  }
+  all = __builtin_amdgcn_readlane(sum, 63);
+  return sum - x;
+}
+
 template <int N, bool kHeld>
 __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
-  __shared__ int counts[2][kKeepWaves], ties[kKeepWaves];
+  __shared__ int bins[kBins];
+  __shared__ int s_above[kKeepWaves], s_ties[kKeepWaves];
+  __shared__ u32 s_ends[2];  // least, largest (turned round); the bin that is looked for
+  __shared__ int s_found[3];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads;
   const int len = a.max_len > 0 ? min(max(a.lens[b], 0), a.max_len) : 0;
@@ -177,73 +385,110 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
   u32 k[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) k[i] = kHeld ? key_at(i) : 0;
-  auto count_if = [&](auto&& f) {
-    int n = 0;
+  auto each = [&](auto&& f) {
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) n += __popcll(__ballot(f(k[i])));
+      for (int i = 0; i < N; ++i) f(i, k[i]);
     } else {
-      for (int i = 0; i < rounds; ++i) n += __popcll(__ballot(f(key_at(i))));
+      for (int i = 0; i < rounds; ++i) f(i, key_at(i));
     }
-    return n;
   };
-  u32 least = 0;
-  int taken = 0, turn = 0;
-#pragma unroll 1
-  for (int bit = 31; bit >= 0 && taken != budget; --bit, turn ^= 1) {
-    const u32 mid = least | 1u << bit;
-    const int mine = count_if([&](u32 x) { return x >= mid; });
-    if (lane == 0) counts[turn][wave] = mine;
-    __syncthreads();  // (the other turn's counts are read before it, written after the next)
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < kKeepWaves; ++w) n += counts[turn][w];
-    if (n >= budget) {
-      least = mid;
-      taken = n;
-    }
-  }
-  const int above = count_if([&](u32 x) { return x > least; }), equal = count_if([&](u32 x) { return x == least; });
+  // where the numbers of places without a place of their own lie
+  if (threadIdx.x < 2) s_ends[threadIdx.x] = ~0u;
   __syncthreads();
+  u32 low = ~0u, high = 0;
+  each([&](int, u32 x) {
+    if (x != 0) low = min(low, x);
+    if (x != ~0u) high = max(high, x);
+  });
+  low = wave_least(low);
+  high = ~wave_least(~high);
   if (lane == 0) {
-    counts[0][wave] = above;
-    ties[wave] = equal;
+    atomicMin(&s_ends[0], low);
+    atomicMin(&s_ends[1], ~high);
+  }
+  __syncthreads();
+  u32 from = s_ends[0], to = ~s_ends[1];    // the number that is looked for lies here, if any
+  int want = budget - min(a.first + a.last, len);  // and is the want-th largest of them (the others above it are counted)
+  u32 least = ~0u;                           // all of the numbers above it or at it stay, but ties
+  while (want > 0) {
+    // (to - from + 1 numbers in bins of 2^shift)
+    const int bits = 32 - __builtin_clz((to - from) | 1), shift = max(bits - kBinsLog2, 0);
+    for (int i = threadIdx.x; i < kBins; i += kKeepWaves * 64) bins[i] = 0;
+    __syncthreads();
+    each([&](int, u32 x) {
+      if (x >= from && x <= to) atomicAdd(&bins[(x - from) >> shift], 1);
+    });
+    __syncthreads();
+    // wave 0 adds up the bins from the last on, 64 runs of them
+    if (wave == 0) {
+      constexpr int kRun = kBins / 64;
+      const int at = kBins - (lane + 1) * kRun;
+      int sum = 0;
+      for (int i = 0; i < kRun; ++i) sum += bins[at + i];
+      int all;
+      int before = lanes_before(sum, lane, all);
+      if (before < want && before + sum >= want) {  // (one lane's run)
+        int i = kRun - 1;
+        while (before + bins[at + i] < want) before += bins[at + i--];
+        s_found[0] = at + i;
+        s_found[1] = before;
+        s_found[2] = bins[at + i];
+      }
+    }
+    __syncthreads();
+    const int bin = s_found[0], some = s_found[2];
+    want -= s_found[1];
+    const u32 start = from + ((u32)bin << shift);
+    if (shift == 0 || some == want) {  // (a bin of one number; or all of it stays)
+      least = start;
+      break;
+    }
+    to = min(to, start + (1u << shift) - 1);
+    from = start;
+    __syncthreads();
+  }
+  // the numbers above `least` stay, and of those at it the first ones (where its bin stays as a whole, all of them do)
+  int above = 0, equal = 0;
+  each([&](int, u32 x) {
+    above += __popcll(__ballot(x > least));
+    equal += __popcll(__ballot(x == least));
+  });
+  if (lane == 0) {
+    s_above[wave] = above;
+    s_ties[wave] = equal;
   }
   __syncthreads();
   int all_above = 0, above_before = 0, ties_before = 0;
 #pragma unroll
   for (int w = 0; w < kKeepWaves; ++w) {
-    all_above += counts[0][w];
+    all_above += s_above[w];
     if (w < wave) {
-      above_before += counts[0][w];
-      ties_before += ties[w];
+      above_before += s_above[w];
+      ties_before += s_ties[w];
     }
   }
-  const int room = budget - all_above;  // for keys at `least`, the first ones
+  const int room = budget - all_above;  // for numbers at `least`
   int left = max(room - ties_before, 0), at = above_before + min(ties_before, room);
-  auto put = [&](int i, u32 x) {
+  each([&](int i, u32 x) {
     const uint64_t before = (1ull << lane) - 1, tie = __ballot(x == least);
     const bool mine = x > least || (x == least && __popcll(tie & before) < left);
     const uint64_t all = __ballot(mine);
     if (mine) out[at + __popcll(all & before)] = (int)(base + i * 64 + lane);
     at += __popcll(all);
     left -= min(left, __popcll(tie));
-  };
-  if constexpr (kHeld) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) put(i, k[i]);
-  } else {
-    for (int i = 0; i < rounds; ++i) put(i, key_at(i));
-  }
+  });
 }
 
 // ---- their move ------------------------------------------------------------------
-// A workgroup takes a run of the keys, or of the values, of a sequence's kv head. In place it takes all of them, one
-// run after the other: a run is read whole before it is written, and places that ascend lie at their number or behind it,
-// so that later runs read nothing that was written. The weights, which may be moved in place beside keys that are not,
-// are always one workgroup's.
+// A workgroup takes the keys, or the values, of a sequence's kv head: of a list's entries kMoveEntries, whose addresses it first
+// works out together in LDS, then their rows in runs, one run's reads under way beside the run before it. Into pages of their
+// own a workgroup moves one run; in place one workgroup moves all: a run is read whole before it is written, and places
+// that ascend lie at their number or behind it, so that later runs read nothing that was written. The weights, which may be
+// moved in place beside keys that are not, are always one workgroup's.
 
 constexpr int kMoveLoads = 8;  // of 16 bytes (a weight), a thread's of a run
+constexpr int kMoveEntries = 2048;
 
 // All reads of the workgroup have come.
 DQ_DEV void reads_done() {
@@ -271,6 +516,8 @@ DQ_DEV void move_weights(const int32_t* kept, int64_t count, int len, const floa
 
 template <bool kInPlace>
 __global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int lanes_log2, int runs) {
+  constexpr int kEntries = kInPlace ? kMoveEntries : 0;
+  __shared__ v4i s_move[kInPlace ? kEntries : 1];  // of an entry: page and place that it comes from (page -1: none), that it goes to
   const CacheArgs& ca = a.cache;
   const int jobs = 2 * (kInPlace ? 1 : runs) + (c.mass != nullptr);
   u32 item = blockIdx.x;
@@ -279,7 +526,7 @@ __global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int 
   const int job = item % jobs, b = item / jobs;
   const int len = seq_len(a, b);
   const int32_t* kept = c.kept + ((int64_t)b * ca.kv_heads + h) * c.budget;
-  const int64_t most = min(c.budget, (int64_t)len);  // (entries behind are none of kv_keep's)
+  const int most = (int)min(c.budget, (int64_t)len);  // (entries behind are none of kv_keep's)
   if (c.mass != nullptr && job == jobs - 1) {
     const int64_t at = b * c.seq + h * c.head;
     move_weights(kept, most, len, c.mass + at, c.mass_out + at);
@@ -289,44 +536,88 @@ __global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int 
   const int32_t* to = kInPlace ? from : c.to_pages + b * c.to_stride;
   uint16_t* pool = (job & 1 ? ca.v : ca.k) + h * ca.head;
   const int rows = 256 >> lanes_log2, r = threadIdx.x >> lanes_log2, d = 8 * (threadIdx.x & ((1 << lanes_log2) - 1));
-  const int run_rows = rows * kMoveLoads, run0 = kInPlace ? 0 : job >> 1;
-  for (int run = run0; run < (kInPlace ? runs : run0 + 1); ++run) {
-    const int64_t i0 = (int64_t)run * run_rows;
-    if (i0 >= most) break;  // (all threads)
+  const int run_rows = rows * kMoveLoads;
+  auto move_of = [&](int i) {
+    v4i e = {-1, 0, 0, 0};
+    const int place = i < most ? kept[i] : -1;
+    if (place < 0 || place >= len) return e;
+    const int sp = place / ca.page_size, tp = i / ca.page_size;
+    const int sid = from[sp], tid = to[tp];
+    if ((u32)sid < (u32)ca.n_pages && (u32)tid < (u32)ca.n_pages) e = v4i{sid, place - sp * ca.page_size, tid, i - tp * ca.page_size};
+    return e;
+  };
+  const bool in = d < a.dim;
+  auto source = [&](v4i e) { return reinterpret_cast<const v4u*>(pool + e[0] * ca.page + e[1] * ca.token + d); };
+  auto target = [&](v4i e) { return reinterpret_cast<v4u*>(pool + e[2] * ca.page + e[3] * ca.token + d); };
+  if constexpr (!kInPlace) {
+    const int i0 = (job >> 1) * run_rows;
+    v4i e[kMoveLoads];
     v4u x[kMoveLoads];
-    int64_t target[kMoveLoads];
 #pragma unroll
-    for (int u = 0; u < kMoveLoads; ++u) {
-      const int64_t i = i0 + u * rows + r;
-      const int place = i < most && d < a.dim ? kept[i] : -1;
-      target[u] = -1;
-      if (place < 0 || place >= len) continue;
-      const int sp = place / ca.page_size, tp = (int)i / ca.page_size;
-      const int sid = from[sp], tid = to[tp];
-      if ((u32)sid >= (u32)ca.n_pages || (u32)tid >= (u32)ca.n_pages) continue;
-      x[u] = *reinterpret_cast<const v4u*>(pool + sid * ca.page + (place - sp * ca.page_size) * ca.token + d);
-      target[u] = tid * ca.page + ((int)i - tp * ca.page_size) * ca.token + d;
-    }
-    if (kInPlace) reads_done();
+    for (int u = 0; u < kMoveLoads; ++u) e[u] = move_of(i0 + u * rows + r);
 #pragma unroll
     for (int u = 0; u < kMoveLoads; ++u)
-      if (target[u] >= 0) *reinterpret_cast<v4u*>(pool + target[u]) = x[u];
+      if (in && e[u][0] >= 0) x[u] = *source(e[u]);
+#pragma unroll
+    for (int u = 0; u < kMoveLoads; ++u)
+      if (in && e[u][0] >= 0) *target(e[u]) = x[u];
+  } else {
+    for (int c0 = 0; c0 < most; c0 += kEntries) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kEntries / 256; ++u) s_move[u * 256 + threadIdx.x] = move_of(c0 + u * 256 + threadIdx.x);
+      __syncthreads();
+      const int end = min(kEntries, most - c0);
+      v4u x[2][kMoveLoads];
+      auto read = [&](int i0, v4u (&y)[kMoveLoads]) {
+#pragma unroll
+        for (int u = 0; u < kMoveLoads; ++u) {
+          const v4i e = s_move[min(i0 + u * rows + r, kEntries - 1)];
+          if (in && i0 + u * rows + r < end && e[0] >= 0) y[u] = *source(e);
+        }
+      };
+      auto write = [&](int i0, v4u (&y)[kMoveLoads]) {
+        // (the run's reads have come, of all waves; those of the next one may be under way)
+#pragma unroll
+        for (int u = 0; u < kMoveLoads; ++u) asm volatile("" : "+v"(y[u]) : : "memory");
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kMoveLoads; ++u) {
+          const v4i e = s_move[min(i0 + u * rows + r, kEntries - 1)];
+          if (in && i0 + u * rows + r < end && e[0] >= 0) *target(e) = y[u];
+        }
+      };
+      read(0, x[0]);
+      for (int i0 = 0; i0 < end; i0 += 2 * run_rows) {
+        if (i0 + run_rows < end) read(i0 + run_rows, x[1]);
+        write(i0, x[0]);
+        if (i0 + run_rows >= end) break;
+        if (i0 + 2 * run_rows < end) read(i0 + 2 * run_rows, x[0]);
+        write(i0 + run_rows, x[1]);
+      }
+    }
   }
 }
 
 }  // namespace
 
+// Rows of a sequence from which on its queries go through LDS. XXX
+constexpr int kManyRows = 64;
+
 hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, const MassArgs& m, hipStream_t s) {
   const int tiles = (a.max_len + kMassKeys - 1) / kMassKeys;
   const dim3 grid((uint32_t)((int64_t)a.batch * m.splits * tiles * a.cache.kv_heads));
+  const bool many = (int64_t)a.max_q * a.group >= kManyRows;
   const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
-    if (a.dim <= 64)
-      hipLaunchKernelGGL((k_mass<tq(), tc(), 64>), grid, dim3(256), 0, s, a, m, tiles);
-    else if (a.dim <= 128)
-      hipLaunchKernelGGL((k_mass<tq(), tc(), 128>), grid, dim3(256), 0, s, a, m, tiles);
-    else
-      hipLaunchKernelGGL((k_mass<tq(), tc(), 256>), grid, dim3(256), 0, s, a, m, tiles);
-    return hipGetLastError();
+    const auto go = [&](auto dp) {
+      if (many)
+        hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);
+      else
+        hipLaunchKernelGGL((k_mass<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);
+      return hipGetLastError();
+    };
+    if (a.dim <= 64) return go(std::integral_constant<int, 64>{});
+    return a.dim <= 128 ? go(std::integral_constant<int, 128>{}) : go(std::integral_constant<int, 256>{});
   });
   if (e != hipSuccess || m.part == nullptr) return e;
   const int64_t keys = (int64_t)a.batch * a.cache.kv_heads * a.max_len;

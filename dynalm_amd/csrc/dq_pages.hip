@@ -150,15 +150,22 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   const int hk = a.cache.kv_heads, page_tiles = (c.pages + 15) / 16;
   const int h = (int)(item % hk), p0 = (int)(item / hk % page_tiles) * 16;
   const int range = (int)(item / hk / page_tiles % ranges), b = (int)(item / hk / page_tiles / ranges);
-  // the range's tokens, of the launch's
+  // the range's tokens, of the launch's (offsets, length and page numbers under way together)
   const int64_t lo = a.q_offsets != nullptr ? a.q_offsets[b] : b, hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
+  const int listed = a.pages[b * a.pages_stride + min(p0 + n, c.pages - 1)];
+  const int pages = (seq_len(a, b) + a.cache.page_size - 1) / a.cache.page_size;
   const int64_t end = min(min(hi, (int64_t)a.tokens), (int64_t)token0 + c.tokens);
   const int64_t first = max(lo, (int64_t)token0) + (int64_t)range * range_tokens, last = min(first + range_tokens, end);
-  const int pages = (seq_len(a, b) + a.cache.page_size - 1) / a.cache.page_size;
   if (p0 >= pages || first >= last) return;
+  const int slots = 16 / lanes, slot = n / lanes, blocks = (a.group + 15) / 16;
+  RawQ<T, DP> raw;
+  auto read_q = [&](int64_t t0, int block) {  // (a lane past the heads takes the last again)
+    load_q<T, DP>(a, true, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + n % lanes, a.group - 1), g, raw);
+  };
+  read_q(first, 0);
 
   // the bounds as A operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values
-  const int id = p0 + n < pages ? a.pages[b * a.pages_stride + p0 + n] : 0;
+  const int id = p0 + n < pages ? listed : 0;
   const bool bad = (u32)id >= (u32)a.cache.n_pages;
   const uint16_t* near = c.bounds + ((int64_t)(bad ? 0 : id) * hk + h) * 2 * a.dim;
   v4u x[2][NS], most[NS];
@@ -178,15 +185,12 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
       most[s][e] = __builtin_bit_cast(u32, __builtin_elementwise_max(u, v));
     }
   const float error = score_error<T, TC>(a.dim);
-  const int slots = 16 / lanes, slot = n / lanes, blocks = (a.group + 15) / 16;
   for (int64_t t0 = first; t0 < last; t0 += slots) {
     const int t = (int)min(t0 + slot, last - 1);
     float low[4], high[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
-    for (int block = 0; block < blocks; ++block) {  // (a lane past the heads takes the last again)
-      RawQ<T, DP> raw;
-      load_q<T, DP>(a, true, t, h * a.group + min(16 * block + n % lanes, a.group - 1), g, raw);
+    for (int block = 0; block < blocks; ++block) {
       int e2 = 0;
       if constexpr (T == DQ_F32 && TC == DQ_F16) {  // scaled to a largest value in [2^14, 2^15)
         float top = 0;
@@ -226,6 +230,10 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
         }
         size = mma<TC>(most[s], mag, size);
       }
+      if (block + 1 < blocks)
+        read_q(t0, block + 1);
+      else if (t0 + slots < last)
+        read_q(t0 + slots, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float d = fmaf(error, size[i], 0x1p-118f);
@@ -260,33 +268,46 @@ DQ_DEV double lanes_sum(double x, int log2) {
   return x;
 }
 
-// The 64-bit score of row t on a page, as a whole number that orders as it does: a wave's work, 2^log2 lanes a query head.
-template <int T, int TC>
-DQ_DEV uint64_t exact_key(const AttnArgs& a, const ChooseArgs& c, int t, int h, int id, int log2, int lane) {
-  if ((u32)id >= (u32)a.cache.n_pages) return kNanKey;
-  const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), heads = 64 >> log2;
+// The 64-bit scores of row t's query heads on `count` pages id(j), as whole numbers that order as they do: most[j] (in LDS, 0 before) is the
+// largest over the heads. A wave's work, from its first pair of page and head on, every `step`th: 2^log2 lanes each, kPairs pairs'
+// loads under way together.
+template <int T, int TC, class F>
+DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int count, F&& id_of, uint64_t* most, int first, int step, int log2,
+                       int lane) {
+  constexpr int kPairs = 2;
+  const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), at_once = 64 >> log2;
   const bool in = d < a.dim;
-  const uint16_t* near = c.bounds + ((int64_t)id * a.cache.kv_heads + h) * 2 * a.dim + (in ? d : 0);
-  const v4u lo = *reinterpret_cast<const v4u*>(near), hi = *reinterpret_cast<const v4u*>(near + a.dim);
-  uint64_t best = 0;
-  for (int i0 = 0; i0 < a.group; i0 += heads) {  // (a lane past the heads takes the last again)
-    const int head = h * a.group + min(i0 + (lane >> log2), a.group - 1);
-    const int64_t at = (int64_t)t * a.q_token + (int64_t)head * a.q_head + d;
-    double s = 0;
+  const int pairs = count * a.group;
+  for (int i0 = first * at_once * kPairs; i0 < pairs; i0 += step * at_once * kPairs) {
+    v4u lo[kPairs], hi[kPairs];
+    float q[kPairs][8];
+    int page[kPairs];
+    bool bad[kPairs];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q = in ? load1<T>(a.q, at + e) : 0.f;
-      const u32 x = q > 0 ? hi[e / 2] : lo[e / 2];
-      s = fma((double)q, (double)(e % 2 ? widen_hi<TC>(x) : widen<TC>(x)), s);
+    for (int k = 0; k < kPairs; ++k) {
+      const int i = min(i0 + k * at_once + (lane >> log2), pairs - 1);  // (past the pairs: the last again)
+      page[k] = i / a.group;
+      const int id = id_of(page[k]);
+      bad[k] = (u32)id >= (u32)a.cache.n_pages;
+      const uint16_t* near = c.bounds + ((int64_t)(bad[k] ? 0 : id) * a.cache.kv_heads + h) * 2 * a.dim + (in ? d : 0);
+      lo[k] = *reinterpret_cast<const v4u*>(near);
+      hi[k] = *reinterpret_cast<const v4u*>(near + a.dim);
+      const int64_t at = (int64_t)t * a.q_token + (int64_t)(h * a.group + i - page[k] * a.group) * a.q_head + d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[k][e] = in ? load1<T>(a.q, at + e) : 0.f;
     }
-    const uint64_t key = order_key(lanes_sum(in ? s : 0.0, log2));
-    best = key > best ? key : best;
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      double s = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const u32 x = q[k][e] > 0 ? hi[k][e / 2] : lo[k][e / 2];
+        s = fma((double)q[k][e], (double)(e % 2 ? widen_hi<TC>(x) : widen<TC>(x)), s);
+      }
+      const uint64_t key = order_key(lanes_sum(in ? s : 0.0, log2));
+      if ((lane & (lanes - 1)) == 0) atomicMax((unsigned long long*)&most[page[k]], (unsigned long long)(bad[k] ? kNanKey : key));
+    }
   }
-  for (int m = lanes; m < 64; m <<= 1) {
-    const uint64_t o = __shfl_xor(best, m, 64);
-    best = o > best ? o : best;
-  }
-  return best;
 }
 
 // Keys of all of a row's pages in 64 bits, where too many meet at the border: they take the intervals' place.
@@ -306,6 +327,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
   const int64_t row = (int64_t)blockIdx.x * R + r;
   if (row >= rows) return;
   const int t = token0 + (int)(row / hk), h = (int)(row % hk);
+  uint64_t* keys = c.keys + row * c.pages;
+  v2f held[N];  // the intervals, under way before anything is known of the row
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      held[i] = c.keys != nullptr ? *reinterpret_cast<const v2f*>(keys + min((w * N + i) * 64 + lane, c.pages - 1)) : v2f{0, 0};
+  }
   const int b = find_seq(a, t, lane);
   if (b < 0) return;
   const int pages = (row_sees(a, b, t, seq_len(a, b)) + a.cache.page_size - 1) / a.cache.page_size;
@@ -317,20 +345,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     return;
   }
   const int32_t* list = a.pages + b * a.pages_stride;
-  uint64_t* keys = c.keys + row * c.pages;
   const int rounds = kHeld ? N : (pages + 64 * W - 1) / (64 * W), base = w * rounds * 64;
-  auto interval = [&](int i, u32& low, u32& high) {
+  auto interval = [&](int i, v2f x, u32& low, u32& high) {
     const int p = base + i * 64 + lane;
-    low = high = p < pages ? ~0u : 0u;  // (0: no page)
-    if (p < c.first || p >= pages - c.last) return;
-    const v2f x = *reinterpret_cast<const v2f*>(keys + p);
-    low = order_key(x[0]);
-    high = order_key(x[1]);
+    const bool always = p < c.first || p >= pages - c.last;
+    low = p >= pages ? 0u : always ? ~0u : order_key(x[0]);  // (0: no page)
+    high = p >= pages ? 0u : always ? ~0u : order_key(x[1]);
   };
   u32 low[N], high[N];
+  if constexpr (kHeld) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (kHeld) interval(i, low[i], high[i]);
+    for (int i = 0; i < N; ++i) interval(i, held[i], low[i], high[i]);
+  }
   // the sum over the row's waves
   int turn = 0;
   auto all_waves = [&](int n) {
@@ -351,17 +377,30 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     } else {
       for (int i = 0; i < rounds; ++i) {
         u32 l, u;
-        interval(i, l, u);
+        interval(i, *reinterpret_cast<const v2f*>(keys + min(base + i * 64 + lane, c.pages - 1)), l, u);
         f(i, l, u);
       }
     }
   };
-  // the n-th largest; early: or a lower one with the same n above it or at it
-  auto nth = [&](int n, bool highs, bool early) {
-    u32 least = 0;
+  // the least over the row's waves
+  auto all_least = [&](u32 x) {
+    x = wave_least(x);
+    if constexpr (W == 1) return x;
+    turn ^= 1;
+    if (lane == 0) s_counts[turn][w] = (int)x;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) x = min(x, (u32)s_counts[turn][i]);
+    return x;
+  };
+  // the n-th largest low (high) end, of values from `bottom` to `top` (and pages of ~0, which are above); early: or a lower
+  // value with n ends above it or at it
+  auto nth = [&](int n, u32 bottom, u32 top, bool highs, bool early) {
+    int bit = 31 - __builtin_clz((bottom ^ top) | 1);
+    u32 least = top & ~((2u << bit) - 1);
     int taken = 0;
 #pragma unroll 1
-    for (int bit = 31; bit >= 0 && !(early && taken == n); --bit) {
+    for (; bit >= 0 && !(early && taken == n); --bit) {
       const u32 mid = least | 1u << bit;
       int k = 0;
       each([&](int, u32 l, u32 u) { k += __popcll(__ballot((highs ? u : l) >= mid)); });
@@ -374,12 +413,38 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     return least;
   };
   // A page whose high end is below the count-th largest low end is out; one whose low end is above the next high
-  // end after the count-th is in; the others are looked at again.
-  const u32 floor = nth(count, false, true);
+  // end after the count-th is in; the others are open.
+  u32 bottom = ~0u, top = 0;
+  each([&](int, u32 l, u32) {
+    if (l != 0) bottom = min(bottom, l);
+    if (l != ~0u) top = max(top, l);
+  });
+  bottom = all_least(bottom);
+  top = ~all_least(~top);
+  const u32 floor = count <= c.first + c.last ? ~0u : nth(count, bottom, top, false, true);
   int able = 0;
   each([&](int, u32, u32 u) { able += __popcll(__ballot(u >= floor)); });
   able = all_waves(able);
-  const u32 ceiling = able > count ? nth(count + 1, true, false) : 0u;
+  u32 ceiling = 0;
+  int over = able - count;  // the next high end is the over-th least of those able
+  if (over > 0 && over <= 8) {
+    u32 from = floor;
+    while (true) {
+      u32 least = ~0u;
+      each([&](int, u32, u32 u) {
+        if (u >= from) least = min(least, u);
+      });
+      least = all_least(least);
+      int same = 0;
+      each([&](int, u32, u32 u) { same += __popcll(__ballot(u == least)); });
+      over -= all_waves(same);
+      ceiling = least;
+      if (over <= 0) break;
+      from = least + 1;
+    }
+  } else if (over > 0) {
+    ceiling = nth(count + 1, 0u, ~1u, true, false);
+  }
   const bool all_in = able == count;
   int open = 0;
   if (!all_in) each([&](int, u32 l, u32 u) { open += __popcll(__ballot(u >= floor && l <= ceiling)); });
@@ -391,6 +456,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
   uint64_t taken = 0;  // of the open ones, in their order
   if (open > 0 && open <= 64) {
     int at = before;
+    s_key[r][lane] = 0;  // (of all waves alike)
     each([&](int i, u32 l, u32 u) {
       const bool mine = u >= floor && l <= ceiling;
       const uint64_t m = __ballot(mine);
@@ -399,10 +465,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     });
     if constexpr (W > 1) __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    for (int j = w; j < open; j += W) {
-      const uint64_t key = exact_key<T, TC>(a, c, t, h, s_list[r][j], log2, lane);
-      if (lane == 0) s_key[r][j] = key;
-    }
+    exact_keys<T, TC>(a, c, t, h, open, [&](int j) { return s_list[r][j]; }, s_key[r], w, W, log2, lane);
     if constexpr (W > 1) __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     const uint64_t key = lane < open ? s_key[r][lane] : 0;
@@ -413,9 +476,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     }
     taken = __ballot(lane < open && rank < room);
   } else if (open > 64) {
-    for (int p = w; p < pages; p += W) {
-      const uint64_t key = p < c.first || p >= pages - c.last ? kAlways : exact_key<T, TC>(a, c, t, h, list[p], log2, lane);
-      if (lane == 0) store_key(keys + p, key);
+    for (int p0 = 0; p0 < pages; p0 += 64) {
+      const int some = min(64, pages - p0);
+      s_key[r][lane] = 0;
+      if constexpr (W > 1) __syncthreads();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      exact_keys<T, TC>(a, c, t, h, some, [&](int j) { return list[p0 + j]; }, s_key[r], w, W, log2, lane);
+      if constexpr (W > 1) __syncthreads();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      const int p = p0 + lane;
+      if (w == 0 && lane < some) store_key(keys + p, p < c.first || p >= pages - c.last ? kAlways : s_key[r][lane]);
+      if constexpr (W > 1) __syncthreads();
     }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "agent");
     if constexpr (W > 1) __syncthreads();

@@ -183,7 +183,7 @@ struct MassPlan {
 };
 
 // Items that a launch of dq_attention_mass aims at, keys of one, and rows that are worth one.
-constexpr int64_t kMassItems = 1024, kMassKeys = 256, kMassRows = 128;
+constexpr int64_t kMassItems = 2048, kMassKeys = 256, kMassRows = 256;
 
 MassPlan plan_mass(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* q) {
   MassPlan p;
@@ -191,7 +191,7 @@ MassPlan plan_mass(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* 
   const int64_t items = s->batch * c->kv_heads * ceil_div(s->max_len, kMassKeys), keys = s->batch * c->kv_heads * s->max_len * 4;
   if (items > 0 && rows > 0) {
     p.splits = std::max<int64_t>(1, std::min({kMassItems / items, rows / kMassRows, kWorkspace / keys}));
-    p.rows = ceil_div(ceil_div(rows, p.splits), 16) * 16;
+    p.rows = ceil_div(ceil_div(rows, p.splits), 64) * 64;
     p.splits = ceil_div(rows, p.rows);
   }
   p.items = items * p.splits;

@@ -313,6 +313,8 @@ MASSES = [
     pytest.param([33, 64], [33, 70], 2, 2, 256, 16, id="prompts"),
     pytest.param([4, 6], [2, 3], 2, 1, 40, 16, id="rows before the first key"),
     pytest.param([300], [300], 4, 1, 96, 32, id="several ranges of rows"),
+    pytest.param([130, 3, 90], [700, 300, 90], 6, 2, 136, 48, id="prompts, heads of 136"),
+    pytest.param([200], [650], 7, 1, 48, 16, id="prompt, 7 heads a kv head"),
 ]
 
 
