@@ -56,7 +56,7 @@ DQ_DEV void load_keys(const AttnArgs& a, int b, int head, int k0, int len, int n
 }
 
 // The sums over a wave's rows into the weights, or into the range's part.
-DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int range, int k0, int len, int old, int n, int g, float (&sum)[kMassTiles],
+DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int part, int k0, int len, int old, int n, int g, float (&sum)[kMassTiles],
                      const bool (&bad)[kMassTiles]) {
   const CacheArgs& ca = a.cache;
 #pragma unroll
@@ -68,7 +68,7 @@ DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int 
   const int key = k0 + 16 * g + n;
   if (key >= len) return;
   if (m.part != nullptr) {
-    m.part[(((int64_t)range * a.batch + b) * ca.kv_heads + head) * a.max_len + key] = x;
+    m.part[(((int64_t)part * a.batch + b) * ca.kv_heads + head) * a.max_len + key] = x;
     return;
   }
   float* out = m.mass + b * m.seq + head * m.head + key;
@@ -84,9 +84,9 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
   u32 item = blockIdx.x;
   const int head = item % ca.kv_heads;
   item /= ca.kv_heads;
-  const int kt = item % key_tiles;
-  item /= key_tiles;
-  const int range = item % m.splits, b = item / m.splits;
+  const int part = item % m.splits;
+  item /= m.splits;
+  const int kt = item % key_tiles, b = item / key_tiles;
   const int len = seq_len(a, b), k0 = (kt * 4 + wave) * 16 * kMassTiles;
   if (k0 >= len) return;
   int first, count;
@@ -100,12 +100,11 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
   float sum[kMassTiles];
 #pragma unroll
   for (int i = 0; i < kMassTiles; ++i) sum[i] = 0;
-  // rows before the first that sees key k0 add nothing
-  const int rows = count * a.group;
+  // rows before the first that sees key k0 add nothing; of the others every splits-th 16 are this part's
+  const int rows = count * a.group, r_end = rows;
   const int64_t sees_from = max((int64_t)0, (int64_t)(k0 - old) * a.group);
-  const int r_end = (int)min((int64_t)rows, m.splits > 1 ? (int64_t)(range + 1) * m.rows : (int64_t)rows);
-  int r0 = (int)max((int64_t)range * m.rows, sees_from / 16 * 16);
-  for (; r0 < r_end; r0 += 16) {
+  for (int64_t at = sees_from + 16 * part; at < r_end; at += 16 * m.splits) {
+    const int r0 = (int)at;
     const int r = min(r0 + n, rows - 1), token = first + r / a.group, qh = head * a.group + r % a.group;
     const bool valid = r0 + n < r_end;
     RawQ<T, DP> raw;
@@ -141,25 +140,28 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
       }
     }
   }
-  put_mass(a, m, b, head, range, k0, len, old, n, g, sum, bad);
+  put_mass(a, m, b, head, part, k0, len, old, n, g, sum, bad);
 }
 
-// Many rows: the same with the rows' queries through LDS, kMassRows at a time and two buffers deep, for the four waves
-// together; a row's 16-byte chunks lie at their number XOR some bits of the row's, which spreads a column of rows over the banks.
+// Many rows: the same with the rows' queries through LDS for the four waves together, two buffers deep. A tile is as many
+// whole tokens as kMassRows rows hold, so that a thread's rows lie at the same offsets from every tile's first token (rows that
+// are left have a weight of 0); a row's 16-byte chunks lie at their number XOR some bits of the row's, which spreads a
+// column of rows over the banks. The products of 16 rows stand beside the exponentials of the 16 before.
+// A prompt of 4,096 tokens, 32 / 8 f16 heads of 128 (68.7 GFLOP): XXX us.
 
 template <int T>
 constexpr int kMassRows = T == DQ_F32 ? 32 : 64;
 
 template <int T, int TC, int DP>
 struct MassLds {
-  uint16_t q[2][kParts<T, TC>][kMassRows<T> * DP];
-  float hi[2][kMassRows<T>], f[2][kMassRows<T>], c[2][kMassRows<T>];
-  int limit[2][kMassRows<T>];
+  alignas(16) uint16_t q[2][kParts<T, TC>][kMassRows<T> * DP];
+  alignas(16) float hi[2][kMassRows<T>], f[2][kMassRows<T>], c[2][kMassRows<T>];
+  alignas(16) int token[kMassRows<T>];  // of a tile's row
 };
 
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256) void k_mass_many(AttnArgs a, MassArgs m, int key_tiles) {
-  constexpr int NP = kParts<T, TC>, QR = kMassRows<T>;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 3 : 1, DP <= 128 ? 3 : 2))) void k_mass_many(AttnArgs a, MassArgs m, int key_tiles) {
+  constexpr int NP = kParts<T, TC>, QR = kMassRows<T>, kBytes = T == DQ_F32 ? 4 : 2;
   constexpr int kChunks = DP / 8, kPasses = QR * kChunks / 256, kPassRows = 256 / kChunks;
   __shared__ MassLds<T, TC, DP> sh;
   const CacheArgs& ca = a.cache;
@@ -168,61 +170,69 @@ __global__ __launch_bounds__(256) void k_mass_many(AttnArgs a, MassArgs m, int k
   u32 item = blockIdx.x;
   const int head = item % ca.kv_heads;
   item /= ca.kv_heads;
-  const int kt = item % key_tiles;
-  item /= key_tiles;
-  const int range = item % m.splits, b = item / m.splits;
+  const int part = item % m.splits;
+  item /= m.splits;
+  const int kt = item % key_tiles, b = item / key_tiles;  // (the first keys are seen by most rows)
   const int len = seq_len(a, b);
   if (kt * kMassKeys >= len) return;
   const int k0 = kt * kMassKeys + wave * 16 * kMassTiles;
   int first, count;
   seq_rows(a, b, first, count);
   const int old = len - count;
-  const int rows = count * a.group;
-  const int r_end = (int)min((int64_t)rows, m.splits > 1 ? (int64_t)(range + 1) * m.rows : (int64_t)rows);
-  // rows before the first that sees one of the workgroup's keys add nothing
-  const int r_begin = (int)max((int64_t)range * m.rows, max((int64_t)0, (int64_t)(kt * kMassKeys - old) * a.group) / QR * QR);
+  const int step = QR / a.group;  // tokens of a tile
+  // tokens before the first that sees one of the workgroup's keys add nothing; of the others every splits-th tile is this part's
+  const int t_end = first + count, stride = step * m.splits;
+  const int t_begin = (int)min((int64_t)t_end, first + max((int64_t)0, (int64_t)kt * kMassKeys - old) + (int64_t)step * part);
 
-  // a thread's 16 bytes (fp32: 32) of a row, kPasses rows of a tile
+  // a thread's 16 bytes (fp32: 32) of a row, kPasses rows of a tile; it is the row's chunk `chunk`
   const int chunk = threadIdx.x % kChunks, pass_row = threadIdx.x / kChunks;
   v4u raw[kPasses][T == DQ_F32 ? 2 : 1];
+  u32 off[kPasses], off0[kPasses];  // in bytes from the tile's first token; of the same head of that token
+  int tok[kPasses];
+  bool in[kPasses];  // (a chunk past the head's values, a row past the tile's tokens is 0)
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = p * kPassRows + pass_row;
+    tok[p] = row / a.group;
+    in[p] = tok[p] < step && 8 * chunk < a.dim;
+    if (!in[p]) tok[p] = 1 << 30;
+    off0[p] = in[p] ? (u32)((row % a.group) * (int)a.q_head + 8 * chunk) * kBytes : 0;
+    off[p] = off0[p] + (in[p] ? (u32)(tok[p] * (int)a.q_token) * kBytes : 0);
+  }
+  const int own_row = threadIdx.x % QR, own_token = own_row / a.group;
+  if (threadIdx.x < QR) sh.token[own_row] = own_token < step ? own_token : 1 << 30;
+  const float* own_lse = m.lse + head * a.group + own_row % a.group;
   float lse = 0;
-  auto read = [&](int r0) {
+  bool lse_in = false;
+  auto read = [&](int t0) {
+    const char* base = static_cast<const char*>(a.q) + ((int64_t)t0 * a.q_token + (int64_t)head * a.group * a.q_head) * kBytes;
+    // (a token behind the last: the first; nothing sees it)
+    if (a.q_vec) {
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int r = r0 + p * kPassRows + pass_row;
-      const bool in = r < r_end && 8 * chunk < a.dim;
-      const int64_t at = (int64_t)(first + r / a.group) * a.q_token + (int64_t)(head * a.group + r % a.group) * a.q_head + 8 * chunk;
+      for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) {
-        v4u x = {0, 0, 0, 0};
-        if (in) {
-          if constexpr (T == DQ_F32) {
-            const float* src = static_cast<const float*>(a.q) + at + 4 * k;
-            if (a.q_vec)
-              x = *reinterpret_cast<const v4u*>(src);
-            else
+        for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k)
+          raw[p][k] = *reinterpret_cast<const v4u*>(base + (t0 + tok[p] < t_end ? off[p] : off0[p]) + 16 * k);
+    } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = as_u(src[i]);
-          } else {
-            const uint16_t* src = static_cast<const uint16_t*>(a.q) + at;
-            if (a.q_vec)
-              x = *reinterpret_cast<const v4u*>(src);
-            else
+      for (int p = 0; p < kPasses; ++p) {
+        const char* src = base + (t0 + tok[p] < t_end ? off[p] : off0[p]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = (u32)src[2 * i] | ((u32)src[2 * i + 1] << 16);
-          }
-        }
-        raw[p][k] = x;
+        for (int i = 0; i < (T == DQ_F32 ? 8 : 4); ++i)
+          raw[p][i / 4][i % 4] = T == DQ_F32 ? reinterpret_cast<const u32*>(src)[i]
+                                             : (u32)reinterpret_cast<const uint16_t*>(src)[2 * i] | (u32)reinterpret_cast<const uint16_t*>(src)[2 * i + 1] << 16;
       }
     }
-    const int r = r0 + (int)threadIdx.x;
-    if (threadIdx.x < QR && r < r_end) lse = m.lse[(int64_t)(first + r / a.group) * a.heads + head * a.group + r % a.group];
+    lse_in = own_token < step && t0 + own_token < t_end;
+    lse = *(own_lse + ((int64_t)t0 + (lse_in ? own_token : 0)) * a.heads);
   };
   auto place = [&](int row, int ch) { return row * DP + 8 * (ch ^ (DP == 64 ? (row >> 1) & 7 : row & 15)); };
-  auto write = [&](int r0, int buf) {
+  auto write = [&](int buf) {
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int row = p * kPassRows + pass_row;
+#pragma unroll
+      for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) raw[p][k] = in[p] ? raw[p][k] : v4u{0, 0, 0, 0};
       if constexpr (T != DQ_F32) {
         *reinterpret_cast<v4u*>(&sh.q[buf][0][place(row, chunk)]) = raw[p][0];
       } else {
@@ -247,73 +257,90 @@ __global__ __launch_bounds__(256) void k_mass_many(AttnArgs a, MassArgs m, int k
       }
     }
     if (threadIdx.x < QR) {
-      const int r = r0 + (int)threadIdx.x;
       float hi, f;
-      split_lse(lse, hi, f);
-      sh.hi[buf][threadIdx.x] = hi;
-      sh.f[buf][threadIdx.x] = f;
-      sh.limit[buf][threadIdx.x] = r < r_end ? old + r / a.group + 1 : 0;
+      split_lse(lse_in ? lse : -INFINITY, hi, f);
+      sh.hi[buf][own_row] = hi;
+      sh.f[buf][own_row] = f;
     }
   };
 
-  if (r_begin < r_end) read(r_begin);
+  if (t_begin < t_end) read(t_begin);
   v4u k[kMassTiles][DP / 32];
   bool bad[kMassTiles];
   load_keys<DP>(a, b, head, k0, len, n, g, k, bad);
   float sum[kMassTiles];
 #pragma unroll
   for (int i = 0; i < kMassTiles; ++i) sum[i] = 0;
-  if (r_begin < r_end) write(r_begin, 0);
+  // (the keys have come: else the loop would wait for them, and with them for the next rows, in every tile)
+#pragma unroll
+  for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) asm volatile("" : "+v"(k[i][s]));
+  if (t_begin < t_end) write(0);
   __syncthreads();
   int buf = 0;
-  for (int r0 = r_begin; r0 < r_end; r0 += QR, buf ^= 1) {
-    const bool more = r0 + QR < r_end;
-    if (more) read(r0 + QR);
-    // (the rows' first sees the least)
-    const bool all_see = r0 + QR <= r_end && k0 + 16 * kMassTiles <= old + r0 / a.group + 1;
-    const bool none_sees = k0 >= old + (min(r0 + QR, r_end) - 1) / a.group + 1;
-    auto tile = [&](auto masked) {
-#pragma unroll 1
-      for (int q0 = 0; q0 < QR; q0 += 16) {
-        v4u q[NP][DP / 32];
+  for (int t0 = t_begin; t0 < t_end; t0 += stride, buf ^= 1) {
+    const bool more = t0 + stride < t_end;
+    if (more) read(t0 + stride);
+    const int sees = old + t0 - first + 1;  // keys of the tile's first token
+    v4f acc[2][kMassTiles];
+    auto products = [&](int q0, v4f (&out)[kMassTiles]) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
+      for (int i = 0; i < kMassTiles; ++i) out[i] = v4f{0, 0, 0, 0};
 #pragma unroll
-          for (int s = 0; s < DP / 32; ++s) q[p][s] = *reinterpret_cast<const v4u*>(&sh.q[buf][p][place(q0 + n, 4 * s + g)]);
-        const v4f hi = *reinterpret_cast<const v4f*>(&sh.hi[buf][q0 + 4 * g]), f = *reinterpret_cast<const v4f*>(&sh.f[buf][q0 + 4 * g]);
-        v4f c = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
-        if constexpr (T == DQ_F32) c = *reinterpret_cast<const v4f*>(&sh.c[buf][q0 + 4 * g]);
-        v4i limit = {0, 0, 0, 0};
-        if constexpr (masked()) limit = *reinterpret_cast<const v4i*>(&sh.limit[buf][q0 + 4 * g]);
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) {
+          const v4u q = *reinterpret_cast<const v4u*>(&sh.q[buf][p][place(q0 + n, 4 * s + g)]);
+#pragma unroll
+          for (int i = 0; i < kMassTiles; ++i) out[i] = mma<TC>(q, k[i][s], out[i]);
+        }
+    };
+    auto weights = [&](int q0, v4f (&x)[kMassTiles], auto masked) {
+      const v4f hi = *reinterpret_cast<const v4f*>(&sh.hi[buf][q0 + 4 * g]), f = *reinterpret_cast<const v4f*>(&sh.f[buf][q0 + 4 * g]);
+      v4f c = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+      if constexpr (T == DQ_F32) c = *reinterpret_cast<const v4f*>(&sh.c[buf][q0 + 4 * g]);
+      v4i token = {0, 0, 0, 0};
+      if constexpr (masked()) token = *reinterpret_cast<const v4i*>(&sh.token[q0 + 4 * g]);
+#pragma unroll
+      for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = fmaf(x[i][e], c[e], -hi[e]);
+#pragma unroll
+      for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = exp2_fast(x[i][e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int limit = token[e] < t_end - t0 ? sees + token[e] : 0;
 #pragma unroll
         for (int i = 0; i < kMassTiles; ++i) {
-          v4f acc = {0, 0, 0, 0};
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-            for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(q[p][s], k[i][s], acc);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float w = exp2_fast(fmaf(acc[e], c[e], -hi[e]));
-            if constexpr (masked())
-              sum[i] += k0 + 16 * i + n < limit[e] ? w * f[e] : 0.f;
-            else
-              sum[i] = fmaf(w, f[e], sum[i]);
-          }
+          if constexpr (masked())
+            sum[i] += k0 + 16 * i + n < limit ? x[i][e] * f[e] : 0.f;
+          else
+            sum[i] = fmaf(x[i][e], f[e], sum[i]);
         }
       }
     };
-    if (all_see)
+    auto tile = [&](auto masked) {
+      products(0, acc[0]);
+#pragma unroll
+      for (int j = 0; j < QR / 16; ++j) {
+        if (j + 1 < QR / 16) products(16 * j + 16, acc[(j + 1) & 1]);
+        weights(16 * j, acc[j & 1], masked);
+      }
+    };
+    if (t0 + step <= t_end && k0 + 16 * kMassTiles <= sees)
       tile(std::false_type{});
-    else if (!none_sees)
+    else if (k0 < sees + min(step, t_end - t0) - 1)  // (the last token sees the most)
       tile(std::true_type{});
-    if (more) write(r0 + QR, buf ^ 1);
+    if (more) write(buf ^ 1);
     __syncthreads();
   }
-  put_mass(a, m, b, head, range, k0, len, old, n, g, sum, bad);
+  put_mass(a, m, b, head, part, k0, len, old, n, g, sum, bad);
 }
 
-// Adds the ranges of rows that were summed apart.
+// Adds the parts of the rows that were summed apart.
 __global__ __launch_bounds__(256) void k_mass_join(AttnArgs a, MassArgs m, int64_t keys) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= keys) return;
@@ -359,10 +386,10 @@ DQ_DEV int lanes_before(int x, int lane, int& all) {
 
 template <int N, bool kHeld>
 __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
+  constexpr int kThreads = kKeepWaves * 64, kOwn = kBins / kThreads;
   __shared__ int bins[kBins];
-  __shared__ int s_above[kKeepWaves], s_ties[kKeepWaves];
-  __shared__ u32 s_ends[2];  // least, largest (turned round); the bin that is looked for
-  __shared__ int s_found[3];
+  __shared__ u32 s_low[kKeepWaves], s_high[kKeepWaves];
+  __shared__ int s_above[kKeepWaves], s_ties[kKeepWaves], s_found[3];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads;
   const int len = a.max_len > 0 ? min(max(a.lens[b], 0), a.max_len) : 0;
@@ -393,9 +420,7 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
       for (int i = 0; i < rounds; ++i) f(i, key_at(i));
     }
   };
-  // where the numbers of places without a place of their own lie
-  if (threadIdx.x < 2) s_ends[threadIdx.x] = ~0u;
-  __syncthreads();
+  // the least and the largest number of those that are not kept in any case
   u32 low = ~0u, high = 0;
   each([&](int, u32 x) {
     if (x != 0) low = min(low, x);
@@ -404,36 +429,51 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
   low = wave_least(low);
   high = ~wave_least(~high);
   if (lane == 0) {
-    atomicMin(&s_ends[0], low);
-    atomicMin(&s_ends[1], ~high);
+    s_low[wave] = low;
+    s_high[wave] = high;
   }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) bins[threadIdx.x * kOwn + i] = 0;
   __syncthreads();
-  u32 from = s_ends[0], to = ~s_ends[1];    // the number that is looked for lies here, if any
-  int want = budget - min(a.first + a.last, len);  // and is the want-th largest of them (the others above it are counted)
-  u32 least = ~0u;                           // all of the numbers above it or at it stay, but ties
+  u32 from = ~0u, to = 0;  // the number that is looked for lies here, if any
+#pragma unroll
+  for (int w = 0; w < kKeepWaves; ++w) {
+    from = min(from, s_low[w]);
+    to = max(to, s_high[w]);
+  }
+  int want = budget - min(a.first + a.last, len);  // it is the want-th largest of the numbers there
+  u32 least = ~0u;                                 // numbers above it or at it stay, but ties
   while (want > 0) {
     // (to - from + 1 numbers in bins of 2^shift)
     const int bits = 32 - __builtin_clz((to - from) | 1), shift = max(bits - kBinsLog2, 0);
-    for (int i = threadIdx.x; i < kBins; i += kKeepWaves * 64) bins[i] = 0;
-    __syncthreads();
     each([&](int, u32 x) {
       if (x >= from && x <= to) atomicAdd(&bins[(x - from) >> shift], 1);
     });
     __syncthreads();
-    // wave 0 adds up the bins from the last on, 64 runs of them
-    if (wave == 0) {
-      constexpr int kRun = kBins / 64;
-      const int at = kBins - (lane + 1) * kRun;
-      int sum = 0;
-      for (int i = 0; i < kRun; ++i) sum += bins[at + i];
-      int all;
-      int before = lanes_before(sum, lane, all);
-      if (before < want && before + sum >= want) {  // (one lane's run)
-        int i = kRun - 1;
-        while (before + bins[at + i] < want) before += bins[at + i--];
-        s_found[0] = at + i;
-        s_found[1] = before;
-        s_found[2] = bins[at + i];
+    // a thread takes kOwn bins, the first thread the last ones: numbers in the bins above them
+    const int at = (kThreads - 1 - (int)threadIdx.x) * kOwn;
+    int own[kOwn], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      sum += own[i] = bins[at + i];
+      bins[at + i] = 0;
+    }
+    int all;
+    int before = lanes_before(sum, lane, all);
+    if (lane == 0) s_above[wave] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kKeepWaves; ++w)
+      if (w < wave) before += s_above[w];
+    if (before < want && before + sum >= want) {  // (one thread)
+#pragma unroll
+      for (int i = kOwn - 1; i >= 0; --i) {
+        if (before < want && before + own[i] >= want) {
+          s_found[0] = at + i;
+          s_found[1] = before;
+          s_found[2] = own[i];
+        }
+        before += own[i];
       }
     }
     __syncthreads();
@@ -446,8 +486,8 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
     }
     to = min(to, start + (1u << shift) - 1);
     from = start;
-    __syncthreads();
   }
+  __syncthreads();
   // the numbers above `least` stay, and of those at it the first ones (where its bin stays as a whole, all of them do)
   int above = 0, equal = 0;
   each([&](int, u32 x) {
@@ -607,8 +647,11 @@ constexpr int kManyRows = 64;
 hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, const MassArgs& m, hipStream_t s) {
   const int tiles = (a.max_len + kMassKeys - 1) / kMassKeys;
   const dim3 grid((uint32_t)((int64_t)a.batch * m.splits * tiles * a.cache.kv_heads));
-  const bool many = (int64_t)a.max_q * a.group >= kManyRows;
   const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
+    // (a tile holds whole tokens, whose rows are addressed from its first in 32 bits)
+    constexpr int kRows = kMassRows<tq()>;
+    const bool near = a.q_token < (1 << 22) && a.q_head < (1 << 22);
+    const bool many = (int64_t)a.max_q * a.group >= kManyRows && a.group <= kRows && near;
     const auto go = [&](auto dp) {
       if (many)
         hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);
@@ -630,6 +673,8 @@ hipError_t launch_kv_keep(int64_t batch, const KeepArgs& k, hipStream_t s) {
   constexpr int kLanes = kKeepWaves * 64;
   if (k.max_len <= 4 * kLanes)
     hipLaunchKernelGGL((k_keep<4, true>), grid, block, 0, s, k);
+  else if (k.max_len <= 8 * kLanes)
+    hipLaunchKernelGGL((k_keep<8, true>), grid, block, 0, s, k);
   else if (k.max_len <= 16 * kLanes)
     hipLaunchKernelGGL((k_keep<16, true>), grid, block, 0, s, k);
   else if (k.max_len <= 64 * kLanes)

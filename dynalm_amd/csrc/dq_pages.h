@@ -33,9 +33,8 @@ struct MassArgs {
   float decay = 0;
   float* mass = nullptr;
   int64_t seq = 0, head = 0;  // strides in values
-  float* part = nullptr;      // [range][sequence][kv head][key] (nullptr: one range, added at once)
-  int32_t splits = 1;         // ranges of a sequence's rows
-  int32_t rows = 0;           // rows of a range, a multiple of 16
+  float* part = nullptr;      // [part][sequence][kv head][key] (nullptr: one part, added at once)
+  int32_t splits = 1;         // parts of a sequence's rows
 };
 hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, const MassArgs& m, hipStream_t s);
 

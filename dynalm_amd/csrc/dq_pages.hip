@@ -115,17 +115,14 @@ DQ_DEV u32 order_key(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-template <int kCtrl>
-DQ_DEV float dpp_f(float x) {
-  return as_f((u32)dpp<kCtrl>((int)as_u(x)));
+// The larger of a lane's and the one's 16 (32) lanes on.
+DQ_DEV float pair_max16(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(as_u(x), as_u(x), false, false);
+  return fmaxf(as_f(a[0]), as_f(a[1]));
 }
-// The largest over each aligned group of `lanes` (1, 2, 4, 8, 16).
-DQ_DEV float lanes_max(float x, int lanes) {
-  if (lanes > 1) x = fmaxf(x, dpp_f<kQuadXor1>(x));
-  if (lanes > 2) x = fmaxf(x, dpp_f<kQuadXor2>(x));
-  if (lanes > 4) x = fmaxf(x, dpp_f<kHalfMirror>(x));
-  if (lanes > 8) x = fmaxf(x, dpp_f<kRowRor8>(x));
-  return x;
+DQ_DEV float pair_max32(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
+  return fmaxf(as_f(a[0]), as_f(a[1]));
 }
 
 template <int T>
@@ -164,7 +161,7 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   };
   read_q(first, 0);
 
-  // the bounds as A operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values
+  // the bounds as B operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values
   const int id = p0 + n < pages ? listed : 0;
   const bool bad = (u32)id >= (u32)a.cache.n_pages;
   const uint16_t* near = c.bounds + ((int64_t)(bad ? 0 : id) * hk + h) * 2 * a.dim;
@@ -175,8 +172,6 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
 #pragma unroll
     for (int i = 0; i < 2; ++i) x[i][s] = d < a.dim ? *reinterpret_cast<const v4u*>(near + i * a.dim + d) : v4u{0, 0, 0, 0};
   }
-  // of the four pages whose products the lane holds
-  const uint64_t bads = __ballot(bad);
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -186,7 +181,6 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
     }
   const float error = score_error<T, TC>(a.dim);
   for (int64_t t0 = first; t0 < last; t0 += slots) {
-    const int t = (int)min(t0 + slot, last - 1);
     float low[4], high[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
@@ -225,29 +219,51 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
         }
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          sum = mma<TC>(x[1][s], part[p] & ~down, sum);
-          sum = mma<TC>(x[0][s], part[p] & down, sum);
+          sum = mma<TC>(part[p] & ~down, x[1][s], sum);
+          sum = mma<TC>(part[p] & down, x[0][s], sum);
         }
-        size = mma<TC>(most[s], mag, size);
+        size = mma<TC>(mag, most[s], size);
       }
       if (block + 1 < blocks)
         read_q(t0, block + 1);
       else if (t0 + slots < last)
         read_q(t0 + slots, 0);
+      // the lane holds its page's products with rows 4 g .. + 3
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float d = fmaf(error, size[i], 0x1p-118f);
-        const bool fine = d < INFINITY && fabsf(sum[i]) < INFINITY && !(bads >> (4 * g + i) & 1);
-        low[i] = fmaxf(low[i], fine ? ldexpf(sum[i] - d, -e2) : -INFINITY);
-        high[i] = fmaxf(high[i], fine ? ldexpf(sum[i] + d, -e2) : INFINITY);
+        const bool fine = d < INFINITY && fabsf(sum[i]) < INFINITY && !bad;
+        const int back = T == DQ_F32 && TC == DQ_F16 ? -__shfl(e2, 4 * g + i, 64) : 0;
+        low[i] = fmaxf(low[i], fine ? ldexpf(sum[i] - d, back) : -INFINITY);
+        high[i] = fmaxf(high[i], fine ? ldexpf(sum[i] + d, back) : INFINITY);
       }
     }
-    uint64_t* out = c.keys + ((t - token0) * (int64_t)hk + h) * c.pages + p0 + 4 * g;
+    // the largest of a token's rows: of a lane's, then of two or all four lane groups
+    if (lanes > 1) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        low[i] = fmaxf(low[i], low[i + 1]);
+        high[i] = fmaxf(high[i], high[i + 1]);
+      }
+    }
+    if (lanes > 2) {
+      low[0] = fmaxf(low[0], low[2]);
+      high[0] = fmaxf(high[0], high[2]);
+    }
+    if (lanes > 4) {
+      low[0] = pair_max16(low[0]);
+      high[0] = pair_max16(high[0]);
+    }
+    if (lanes > 8) {
+      low[0] = pair_max32(low[0]);
+      high[0] = pair_max32(high[0]);
+    }
+    const int64_t row0 = t0 - token0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      low[i] = lanes_max(low[i], lanes);
-      high[i] = lanes_max(high[i], lanes);
-      if (n % lanes == 0 && t0 + slot < last && p0 + 4 * g + i < pages) *reinterpret_cast<v2f*>(out + i) = v2f{low[i], high[i]};
+      const int row = 4 * g + i, to = row / lanes;
+      if (row % lanes == 0 && t0 + to < last && p0 + n < pages)
+        *reinterpret_cast<v2f*>(c.keys + ((row0 + to) * hk + h) * c.pages + p0 + n) = v2f{low[i], high[i]};
     }
   }
 }
@@ -274,7 +290,7 @@ DQ_DEV double lanes_sum(double x, int log2) {
 template <int T, int TC, class F>
 DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int count, F&& id_of, uint64_t* most, int first, int step, int log2,
                        int lane) {
-  constexpr int kPairs = 2;
+  constexpr int kPairs = 4;
   const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), at_once = 64 >> log2;
   const bool in = d < a.dim;
   const int pairs = count * a.group;

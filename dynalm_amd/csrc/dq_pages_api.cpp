@@ -178,22 +178,18 @@ int check_page_attention(const dq_kv_cache* c, const dq_sequences* s, const dq_h
 }
 
 struct MassPlan {
-  int64_t splits = 1, rows = 0, items = 0;
+  int64_t splits = 1, items = 0;
   int64_t bytes = 0;
 };
 
 // Items that a launch of dq_attention_mass aims at, keys of one, and rows that are worth one.
-constexpr int64_t kMassItems = 2048, kMassKeys = 256, kMassRows = 256;
+constexpr int64_t kMassItems = 1536, kMassKeys = 256, kMassRows = 256;
 
 MassPlan plan_mass(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* q) {
   MassPlan p;
   const int64_t rows = std::min(s->max_q, s->tokens) * (q->heads / c->kv_heads);
   const int64_t items = s->batch * c->kv_heads * ceil_div(s->max_len, kMassKeys), keys = s->batch * c->kv_heads * s->max_len * 4;
-  if (items > 0 && rows > 0) {
-    p.splits = std::max<int64_t>(1, std::min({kMassItems / items, rows / kMassRows, kWorkspace / keys}));
-    p.rows = ceil_div(ceil_div(rows, p.splits), 64) * 64;
-    p.splits = ceil_div(rows, p.rows);
-  }
+  if (items > 0) p.splits = std::max<int64_t>(1, std::min({kMassItems / items, rows / kMassRows, kWorkspace / keys}));
   p.items = items * p.splits;
   if (p.splits > 1) p.bytes = p.splits * keys;
   return p;
@@ -332,7 +328,6 @@ int dq_attention_mass(const dq_kv_cache* cache, const dq_sequences* s, const dq_
   m.seq = seq_stride;
   m.head = head_stride;
   m.splits = (int32_t)p.splits;
-  m.rows = (int32_t)p.rows;
   if (p.splits > 1) m.part = static_cast<float*>(workspace);
   const hipError_t e = launch_attention_mass(q->dtype, cache->dtype, query_args(cache, s, q, scale), m, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? DQ_OK : hip_fail(e, "attention_mass launch");
