@@ -130,6 +130,21 @@ DQ_DEV bool nonfinite(u32 x) {
 
 DQ_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Eight values of q from value `at` on.
+template <int T>
+DQ_DEV void load8(const AttnArgs& a, int64_t at, v4u (&x)[T == DQ_F32 ? 2 : 1]) {
+  const char* p = static_cast<const char*>(a.q) + at * (T == DQ_F32 ? 4 : 2);
+  if (a.q_vec) {
+#pragma unroll
+    for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) x[k] = reinterpret_cast<const v4u*>(p)[k];
+  } else {
+#pragma unroll
+    for (int i = 0; i < (T == DQ_F32 ? 8 : 4); ++i)
+      x[i / 4][i % 4] = T == DQ_F32 ? reinterpret_cast<const u32*>(p)[i]
+                                    : (u32)reinterpret_cast<const uint16_t*>(p)[2 * i] | (u32)reinterpret_cast<const uint16_t*>(p)[2 * i + 1] << 16;
+  }
+}
+
 // The query fragments of rows: lane l has row l % 16 and, of every 32 values, 8 (l / 16) .. + 7. First their loads,
 // then, once other loads are under way too, the operands; the latter returns
 // the factor from products to scores in powers of two: fp32 rows are scaled to a largest value

@@ -442,7 +442,8 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
     to = max(to, s_high[w]);
   }
   int want = budget - min(a.first + a.last, len);  // it is the want-th largest of the numbers there
-  u32 least = ~0u;                                 // numbers above it or at it stay, but ties
+  u32 least = ~0u;                                 // numbers above it or at it stay; of those at it the first, where there are ties
+  bool ties = false;
   while (want > 0) {
     // (to - from + 1 numbers in bins of 2^shift)
     const int bits = 32 - __builtin_clz((to - from) | 1), shift = max(bits - kBinsLog2, 0);
@@ -482,21 +483,19 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
     const u32 start = from + ((u32)bin << shift);
     if (shift == 0 || some == want) {  // (a bin of one number; or all of it stays)
       least = start;
+      ties = some != want;
       break;
     }
     to = min(to, start + (1u << shift) - 1);
     from = start;
   }
   __syncthreads();
-  // the numbers above `least` stay, and of those at it the first ones (where its bin stays as a whole, all of them do)
-  int above = 0, equal = 0;
-  each([&](int, u32 x) {
-    above += __popcll(__ballot(x > least));
-    equal += __popcll(__ballot(x == least));
-  });
+  int mine = 0, tied = 0;
+  each([&](int, u32 x) { mine += __popcll(__ballot(x >= least)); });
+  if (ties) each([&](int, u32 x) { tied += __popcll(__ballot(x == least)); });
   if (lane == 0) {
-    s_above[wave] = above;
-    s_ties[wave] = equal;
+    s_above[wave] = mine - tied;
+    s_ties[wave] = tied;
   }
   __syncthreads();
   int all_above = 0, above_before = 0, ties_before = 0;
@@ -508,15 +507,18 @@ __global__ __launch_bounds__(kKeepWaves * 64) void k_keep(KeepArgs a) {
       ties_before += s_ties[w];
     }
   }
-  const int room = budget - all_above;  // for numbers at `least`
+  const int room = budget - all_above;  // for ties
   int left = max(room - ties_before, 0), at = above_before + min(ties_before, room);
+  const uint64_t lower = (1ull << lane) - 1;
   each([&](int i, u32 x) {
-    const uint64_t before = (1ull << lane) - 1, tie = __ballot(x == least);
-    const bool mine = x > least || (x == least && __popcll(tie & before) < left);
-    const uint64_t all = __ballot(mine);
-    if (mine) out[at + __popcll(all & before)] = (int)(base + i * 64 + lane);
-    at += __popcll(all);
-    left -= min(left, __popcll(tie));
+    uint64_t stays = __ballot(x >= least);
+    if (ties) {
+      const uint64_t tie = __ballot(x == least);
+      stays = __ballot(x > least || (x == least && __popcll(tie & lower) < left));
+      left -= min(left, __popcll(tie));
+    }
+    if (stays >> lane & 1) out[at + __popcll(stays & lower)] = (int)(base + i * 64 + lane);
+    at += __popcll(stays);
   });
 }
 

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   if (item >= items) return;
   const int hk = a.cache.kv_heads, page_tiles = (c.pages + 15) / 16;
-  const int h = (int)(item % hk), p0 = (int)(item / hk % page_tiles) * 16;
+  const int p0 = (int)(item % page_tiles) * 16, h = (int)(item / page_tiles % hk);  // (a workgroup's waves read the same rows)
   const int range = (int)(item / hk / page_tiles % ranges), b = (int)(item / hk / page_tiles / ranges);
   // the range's tokens, of the launch's (offsets, length and page numbers under way together)
   const int64_t lo = a.q_offsets != nullptr ? a.q_offsets[b] : b, hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
@@ -284,43 +284,42 @@ DQ_DEV double lanes_sum(double x, int log2) {
   return x;
 }
 
-// The 64-bit scores of row t's query heads on `count` pages id(j), as whole numbers that order as they do: most[j] (in LDS, 0 before) is the
-// largest over the heads. A wave's work, from its first pair of page and head on, every `step`th: 2^log2 lanes each, kPairs pairs'
-// loads under way together.
+// The 64-bit scores of row t's query heads on `count` pages id_of(j), as whole numbers that order as they do: most[j] (in LDS, 0 before)
+// is the largest over the heads. A wave's work: every `step`th, from its `first` on, of the steps of a page and 64 / 2^log2
+// of its heads; kSteps steps' loads are under way together.
 template <int T, int TC, class F>
 DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int count, F&& id_of, uint64_t* most, int first, int step, int log2,
                        int lane) {
-  constexpr int kPairs = 4;
-  const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), at_once = 64 >> log2;
+  constexpr int kSteps = 4;
+  const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), at_once = 64 >> log2, turns = (a.group + at_once - 1) / at_once;
   const bool in = d < a.dim;
-  const int pairs = count * a.group;
-  for (int i0 = first * at_once * kPairs; i0 < pairs; i0 += step * at_once * kPairs) {
-    v4u lo[kPairs], hi[kPairs];
-    float q[kPairs][8];
-    int page[kPairs];
-    bool bad[kPairs];
+  const int steps = count * turns;
+  for (int i0 = first * kSteps; i0 < steps; i0 += step * kSteps) {
+    v4u lo[kSteps], hi[kSteps], x[kSteps][T == DQ_F32 ? 2 : 1];
+    int page[kSteps];
+    bool bad[kSteps];
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) {
-      const int i = min(i0 + k * at_once + (lane >> log2), pairs - 1);  // (past the pairs: the last again)
-      page[k] = i / a.group;
+    for (int k = 0; k < kSteps; ++k) {
+      const int i = min(i0 + k, steps - 1);  // (past the steps: the last again)
+      page[k] = i / turns;
+      const int head = min((i - page[k] * turns) * at_once + (lane >> log2), a.group - 1);
       const int id = id_of(page[k]);
       bad[k] = (u32)id >= (u32)a.cache.n_pages;
       const uint16_t* near = c.bounds + ((int64_t)(bad[k] ? 0 : id) * a.cache.kv_heads + h) * 2 * a.dim + (in ? d : 0);
       lo[k] = *reinterpret_cast<const v4u*>(near);
       hi[k] = *reinterpret_cast<const v4u*>(near + a.dim);
-      const int64_t at = (int64_t)t * a.q_token + (int64_t)(h * a.group + i - page[k] * a.group) * a.q_head + d;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[k][e] = in ? load1<T>(a.q, at + e) : 0.f;
+      load8<T>(a, (int64_t)t * a.q_token + (int64_t)(h * a.group + head) * a.q_head + (in ? d : 0), x[k]);
     }
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) {
-      double s = 0;
+    for (int k = 0; k < kSteps; ++k) {
+      double s[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const u32 x = q[k][e] > 0 ? hi[k][e / 2] : lo[k][e / 2];
-        s = fma((double)q[k][e], (double)(e % 2 ? widen_hi<TC>(x) : widen<TC>(x)), s);
+        const float q = T == DQ_F32 ? as_f(x[k][e / 4 % (T == DQ_F32 ? 2 : 1)][e % 4]) : e % 2 ? widen_hi<T>(x[k][0][e / 2]) : widen<T>(x[k][0][e / 2]);
+        const u32 y = q > 0 ? hi[k][e / 2] : lo[k][e / 2];
+        s[e % 2] = fma((double)q, (double)(e % 2 ? widen_hi<TC>(y) : widen<TC>(y)), s[e % 2]);
       }
-      const uint64_t key = order_key(lanes_sum(in ? s : 0.0, log2));
+      const uint64_t key = order_key(lanes_sum(in ? s[0] + s[1] : 0.0, log2));
       if ((lane & (lanes - 1)) == 0) atomicMax((unsigned long long*)&most[page[k]], (unsigned long long)(bad[k] ? kNanKey : key));
     }
   }
@@ -361,6 +360,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     return;
   }
   const int32_t* list = a.pages + b * a.pages_stride;
+  int number[N];  // of the pages held
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) number[i] = list[min((w * N + i) * 64 + lane, pages - 1)];
+  }
   const int rounds = kHeld ? N : (pages + 64 * W - 1) / (64 * W), base = w * rounds * 64;
   auto interval = [&](int i, v2f x, u32& low, u32& high) {
     const int p = base + i * 64 + lane;
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     each([&](int i, u32 l, u32 u) {
       const bool mine = u >= floor && l <= ceiling;
       const uint64_t m = __ballot(mine);
-      if (mine) s_list[r][at + __popcll(m & ((1ull << lane) - 1))] = list[base + i * 64 + lane];
+      if (mine) s_list[r][at + __popcll(m & ((1ull << lane) - 1))] = kHeld ? number[kHeld ? i : 0] : list[base + i * 64 + lane];
       at += __popcll(m);
     });
     if constexpr (W > 1) __syncthreads();
@@ -595,7 +599,7 @@ DQ_DEV int to_front(int x, uint64_t mask, int lane) {
 }
 
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256) void k_page_attn(AttnArgs a, const int32_t* chosen, int64_t count, int splits, int chunk, int tiles) {
+__global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_page_attn(AttnArgs a, const int32_t* chosen, int64_t count, int splits, int chunk, int tiles) {
   constexpr int NP = kParts<T, TC>;
   constexpr int NC = DP / 16;
   __shared__ PageLds<DP> sh;
@@ -608,14 +612,18 @@ __global__ __launch_bounds__(256) void k_page_attn(AttnArgs a, const int32_t* ch
   const int tile0 = item % tiles * 16;
   item /= tiles;
   const int range = item % splits, t = item / splits;
+  const int rows = min(16, a.group - tile0);
+  const int64_t e0 = (int64_t)range * chunk, e1 = min(e0 + chunk, count);
+  const int32_t* list = chosen + ((int64_t)t * ca.kv_heads + head) * count;
+  // (the list, the queries and the sequence under way together)
+  int entry = e0 + lane < e1 ? list[e0 + lane] : -1;
+  RawQ<T, DP> raw;
+  load_q<T, DP>(a, n < rows, t, head * a.group + tile0 + min(n, rows - 1), g, raw);
   const int b = find_seq(a, t, lane);
   if (b < 0) return;
   if (threadIdx.x == 0) sh.bad = 0;
   __syncthreads();
-  const int rows = min(16, a.group - tile0);
   const int sees = row_sees(a, b, t, seq_len(a, b));
-  RawQ<T, DP> raw;
-  load_q<T, DP>(a, n < rows, t, head * a.group + tile0 + min(n, rows - 1), g, raw);
   v4u q[NP][DP / 32];
   const float c = q_operands<T, TC, DP>(a, raw, q);
 
@@ -639,11 +647,9 @@ __global__ __launch_bounds__(256) void k_page_attn(AttnArgs a, const int32_t* ch
 
   const int units = ca.page_size / 16;  // of 16 keys, of a page
   const int skip = 8 / units, skip_rest = 8 % units;
-  const int64_t e0 = (int64_t)range * chunk, e1 = min(e0 + chunk, count);
-  const int32_t* list = chosen + ((int64_t)t * ca.kv_heads + head) * count;
   for (int64_t eb = e0; eb < e1; eb += 64) {
     // the next 64 entries, a lane each; those that hold visible keys to the front
-    int entry = eb + lane < e1 ? list[eb + lane] : -1;
+    if (eb > e0) entry = eb + lane < e1 ? list[eb + lane] : -1;
     const bool some = entry >= 0 && (int64_t)entry * ca.page_size < sees;
     int id = some ? a.pages[b * a.pages_stride + entry] : 0;
     if ((u32)id >= (u32)ca.n_pages) {
