@@ -15,6 +15,9 @@ DQ_DEV int row_sees(const AttnArgs& a, int b, int t, int len) {
   return (int)(n < 0 ? 0 : n < len ? n : len);
 }
 
+// Pages that hold a number of keys.
+DQ_DEV int pages_of(int keys, int page_size) { return keys > 0 ? (keys - 1) / page_size + 1 : 0; }
+
 // ---- bounds of a page -------------------------------------------------------
 // A wave takes a page of a kv head: a lane 8 channels of every 64 / lanes'th key. 16-bit floats are compared as
 // whole numbers of their order (negative ones with their other bits turned round), two at a time; NaN lies
@@ -149,8 +152,12 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   const int range = (int)(item / hk / page_tiles % ranges), b = (int)(item / hk / page_tiles / ranges);
   // the range's tokens, of the launch's (offsets, length and page numbers under way together)
   const int64_t lo = a.q_offsets != nullptr ? a.q_offsets[b] : b, hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
-  const int listed = a.pages[b * a.pages_stride + min(p0 + n, c.pages - 1)];
-  const int pages = (seq_len(a, b) + a.cache.page_size - 1) / a.cache.page_size;
+  // (the last sequence's list may end with its keys)
+  const int32_t* list = a.pages + b * a.pages_stride;
+  int listed = 0;
+  if (b + 1 < a.batch) listed = list[min(p0 + n, c.pages - 1)];
+  const int pages = pages_of(seq_len(a, b), a.cache.page_size);
+  if (b + 1 == a.batch && p0 + n < pages) listed = list[p0 + n];
   const int64_t end = min(min(hi, (int64_t)a.tokens), (int64_t)token0 + c.tokens);
   const int64_t first = max(lo, (int64_t)token0) + (int64_t)range * range_tokens, last = min(first + range_tokens, end);
   if (p0 >= pages || first >= last) return;
@@ -351,7 +358,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
   }
   const int b = find_seq(a, t, lane);
   if (b < 0) return;
-  const int pages = (row_sees(a, b, t, seq_len(a, b)) + a.cache.page_size - 1) / a.cache.page_size;
+  const int pages = pages_of(row_sees(a, b, t, seq_len(a, b)), a.cache.page_size);
   int32_t* out = c.chosen + ((int64_t)t * hk + h) * c.count;
   const int count = (int)min(c.count, (int64_t)pages), tid = w * 64 + lane;
   for (int64_t i = count + tid; i < c.count; i += 64 * W) out[i] = -1;
@@ -652,7 +659,7 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
     if (eb > e0) entry = eb + lane < e1 ? list[eb + lane] : -1;
     const bool some = entry >= 0 && (int64_t)entry * ca.page_size < sees;
     int id = some ? a.pages[b * a.pages_stride + entry] : 0;
-    if ((u32)id >= (u32)ca.n_pages) {
+    if (some && (u32)id >= (u32)ca.n_pages) {
       bad = true;
       id = 0;
     }

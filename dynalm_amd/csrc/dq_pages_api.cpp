@@ -132,7 +132,7 @@ AttnArgs query_args(const dq_kv_cache* c, const dq_sequences* s, const dq_heads*
 // Tokens whose scores a launch of dq_choose_pages writes (0: one's are too many).
 int64_t choose_tokens(const dq_kv_cache* c, const dq_sequences* s, bool scores) {
   const int64_t pages = ceil_div(s->max_len, c->page_size);
-  int64_t n = kMaxGroups / 4 / c->kv_heads;  // (a workgroup of 1,024 threads a row at most)
+  int64_t n = (kMaxGroups / 4 - 1) / c->kv_heads;  // (a workgroup of 1,024 threads a row at most)
   if (scores) n = std::min(n, kWorkspace / 8 / pages / c->kv_heads);
   return std::min(n, s->tokens);
 }
@@ -158,7 +158,7 @@ constexpr int64_t kPageItems = 512, kPageKeys = 256;
 PagePlan plan_pages(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* q, int64_t count) {
   PagePlan p;
   const int64_t group = q->heads / c->kv_heads, rows = s->tokens * c->kv_heads * ceil_div(group, 16);
-  const int64_t keys = std::min(count, ceil_div(s->max_len, c->page_size)) * c->page_size;
+  const int64_t keys = std::min(std::min(count, ceil_div(s->max_len, c->page_size)) * c->page_size, s->max_len);
   if (rows > 0) p.splits = std::max<int64_t>(1, std::min(kPageItems / rows, keys / kPageKeys));
   p.chunk = std::max<int64_t>(1, ceil_div(count, p.splits));
   p.splits = std::max<int64_t>(1, ceil_div(count, p.chunk));
@@ -253,6 +253,7 @@ int dq_choose_pages(const dq_kv_cache* cache, const dq_sequences* s, const dq_he
   c.last = (int32_t)last;
   c.count = count;
   c.tokens = choose_tokens(cache, s, scores);
+  if (c.tokens == 0) return too_many("heads");
   if (scores) {
     if (bounds == nullptr) return bad("bounds: null argument");
     if (reinterpret_cast<uintptr_t>(bounds) % 16 != 0) return bad("bounds: must be 16-byte aligned");

@@ -611,7 +611,7 @@ DQ_API int dq_choose_pages(const dq_kv_cache* cache, const dq_sequences* s, cons
 /* dq_shared_attention's rows over the keys of chosen pages alone:
  *     out[t, h] = sum_j p_j v_j,  p = softmax over the visible j on a chosen page of scale * q[t, h] . k_j
  * chosen is dq_choose_pages' list, or any other of that form: tokens x kv_heads x count indices into a sequence's pages, in any
- * order; entries outside the pages that hold visible keys are left out, a page that is given twice counts twice. Types, rounding, lse, infinite and NaN
+ * order; entries outside the pages that hold visible keys are left out, a page that is given twice counts twice. out must not overlap q. Types, rounding, lse, infinite and NaN
  * values, rows without keys and page numbers outside the cache (of a chosen page) are as there.
  * workspace: dq_page_attention_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
 DQ_API int64_t dq_page_attention_workspace(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, int64_t count);
@@ -644,7 +644,7 @@ DQ_API int dq_kv_keep(const dq_sequences* s, int64_t kv_heads, const float* mass
 /* Moves the keys and values of places kept[b][g][i] of sequence b to places i, in each kv head by itself, of the pages
  * to_pages[b * to_stride], ... (NULL: of the sequence's own, in place; then kept must ascend, as dq_kv_keep's does). Entries
  * outside [0, lens[b]) and pages outside the cache are left out. With mass and mass_out (both or neither), mass_out[b][g][i] is
- * mass[b][g][kept[b][g][i]] too, at the same strides; mass_out may be mass. Pages that are written to must be of one sequence and
+ * mass[b][g][kept[b][g][i]] too, at the same strides; mass_out may be mass, and must not overlap it otherwise. Pages that are written to must be of one sequence and
  * (to_pages) be read by none. Keys have been rotated to their positions when they were appended: those that stay keep them. */
 DQ_API int dq_kv_compact(const dq_kv_cache* cache, const dq_sequences* s, const int32_t* kept, int64_t budget,
                          const int32_t* to_pages, int64_t to_stride, const float* mass, float* mass_out, int64_t seq_stride,

@@ -714,3 +714,68 @@ def test_offsets_and_lengths_of_any_values_stay_inside(cuda):
         for x, value, n in ((wide, 55.0, 10), (lse, 33.0, 10), (lists, 77, 10), (mass, 33.0, 1), (bounds, 44.0, 1)):
             assert torch.all(x[:n] == value) and torch.all(x[-n:] == value)
         assert torch.all(mass[..., 44:] == 33.0)
+
+
+@pytest.mark.parametrize("count", [1, 3])
+def test_no_keys_at_all(cuda, count):
+    """max_len 0 and a cache without pages: no page is chosen, rows are zeros, nothing is kept."""
+    cache = dq.KvCache(None, None, dq.F16, 2, 64, 16, 0, 0, 64, 64)
+    s = dq.Sequences(3, 3, None, 1, None, 0, None, 0)
+    q, out = torch.randn((3, 4, 64), device="cuda"), torch.full((3, 4, 64), 55.0, device="cuda")
+    lse, chosen = torch.full((3, 4), 33.0, device="cuda"), torch.full((3, 2, count), 77, dtype=torch.int32, device="cuda")
+    kept, kept_lens = torch.full((3, 2, 5), 77, dtype=torch.int32, device="cuda"), torch.full((3,), 77, dtype=torch.int32, device="cuda")
+    dq.page_bounds(cache, s, None, 0, None, stream())
+    dq.choose_pages(cache, s, B.heads(q), None, 0, 1, count, chosen, None, 0, stream())
+    dq.page_attention(cache, s, B.heads(q), B.heads(out), lse, chosen, count, 0.1, None, 0, stream())
+    dq.attention_mass(cache, s, B.heads(q), lse, 0.1, 0.5, None, 0, 0, None, 0, stream())
+    dq.kv_keep(s, 2, None, 0, 0, 1, 1, 5, kept, kept_lens, stream())
+    dq.kv_compact(cache, s, kept, 5, stream=stream())
+    assert torch.all(chosen == -1) and torch.all(out == 0) and torch.all(lse == -math.inf)
+    assert torch.all(kept == -1) and torch.all(kept_lens == 0)
+
+
+def test_a_list_that_ends_with_the_last_sequence(cuda):
+    """Of the last sequence only the page numbers that hold keys need exist: what lies behind the list changes nothing."""
+    c = Call(71, [1, 1], [900, 200], 4, 2, 64, "f16", "f16", 16)
+    stride = c.table.stride(0)
+    flat = torch.full((stride + 13 + 64,), 2**31 - 1, dtype=torch.int32, device="cuda")
+    flat[: stride + 13] = c.table.reshape(-1)[: stride + 13]
+    c.table = flat.as_strided((2, 13), (stride, 1))
+    bounds = L.run_bounds(c)
+    chosen = L.run_choose(c, bounds, 1, 1, 6)
+    flat[stride + 13 :] = 0
+    again = L.run_choose(c, bounds, 1, 1, 6)
+    first = Call(71, [1, 1], [900, 200], 4, 2, 64, "f16", "f16", 16)
+    assert torch.equal(chosen, again) and torch.equal(chosen.cpu(), L.choose(first, bounds, 1, 1, 6))
+
+
+def test_decay_of_sequences_without_rows(cuda):
+    """No rows at all: every key's weight decays."""
+    c = Call(72, [0, 0], [50, 20], 2, 1, 64, "f32", "f16", 16)
+    old = torch.rand((2, 1, 50), device="cuda")
+    s = dq.Sequences(2, 0, c.offsets_d.data_ptr(), 1, c.table.data_ptr(), c.table.stride(0), c.lens_d.data_ptr(), 50)
+    got = old.clone()
+    q = dq.Heads(None, dq.F32, 2, 128, 64)
+    dq.attention_mass(c.c(), s, q, None, 0.1, 0.5, got, 50, 50, None, 0, stream())
+    want = old.clone()
+    want[0] *= 0.5
+    want[1, :, :20] *= 0.5
+    assert torch.equal(got, want)
+
+
+def test_pages_of_more_keys_than_any_sequence(cuda):
+    """One page holds all: a page size near 2^31, of which a few places exist, is counted without overflow."""
+    hk, dim, n = 1, 64, 40
+    c = Call(73, [1, 2], [n, 33], 2, hk, dim, "f32", "f16", 48)
+    cache = dq.KvCache(c.kc.data_ptr(), c.vc.data_ptr(), dq.F16, hk, dim, 2**31 - 16, c.kc.shape[0], c.kc.stride(0), c.kc.stride(1), c.kc.stride(2))
+    s = c.seqs()
+    bounds = torch.zeros((c.kc.shape[0], hk, 2, dim), dtype=torch.float16, device="cuda")
+    dq.page_bounds(cache, s, None, 0, bounds, stream())
+    L.same(bounds, L.page_bounds(c, None, torch.zeros_like(bounds).cpu()))
+    chosen = torch.full((3, hk, 2), 77, dtype=torch.int32, device="cuda")
+    dq.choose_pages(cache, s, B.heads(c.q), bounds, 0, 1, 2, chosen, None, 0, stream())
+    assert chosen.tolist() == [[[0, -1]]] * 3
+    out = torch.empty_like(c.q)
+    dq.page_attention(cache, s, B.heads(c.q), B.heads(out), None, chosen, 2, c.scale, None, 0, stream())
+    want, _, bound, _ = L.page_attention(c, chosen)
+    B.close(out, want, bound, "f32")
