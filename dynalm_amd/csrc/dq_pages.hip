@@ -598,11 +598,12 @@ struct PageKv {
   u32 v[8][DP / 32];
 };
 
-// Moves x of the lanes in `mask` to lanes 0, 1, ... in turn.
-DQ_DEV int to_front(int x, uint64_t mask, int lane) {
-  const uint64_t before = (1ull << lane) - 1;
-  const int to = mask >> lane & 1 ? __popcll(mask & before) : __popcll(mask) + __popcll(~mask & before);
-  return __builtin_amdgcn_ds_permute(4 * to, x);
+// Where the lane goes if those of `first`, then those of `second`, then the others are lined up.
+DQ_DEV int front_place(uint64_t first, uint64_t second, int lane) {
+  const uint64_t lower = (1ull << lane) - 1;
+  if (first >> lane & 1) return __popcll(first & lower);
+  if (second >> lane & 1) return __popcll(first) + __popcll(second & lower);
+  return __popcll(first | second) + __popcll(~(first | second) & lower);
 }
 
 template <int T, int TC, int DP>
@@ -663,10 +664,14 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
       bad = true;
       id = 0;
     }
-    const uint64_t mask = __ballot(some);
-    entry = to_front(entry, mask, lane);
-    id = to_front(id, mask, lane);
-    const int halves = __popcll(mask) * units;  // of tiles: runs of 16 keys
+    // (the page of the last visible key, which may hold few, at the end of them)
+    const int seen = some ? min((sees - entry * ca.page_size + 15) / 16, units) : 0;  // 16s of keys
+    const uint64_t full = __ballot(seen == units), part = __ballot(some && seen < units);
+    const int left = units - (part != 0 ? __builtin_amdgcn_readlane(seen, 63 - __builtin_clzll(part)) : units);
+    const int to = front_place(full, part, lane);
+    entry = __builtin_amdgcn_ds_permute(4 * to, entry);
+    id = __builtin_amdgcn_ds_permute(4 * to, id);
+    const int halves = __popcll(full | part) * units - left;  // of tiles: runs of 16 keys
     int e = 2 * wave / units, sub = 2 * wave % units;
     for (int half = 2 * wave; half < halves; half += 8) {
       PageKv<DP> r;

@@ -172,6 +172,7 @@ int check_page_attention(const dq_kv_cache* c, const dq_sequences* s, const dq_h
   if (int rc = check_token_stride(c); rc != DQ_OK) return rc;
   if (int rc = check_sequences(s, c->page_size); rc != DQ_OK) return rc;
   if (int rc = check_queries(c, s, q, data); rc != DQ_OK) return rc;
+  if (c->page_size > (1 << 24)) return set_error(DQ_UNSUPPORTED, "cache: page_size %d", c->page_size);  // (64 pages' keys are counted in 32 bits)
   if (count < 1 || count > kMostKeys) return set_error(DQ_INVALID_ARGUMENT, "count %lld", (ll)count);
   if (plan_pages(c, s, q, count).items >= kMaxGroups) return too_many("rows");
   return DQ_OK;

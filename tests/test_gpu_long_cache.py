@@ -763,19 +763,24 @@ def test_decay_of_sequences_without_rows(cuda):
     assert torch.equal(got, want)
 
 
-def test_pages_of_more_keys_than_any_sequence(cuda):
-    """One page holds all: a page size near 2^31, of which a few places exist, is counted without overflow."""
-    hk, dim, n = 1, 64, 40
-    c = Call(73, [1, 2], [n, 33], 2, hk, dim, "f32", "f16", 48)
-    cache = dq.KvCache(c.kc.data_ptr(), c.vc.data_ptr(), dq.F16, hk, dim, 2**31 - 16, c.kc.shape[0], c.kc.stride(0), c.kc.stride(1), c.kc.stride(2))
-    s = c.seqs()
-    bounds = torch.zeros((c.kc.shape[0], hk, 2, dim), dtype=torch.float16, device="cuda")
-    dq.page_bounds(cache, s, None, 0, bounds, stream())
-    L.same(bounds, L.page_bounds(c, None, torch.zeros_like(bounds).cpu()))
-    chosen = torch.full((3, hk, 2), 77, dtype=torch.int32, device="cuda")
-    dq.choose_pages(cache, s, B.heads(c.q), bounds, 0, 1, 2, chosen, None, 0, stream())
-    assert chosen.tolist() == [[[0, -1]]] * 3
-    out = torch.empty_like(c.q)
-    dq.page_attention(cache, s, B.heads(c.q), B.heads(out), None, chosen, 2, c.scale, None, 0, stream())
-    want, _, bound, _ = L.page_attention(c, chosen)
-    B.close(out, want, bound, "f32")
+@pytest.mark.parametrize("type,cache", KINDS)
+def test_pages_of_more_keys_than_any_sequence(cuda, type, cache):
+    """A page holds a sequence's whole cache, most of it never written."""
+    hk, dim, page = 2, 64, 1 << 16
+    c = Call(73, [1, 2, 1], [40, 33, 700], 4, hk, dim, type, cache, page)
+    assert c.kc.shape[0] == 4 and c.pages == 1
+    bounds = L.run_bounds(c)
+    L.same(bounds, L.page_bounds(c, None, torch.full_like(bounds, 55.0).cpu()))
+    chosen = L.run_choose(c, bounds, 0, 1, 2)
+    assert chosen.tolist() == [[[0, -1]] * hk] * 4
+    L.check_attention(c, chosen)
+    L.check_attention(c, torch.tensor([0, -1, 0, 5], dtype=torch.int32).repeat(4, hk, 1))
+    lse = own_lse(c)
+    got = L.run_mass(c, lse, torch.zeros((3, hk, 700), device="cuda"), 0.0)
+    want, bound = L.mass(c, lse, torch.zeros((3, hk, 700)), 0.0)
+    B.close(got, want, bound, "f32")
+    kept = lists(c, 30)
+    dq.kv_compact(c.c(), c.seqs(), kept.cuda(), 30, stream=stream())
+    for b in range(3):
+        for h in range(hk):
+            assert torch.equal(c.kc[int(c.table[b, 0]), :30, h].cpu(), c.ks[b][kept[b, h].long(), h])

@@ -105,6 +105,7 @@ def test_attend_refusals():
         refused(BAD, attend, **kw)
     refused(NO, attend, out=heads(dtype=dq.F16))
     refused(NO, attend, c=cache(token_stride=1 << 26))
+    refused(NO, attend, c=cache(page_size=(1 << 24) + 16, page_stride=1 << 31))
     refused(NO, attend, s=seqs(tokens=1 << 29, batch=1 << 29))
     refused(NO, attend, s=seqs(tokens=1 << 24, batch=1 << 24), q=heads(heads=2), out=heads(heads=2))
     many = {"s": seqs(max_len=3000, pages_stride=200), "count": 100}
