@@ -538,13 +538,14 @@ DQ_DEV void reads_done() {
   __syncthreads();
 }
 
+template <int kThreads>
 DQ_DEV void move_weights(const int32_t* kept, int64_t count, int len, const float* mass, float* out) {
-  for (int64_t i0 = 0; i0 < count; i0 += 256 * kMoveLoads) {
+  for (int64_t i0 = 0; i0 < count; i0 += kThreads * kMoveLoads) {
     float w[kMoveLoads];
     bool moves[kMoveLoads];
 #pragma unroll
     for (int u = 0; u < kMoveLoads; ++u) {
-      const int64_t i = i0 + u * 256 + threadIdx.x;
+      const int64_t i = i0 + u * kThreads + threadIdx.x;
       const int place = i < count ? kept[i] : -1;
       moves[u] = place >= 0 && place < len;
       w[u] = moves[u] ? mass[place] : 0.f;
@@ -552,12 +553,12 @@ DQ_DEV void move_weights(const int32_t* kept, int64_t count, int len, const floa
     reads_done();
 #pragma unroll
     for (int u = 0; u < kMoveLoads; ++u)
-      if (moves[u]) out[i0 + u * 256 + threadIdx.x] = w[u];
+      if (moves[u]) out[i0 + u * kThreads + threadIdx.x] = w[u];
   }
 }
 
-template <bool kInPlace>
-__global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int lanes_log2, int runs) {
+template <bool kInPlace, int kThreads>
+__global__ __launch_bounds__(kThreads) void k_compact(AttnArgs a, CompactArgs c, int lanes_log2, int runs) {
   constexpr int kEntries = kInPlace ? kMoveEntries : 0;
   __shared__ v4i s_move[kInPlace ? kEntries : 1];  // of an entry: page and place that it comes from (page -1: none), that it goes to
   const CacheArgs& ca = a.cache;
@@ -571,14 +572,15 @@ __global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int 
   const int most = (int)min(c.budget, (int64_t)len);  // (entries behind are none of kv_keep's)
   if (c.mass != nullptr && job == jobs - 1) {
     const int64_t at = b * c.seq + h * c.head;
-    move_weights(kept, most, len, c.mass + at, c.mass_out + at);
+    move_weights<kThreads>(kept, most, len, c.mass + at, c.mass_out + at);
     return;
   }
   const int32_t* from = a.pages + b * a.pages_stride;
   const int32_t* to = kInPlace ? from : c.to_pages + b * c.to_stride;
   uint16_t* pool = (job & 1 ? ca.v : ca.k) + h * ca.head;
-  const int rows = 256 >> lanes_log2, r = threadIdx.x >> lanes_log2, d = 8 * (threadIdx.x & ((1 << lanes_log2) - 1));
-  const int run_rows = rows * kMoveLoads;
+  const int rows = kThreads >> lanes_log2, r = threadIdx.x >> lanes_log2, d = 8 * (threadIdx.x & ((1 << lanes_log2) - 1));
+  constexpr int kLoads = kMoveLoads;
+  const int run_rows = rows * kLoads;
   auto move_of = [&](int i) {
     v4i e = {-1, 0, 0, 0};
     const int place = i < most ? kept[i] : -1;
@@ -593,38 +595,38 @@ __global__ __launch_bounds__(256) void k_compact(AttnArgs a, CompactArgs c, int 
   auto target = [&](v4i e) { return reinterpret_cast<v4u*>(pool + e[2] * ca.page + e[3] * ca.token + d); };
   if constexpr (!kInPlace) {
     const int i0 = (job >> 1) * run_rows;
-    v4i e[kMoveLoads];
-    v4u x[kMoveLoads];
+    v4i e[kLoads];
+    v4u x[kLoads];
 #pragma unroll
-    for (int u = 0; u < kMoveLoads; ++u) e[u] = move_of(i0 + u * rows + r);
+    for (int u = 0; u < kLoads; ++u) e[u] = move_of(i0 + u * rows + r);
 #pragma unroll
-    for (int u = 0; u < kMoveLoads; ++u)
+    for (int u = 0; u < kLoads; ++u)
       if (in && e[u][0] >= 0) x[u] = *source(e[u]);
 #pragma unroll
-    for (int u = 0; u < kMoveLoads; ++u)
+    for (int u = 0; u < kLoads; ++u)
       if (in && e[u][0] >= 0) *target(e[u]) = x[u];
   } else {
     for (int c0 = 0; c0 < most; c0 += kEntries) {
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < kEntries / 256; ++u) s_move[u * 256 + threadIdx.x] = move_of(c0 + u * 256 + threadIdx.x);
+      for (int u = 0; u < kEntries / kThreads; ++u) s_move[u * kThreads + threadIdx.x] = move_of(c0 + u * kThreads + threadIdx.x);
       __syncthreads();
       const int end = min(kEntries, most - c0);
-      v4u x[2][kMoveLoads];
-      auto read = [&](int i0, v4u (&y)[kMoveLoads]) {
+      v4u x[2][kLoads];
+      auto read = [&](int i0, v4u (&y)[kLoads]) {
 #pragma unroll
-        for (int u = 0; u < kMoveLoads; ++u) {
+        for (int u = 0; u < kLoads; ++u) {
           const v4i e = s_move[min(i0 + u * rows + r, kEntries - 1)];
           if (in && i0 + u * rows + r < end && e[0] >= 0) y[u] = *source(e);
         }
       };
-      auto write = [&](int i0, v4u (&y)[kMoveLoads]) {
+      auto write = [&](int i0, v4u (&y)[kLoads]) {
         // (the run's reads have come, of all waves; those of the next one may be under way)
 #pragma unroll
-        for (int u = 0; u < kMoveLoads; ++u) asm volatile("" : "+v"(y[u]) : : "memory");
+        for (int u = 0; u < kLoads; ++u) asm volatile("" : "+v"(y[u]) : : "memory");
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kMoveLoads; ++u) {
+        for (int u = 0; u < kLoads; ++u) {
           const v4i e = s_move[min(i0 + u * rows + r, kEntries - 1)];
           if (in && i0 + u * rows + r < end && e[0] >= 0) *target(e) = y[u];
         }
@@ -686,6 +688,9 @@ hipError_t launch_kv_keep(int64_t batch, const KeepArgs& k, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Sequences and heads below which a workgroup of a move in place has 512 threads. XXX
+constexpr int64_t kFewMoves = 128;
+
 hipError_t launch_kv_compact(const AttnArgs& a, const CompactArgs& c, hipStream_t s) {
   int log2 = 0;
   while ((8 << log2) < a.dim) ++log2;
@@ -694,10 +699,12 @@ hipError_t launch_kv_compact(const AttnArgs& a, const CompactArgs& c, hipStream_
   const bool in_place = c.to_pages == nullptr;
   const int64_t jobs = 2 * (in_place ? 1 : runs) + (c.mass != nullptr);
   const dim3 grid((uint32_t)(jobs * a.batch * a.cache.kv_heads));
-  if (in_place)
-    hipLaunchKernelGGL((k_compact<true>), grid, dim3(256), 0, s, a, c, log2, runs);
+  if (!in_place)
+    hipLaunchKernelGGL((k_compact<false, 256>), grid, dim3(256), 0, s, a, c, log2, runs);
+  else if (a.batch * a.cache.kv_heads < kFewMoves)
+    hipLaunchKernelGGL((k_compact<true, 512>), grid, dim3(512), 0, s, a, c, log2, runs);
   else
-    hipLaunchKernelGGL((k_compact<false>), grid, dim3(256), 0, s, a, c, log2, runs);
+    hipLaunchKernelGGL((k_compact<true, 256>), grid, dim3(256), 0, s, a, c, log2, runs);
   return hipGetLastError();
 }
 

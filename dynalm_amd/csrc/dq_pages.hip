@@ -131,19 +131,117 @@ DQ_DEV float pair_max32(float x) {
 template <int T>
 constexpr int kScoreParts = T == DQ_F32 ? 2 : 1;
 
-// What S may be off by, of A: a rounding (or a cut) of each of the 2 dim sums and of those of the parts, an fp32 q's third part,
-// A's own error, the interval's ends.
+// What S may be off by, of A: a rounding (or a cut) of each of the 2 dim sums, A's own error, the interval's ends; with an fp32 q
+// the sums of its second part, which are 2^-8 (f16: 2^-11) as large, and what two parts leave out of a value: 2^-18 (f16: 2^-22) of it.
 template <int T, int TC>
 DQ_DEV float score_error(int dim) {
-  return (2 * kScoreParts<T> * dim + 64) * 0x1p-23f + (T != DQ_F32 ? 0.f : TC == DQ_F16 ? 0x1p-20f : 0x1p-16f);
+  return (2 * dim + 64) * (T == DQ_F32 ? 0x1.04p-23f : 0x1p-23f) + (T != DQ_F32 ? 0.f : TC == DQ_F16 ? 0x1p-21f : 0x1p-17f);
+}
+
+// The bounds of 16 pages as B operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values.
+template <int DP>
+struct PageTile {
+  v4u lo[DP / 32], hi[DP / 32];
+  bool bad;
+};
+template <int DP>
+DQ_DEV void load_page_tile(const AttnArgs& a, const ChooseArgs& c, int h, int id, int g, PageTile<DP>& p) {
+  p.bad = (u32)id >= (u32)a.cache.n_pages;
+  const uint16_t* near = c.bounds + ((int64_t)(p.bad ? 0 : id) * a.cache.kv_heads + h) * 2 * a.dim;
+#pragma unroll
+  for (int s = 0; s < DP / 32; ++s) {
+    const int d = 32 * s + 8 * g;
+    p.lo[s] = d < a.dim ? *reinterpret_cast<const v4u*>(near + d) : v4u{0, 0, 0, 0};
+    p.hi[s] = d < a.dim ? *reinterpret_cast<const v4u*>(near + a.dim + d) : v4u{0, 0, 0, 0};
+  }
+}
+// The larger magnitudes of the bounds.
+template <int DP>
+DQ_DEV void magnitudes(const PageTile<DP>& p, v4u (&most)[DP / 32]) {
+#pragma unroll
+  for (int s = 0; s < DP / 32; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const v2us u = __builtin_bit_cast(v2us, p.lo[s][e] & 0x7FFF7FFFu), v = __builtin_bit_cast(v2us, p.hi[s][e] & 0x7FFF7FFFu);
+      most[s][e] = __builtin_bit_cast(u32, __builtin_elementwise_max(u, v));
+    }
+}
+
+// The intervals of the lane's page with rows 4 g .. + 3 of 16 query rows, where they pass low and high. next() is called once
+// the rows are no longer needed.
+template <int T, int TC, int DP, class F>
+DQ_DEV void tile_scores(const RawQ<T, DP>& raw, const PageTile<DP>& page, const v4u (&most)[DP / 32], float error, int g, float (&low)[4],
+                        float (&high)[4], F&& next) {
+  constexpr int NS = DP / 32, NP = kScoreParts<T>;
+  int e2 = 0;
+  if constexpr (T == DQ_F32 && TC == DQ_F16) {  // scaled to a largest value in [2^14, 2^15)
+    float top = 0;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(as_f(raw.x[s][i / 4][i % 4])));
+    top = row_max(top);
+    e2 = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+  }
+  v4f sums[NP], size = {0, 0, 0, 0};
+#pragma unroll
+  for (int p = 0; p < NP; ++p) sums[p] = v4f{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    v4u part[NP], down, mag;  // down: the halves of values that are not above 0
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (T == DQ_F32) {
+        const float y0 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2]), e2), y1 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2 + 1]), e2);
+        u32 p = pack<TC>(y0, y1);
+        part[0][e] = p;
+        part[1][e] = pack<TC>(y0 - widen<TC>(p), y1 - widen_hi<TC>(p));
+        down[e] = (y0 > 0 ? 0u : 0xFFFFu) | (y1 > 0 ? 0u : 0xFFFF0000u);
+        // (what the parts leave out is less than 2^-17 (f16: 2^-21) of the value, or of the least magnitude that counts here)
+        constexpr float kLeast = TC == DQ_F16 ? 0x1p-4f : 0x1p-100f;
+        mag[e] = pack<TC>(y0 != y0 ? y0 : fmaxf(fabsf(y0), kLeast), y1 != y1 ? y1 : fmaxf(fabsf(y1), kLeast));
+      } else {
+        const u32 y = raw.x[s][0][e];
+        part[0][e] = y;
+        down[e] = __builtin_bit_cast(u32, __builtin_bit_cast(v2s, y) >> 15);
+        mag[e] = y & 0x7FFF7FFFu;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      sums[p] = mma<TC>(part[p] & ~down, page.hi[s], sums[p]);
+      sums[p] = mma<TC>(part[p] & down, page.lo[s], sums[p]);
+    }
+    size = mma<TC>(mag, most[s], size);
+  }
+  next();
+  const v4f sum = NP == 1 ? sums[0] : sums[0] + sums[NP - 1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float d = fmaf(error, size[i], 0x1p-118f);
+    const bool fine = d < INFINITY && fabsf(sum[i]) < INFINITY && !page.bad;
+    const int back = T == DQ_F32 && TC == DQ_F16 ? -__shfl(e2, 4 * g + i, 64) : 0;
+    low[i] = fmaxf(low[i], fine ? ldexpf(sum[i] - d, back) : -INFINITY);
+    high[i] = fmaxf(high[i], fine ? ldexpf(sum[i] + d, back) : INFINITY);
+  }
+}
+
+// The largest over a token's `lanes` rows: of a lane's, then of two or all four lane groups.
+DQ_DEV void token_max(float (&x)[4], int lanes) {
+  if (lanes > 1) {
+    x[0] = fmaxf(x[0], x[1]);
+    x[2] = fmaxf(x[2], x[3]);
+  }
+  if (lanes > 2) x[0] = fmaxf(x[0], x[2]);
+  if (lanes > 4) x[0] = pair_max16(x[0]);
+  if (lanes > 8) x[0] = pair_max32(x[0]);
 }
 
 // A wave takes 16 pages of a kv head, whose bounds it holds, and of a sequence's rows a range, 16 at a time: `slots` tokens
-// of `lanes` lanes, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
+// of `lanes` rows, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
 template <int T, int TC, int DP>
 __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int lanes, int ranges, int range_tokens,
                                                      int64_t items) {
-  constexpr int NS = DP / 32, NP = kScoreParts<T>;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   if (item >= items) return;
@@ -163,108 +261,29 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   if (p0 >= pages || first >= last) return;
   const int slots = 16 / lanes, slot = n / lanes, blocks = (a.group + 15) / 16;
   RawQ<T, DP> raw;
-  auto read_q = [&](int64_t t0, int block) {  // (a lane past the heads takes the last again)
+  auto read_q = [&](int64_t t0, int block) {  // (a row past the heads is the last again)
     load_q<T, DP>(a, true, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + n % lanes, a.group - 1), g, raw);
   };
   read_q(first, 0);
-
-  // the bounds as B operands: lane n of a group has page n, 8 (lane / 16) .. + 7 of every 32 values
-  const int id = p0 + n < pages ? listed : 0;
-  const bool bad = (u32)id >= (u32)a.cache.n_pages;
-  const uint16_t* near = c.bounds + ((int64_t)(bad ? 0 : id) * hk + h) * 2 * a.dim;
-  v4u x[2][NS], most[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int d = 32 * s + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) x[i][s] = d < a.dim ? *reinterpret_cast<const v4u*>(near + i * a.dim + d) : v4u{0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const v2us u = __builtin_bit_cast(v2us, x[0][s][e] & 0x7FFF7FFFu), v = __builtin_bit_cast(v2us, x[1][s][e] & 0x7FFF7FFFu);
-      most[s][e] = __builtin_bit_cast(u32, __builtin_elementwise_max(u, v));
-    }
+  PageTile<DP> page;
+  load_page_tile<DP>(a, c, h, p0 + n < pages ? listed : 0, g, page);
+  v4u most[DP / 32];
+  magnitudes<DP>(page, most);
   const float error = score_error<T, TC>(a.dim);
   for (int64_t t0 = first; t0 < last; t0 += slots) {
     float low[4], high[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
     for (int block = 0; block < blocks; ++block) {
-      int e2 = 0;
-      if constexpr (T == DQ_F32 && TC == DQ_F16) {  // scaled to a largest value in [2^14, 2^15)
-        float top = 0;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(as_f(raw.x[s][i / 4][i % 4])));
-        top = row_max(top);
-        e2 = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-      }
-      v4f sum = {0, 0, 0, 0}, size = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        v4u part[NP], down, mag;  // down: the halves of values that are not above 0
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (T == DQ_F32) {
-            const float y0 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2]), e2), y1 = ldexpf(as_f(raw.x[s][e / 2][e % 2 * 2 + 1]), e2);
-            u32 p = pack<TC>(y0, y1);
-            part[0][e] = p;
-            part[1][e] = pack<TC>(y0 - widen<TC>(p), y1 - widen_hi<TC>(p));
-            down[e] = (y0 > 0 ? 0u : 0xFFFFu) | (y1 > 0 ? 0u : 0xFFFF0000u);
-            // (what the parts leave out is less than 2^-20 (2^-16) of the value, or of the least magnitude that counts here)
-            constexpr float kLeast = TC == DQ_F16 ? 0x1p-4f : 0x1p-100f;
-            mag[e] = pack<TC>(y0 != y0 ? y0 : fmaxf(fabsf(y0), kLeast), y1 != y1 ? y1 : fmaxf(fabsf(y1), kLeast));
-          } else {
-            const u32 y = raw.x[s][0][e];
-            part[0][e] = y;
-            down[e] = __builtin_bit_cast(u32, __builtin_bit_cast(v2s, y) >> 15);
-            mag[e] = y & 0x7FFF7FFFu;
-          }
-        }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          sum = mma<TC>(part[p] & ~down, x[1][s], sum);
-          sum = mma<TC>(part[p] & down, x[0][s], sum);
-        }
-        size = mma<TC>(mag, most[s], size);
-      }
-      if (block + 1 < blocks)
-        read_q(t0, block + 1);
-      else if (t0 + slots < last)
-        read_q(t0 + slots, 0);
-      // the lane holds its page's products with rows 4 g .. + 3
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float d = fmaf(error, size[i], 0x1p-118f);
-        const bool fine = d < INFINITY && fabsf(sum[i]) < INFINITY && !bad;
-        const int back = T == DQ_F32 && TC == DQ_F16 ? -__shfl(e2, 4 * g + i, 64) : 0;
-        low[i] = fmaxf(low[i], fine ? ldexpf(sum[i] - d, back) : -INFINITY);
-        high[i] = fmaxf(high[i], fine ? ldexpf(sum[i] + d, back) : INFINITY);
-      }
+      tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, [&]() {
+        if (block + 1 < blocks)
+          read_q(t0, block + 1);
+        else if (t0 + slots < last)
+          read_q(t0 + slots, 0);
+      });
     }
-    // the largest of a token's rows: of a lane's, then of two or all four lane groups
-    if (lanes > 1) {
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        low[i] = fmaxf(low[i], low[i + 1]);
-        high[i] = fmaxf(high[i], high[i + 1]);
-      }
-    }
-    if (lanes > 2) {
-      low[0] = fmaxf(low[0], low[2]);
-      high[0] = fmaxf(high[0], high[2]);
-    }
-    if (lanes > 4) {
-      low[0] = pair_max16(low[0]);
-      high[0] = pair_max16(high[0]);
-    }
-    if (lanes > 8) {
-      low[0] = pair_max32(low[0]);
-      high[0] = pair_max32(high[0]);
-    }
+    token_max(low, lanes);
+    token_max(high, lanes);
     const int64_t row0 = t0 - token0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -293,20 +312,19 @@ DQ_DEV double lanes_sum(double x, int log2) {
 
 // The 64-bit scores of row t's query heads on `count` pages id_of(j), as whole numbers that order as they do: most[j] (in LDS, 0 before)
 // is the largest over the heads. A wave's work: every `step`th, from its `first` on, of the steps of a page and 64 / 2^log2
-// of its heads; kSteps steps' loads are under way together.
-template <int T, int TC, class F>
+// of its heads; N steps' loads are under way together.
+template <int T, int TC, int N = 4, class F>
 DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int count, F&& id_of, uint64_t* most, int first, int step, int log2,
                        int lane) {
-  constexpr int kSteps = 4;
   const int lanes = 1 << log2, d = 8 * (lane & (lanes - 1)), at_once = 64 >> log2, turns = (a.group + at_once - 1) / at_once;
   const bool in = d < a.dim;
   const int steps = count * turns;
-  for (int i0 = first * kSteps; i0 < steps; i0 += step * kSteps) {
-    v4u lo[kSteps], hi[kSteps], x[kSteps][T == DQ_F32 ? 2 : 1];
-    int page[kSteps];
-    bool bad[kSteps];
+  for (int i0 = first * N; i0 < steps; i0 += step * N) {
+    v4u lo[N], hi[N], x[N][T == DQ_F32 ? 2 : 1];
+    int page[N];
+    bool bad[N];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
+    for (int k = 0; k < N; ++k) {
       const int i = min(i0 + k, steps - 1);  // (past the steps: the last again)
       page[k] = i / turns;
       const int head = min((i - page[k] * turns) * at_once + (lane >> log2), a.group - 1);
@@ -318,7 +336,7 @@ DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int
       load8<T>(a, (int64_t)t * a.q_token + (int64_t)(h * a.group + head) * a.q_head + (in ? d : 0), x[k]);
     }
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
+    for (int k = 0; k < N; ++k) {
       double s[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -336,29 +354,23 @@ DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int
 DQ_DEV uint64_t load_key(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 DQ_DEV void store_key(uint64_t* p, uint64_t x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// The choice: W waves take a row's kv head (W 1: four rows a workgroup). The count-th largest of the intervals' ends is found bit
-// by bit, on whole numbers that order as they do. kHeld: a row's intervals lie in registers, N to a lane, else they are read again for every
-// bit. Wave w takes a run of the pages, so that the list comes out ascending.
-template <int T, int TC, int N, int W, bool kHeld>
-__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs a, ChooseArgs c, int token0, int64_t rows, int log2) {
-  constexpr int R = W == 1 ? 4 : 1;  // rows of a workgroup
-  __shared__ int s_counts[2][W], s_list[R][64];
-  __shared__ uint64_t s_key[R][64];
-  const int lane = threadIdx.x & 63, hk = a.cache.kv_heads;
-  const int in_group = uniform(threadIdx.x >> 6), w = W == 1 ? 0 : in_group, r = W == 1 ? in_group : 0;
-  const int64_t row = (int64_t)blockIdx.x * R + r;
-  if (row >= rows) return;
-  const int t = token0 + (int)(row / hk), h = (int)(row % hk);
-  uint64_t* keys = c.keys + row * c.pages;
-  v2f held[N];  // the intervals, under way before anything is known of the row
-  if constexpr (kHeld) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      held[i] = c.keys != nullptr ? *reinterpret_cast<const v2f*>(keys + min((w * N + i) * 64 + lane, c.pages - 1)) : v2f{0, 0};
-  }
-  const int b = find_seq(a, t, lane);
-  if (b < 0) return;
-  const int pages = pages_of(row_sees(a, b, t, seq_len(a, b)), a.cache.page_size);
+// The choice: W waves take a row's kv head. The count-th largest of the intervals' ends is found bit by bit, on whole numbers that
+// order as they do. kHeld: a row's intervals lie in registers, N to a lane (`held`), else they are read again for every bit. Wave w takes
+// a run of the pages, so that the list comes out ascending. exact(n) sums the scores of the n open pages in sh.list into sh.key;
+// it is called once for a row with more pages than it reads.
+template <int W>
+struct ChoiceLds {
+  int counts[2][W], list[64];
+  uint64_t key[64];
+};
+
+template <int T, int TC, int N, int W, bool kHeld, class F>
+DQ_DEV void choose_row(const AttnArgs& a, const ChooseArgs& c, int t, int h, int b, int pages, uint64_t* keys, const v2f (&held)[N], ChoiceLds<W>& sh,
+                       int w, int lane, int log2, F&& exact) {
+  auto &s_counts = sh.counts;
+  auto &s_list = sh.list;
+  auto &s_key = sh.key;
+  const int hk = a.cache.kv_heads;
   int32_t* out = c.chosen + ((int64_t)t * hk + h) * c.count;
   const int count = (int)min(c.count, (int64_t)pages), tid = w * 64 + lane;
   for (int64_t i = count + tid; i < c.count; i += 64 * W) out[i] = -1;
@@ -481,38 +493,41 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     for (int i = 0; i < w; ++i) before += s_counts[turn][i];
   const int room = count - (able - open);  // for open ones
   uint64_t taken = 0;  // of the open ones, in their order
-  if (open > 0 && open <= 64) {
+  const int looked = open <= 64 ? open : 0;
+  if (looked > 0) {
     int at = before;
-    s_key[r][lane] = 0;  // (of all waves alike)
+    s_key[lane] = 0;  // (of all waves alike)
     each([&](int i, u32 l, u32 u) {
       const bool mine = u >= floor && l <= ceiling;
       const uint64_t m = __ballot(mine);
-      if (mine) s_list[r][at + __popcll(m & ((1ull << lane) - 1))] = kHeld ? number[kHeld ? i : 0] : list[base + i * 64 + lane];
+      if (mine) s_list[at + __popcll(m & ((1ull << lane) - 1))] = kHeld ? number[kHeld ? i : 0] : list[base + i * 64 + lane];
       at += __popcll(m);
     });
     if constexpr (W > 1) __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    exact_keys<T, TC>(a, c, t, h, open, [&](int j) { return s_list[r][j]; }, s_key[r], w, W, log2, lane);
+  }
+  exact(looked);
+  if (looked > 0) {
     if constexpr (W > 1) __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    const uint64_t key = lane < open ? s_key[r][lane] : 0;
+    const uint64_t key = lane < open ? s_key[lane] : 0;
     int rank = 0;
     for (int j = 0; j < open; ++j) {
-      const uint64_t o = s_key[r][j];
+      const uint64_t o = s_key[j];
       rank += o > key || (o == key && j < lane);
     }
     taken = __ballot(lane < open && rank < room);
   } else if (open > 64) {
     for (int p0 = 0; p0 < pages; p0 += 64) {
       const int some = min(64, pages - p0);
-      s_key[r][lane] = 0;
+      s_key[lane] = 0;
       if constexpr (W > 1) __syncthreads();
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-      exact_keys<T, TC>(a, c, t, h, some, [&](int j) { return list[p0 + j]; }, s_key[r], w, W, log2, lane);
+      exact_keys<T, TC>(a, c, t, h, some, [&](int j) { return list[p0 + j]; }, s_key, w, W, log2, lane);
       if constexpr (W > 1) __syncthreads();
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
       const int p = p0 + lane;
-      if (w == 0 && lane < some) store_key(keys + p, p < c.first || p >= pages - c.last ? kAlways : s_key[r][lane]);
+      if (w == 0 && lane < some) store_key(keys + p, p < c.first || p >= pages - c.last ? kAlways : s_key[lane]);
       if constexpr (W > 1) __syncthreads();
     }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "agent");
@@ -577,6 +592,88 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
     at += __popcll(m);
     seen += __popcll(mo);
   });
+}
+
+// W 1: four rows a workgroup.
+template <int T, int TC, int N, int W, bool kHeld>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs a, ChooseArgs c, int token0, int64_t rows, int log2) {
+  constexpr int R = W == 1 ? 4 : 1;  // rows of a workgroup
+  __shared__ ChoiceLds<W> sh[R];
+  const int lane = threadIdx.x & 63, hk = a.cache.kv_heads;
+  const int in_group = uniform(threadIdx.x >> 6), w = W == 1 ? 0 : in_group, r = W == 1 ? in_group : 0;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
+  if (row >= rows) return;
+  const int t = token0 + (int)(row / hk), h = (int)(row % hk);
+  uint64_t* keys = c.keys + row * c.pages;
+  v2f held[N];  // the intervals, under way before anything is known of the row
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      held[i] = c.keys != nullptr ? *reinterpret_cast<const v2f*>(keys + min((w * N + i) * 64 + lane, c.pages - 1)) : v2f{0, 0};
+  }
+  const int b = find_seq(a, t, lane);
+  if (b < 0) return;
+  const int pages = pages_of(row_sees(a, b, t, seq_len(a, b)), a.cache.page_size);
+  choose_row<T, TC, N, W, kHeld>(a, c, t, h, b, pages, keys, held, sh[r], w, lane, log2, [&](int n) {
+    exact_keys<T, TC>(a, c, t, h, n, [&](int j) { return sh[r].list[j]; }, sh[r].key, w, W, log2, lane);
+  });
+}
+
+// Both steps in one launch, for rows whose pages no other row's scores share: a workgroup's waves score a row's pages, 16 each
+// in turn, into LDS; the first wave chooses.
+constexpr int kPickPages = 512;
+
+template <int T, int TC, int DP>
+__global__ __launch_bounds__(DP <= 128 ? 1024 : 512) void k_page_pick(AttnArgs a, ChooseArgs c, int token0, int log2) {
+  constexpr int kWaves = DP <= 128 ? 16 : 8, N = kPickPages / 64;
+  __shared__ ChoiceLds<1> sh;
+  __shared__ v2f s_scores[kPickPages];
+  __shared__ int s_open;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hk = a.cache.kv_heads;
+  const int n = lane & 15, g = lane >> 4;
+  const int h = (int)(blockIdx.x % hk), t = token0 + (int)(blockIdx.x / hk);
+  const int b = find_seq(a, t, lane);
+  if (b < 0) return;
+  const int blocks = (a.group + 15) / 16;
+  RawQ<T, DP> raw;
+  load_q<T, DP>(a, true, t, h * a.group + min(n, a.group - 1), g, raw);  // (a row past the heads is the last again)
+  const int32_t* list = a.pages + b * a.pages_stride;
+  const int pages = pages_of(row_sees(a, b, t, seq_len(a, b)), a.cache.page_size);
+  if (pages > c.count) {
+    const float error = score_error<T, TC>(a.dim);
+    for (int p0 = 16 * wave; p0 < pages; p0 += 16 * kWaves) {
+      PageTile<DP> page;
+      load_page_tile<DP>(a, c, h, p0 + n < pages ? list[p0 + n] : 0, g, page);
+      v4u most[DP / 32];
+      magnitudes<DP>(page, most);
+      float low[4], high[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
+      for (int block = 0; block < blocks; ++block) {
+        if (blocks > 1) load_q<T, DP>(a, true, t, h * a.group + min(16 * block + n, a.group - 1), g, raw);
+        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, []() {});
+      }
+      token_max(low, 16);
+      token_max(high, 16);
+      if (g == 0 && p0 + n < pages) s_scores[p0 + n] = v2f{low[0], high[0]};
+    }
+  }
+  __syncthreads();
+  // all waves sum what is open
+  auto exact = [&](int n) {
+    if (wave == 0 && lane == 0) s_open = n;
+    __syncthreads();
+    exact_keys<T, TC, 1>(a, c, t, h, s_open, [&](int j) { return sh.list[j]; }, sh.key, wave, kWaves, log2, lane);
+    __syncthreads();
+  };
+  if (wave > 0) {
+    if (pages > c.count) exact(0);
+    return;
+  }
+  v2f held[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) held[i] = s_scores[i * 64 + lane];
+  choose_row<T, TC, N, 1, true>(a, c, t, h, b, pages, c.keys + ((int64_t)(t - token0) * hk + h) * c.pages, held, sh, 0, lane, log2, exact);
 }
 
 // ---- attention over chosen pages ---------------------------------------------
@@ -818,6 +915,8 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
 
 // Waves that a launch of scores aims at.
 constexpr int64_t kScoreWaves = 4096;
+// Rows of a sequence from which on their scores share what is read of a page. XXX
+constexpr int kSharedRows = 4;
 
 // lanes that hold a head's values, 8 each: their number's logarithm
 int lanes_log2(int dim) {
@@ -849,6 +948,17 @@ hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, cons
   for (int64_t t = 0; t < a.tokens; t += c.tokens) {
     const int64_t rows = (a.tokens - t < c.tokens ? a.tokens - t : c.tokens) * a.cache.kv_heads;
     const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
+      const int log2 = lanes_log2(a.dim);
+      if (c.pages > c.count && c.pages <= kPickPages && a.max_q < kSharedRows) {
+        const dim3 grid((uint32_t)rows);
+        if (a.dim <= 64)
+          hipLaunchKernelGGL((k_page_pick<tq(), tc(), 64>), grid, dim3(1024), 0, s, a, c, (int)t, log2);
+        else if (a.dim <= 128)
+          hipLaunchKernelGGL((k_page_pick<tq(), tc(), 128>), grid, dim3(1024), 0, s, a, c, (int)t, log2);
+        else
+          hipLaunchKernelGGL((k_page_pick<tq(), tc(), 256>), grid, dim3(512), 0, s, a, c, (int)t, log2);
+        return hipGetLastError();
+      }
       if (c.pages > c.count) {  // (else every page is read)
         const int64_t tiles = (a.max_q + slots - 1) / slots, waves = (int64_t)a.batch * a.cache.kv_heads * ((c.pages + 15) / 16);
         const int64_t ranges = std::max<int64_t>(1, std::min(tiles, kScoreWaves / waves)), per = (tiles + ranges - 1) / ranges * slots;
@@ -862,7 +972,6 @@ hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, cons
           hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
       }
-      const int log2 = lanes_log2(a.dim);
       if (c.pages <= 8 * 64)
         hipLaunchKernelGGL((k_page_choice<tq(), tc(), 8, 1, true>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, c, (int)t, rows, log2);
       else if (c.pages <= 8 * 16 * 64)

@@ -183,14 +183,19 @@ struct MassPlan {
   int64_t bytes = 0;
 };
 
-// Items that a launch of dq_attention_mass aims at, keys of one, and rows that are worth one.
+// Items that a launch of dq_attention_mass aims at, keys of one, and rows that are worth one: fewer where items are so few that CUs
+// would be idle. XXX
 constexpr int64_t kMassItems = 1536, kMassKeys = 256, kMassRows = 256;
+constexpr int64_t kMassFewItems = 256, kMassFewRows = 64;
 
 MassPlan plan_mass(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* q) {
   MassPlan p;
   const int64_t rows = std::min(s->max_q, s->tokens) * (q->heads / c->kv_heads);
   const int64_t items = s->batch * c->kv_heads * ceil_div(s->max_len, kMassKeys), keys = s->batch * c->kv_heads * s->max_len * 4;
-  if (items > 0) p.splits = std::max<int64_t>(1, std::min({kMassItems / items, rows / kMassRows, kWorkspace / keys}));
+  if (items > 0) {
+    p.splits = std::max(std::min(kMassItems / items, rows / kMassRows), std::min(kMassFewItems / items, rows / kMassFewRows));
+    p.splits = std::max<int64_t>(1, std::min(p.splits, kWorkspace / keys));
+  }
   p.items = items * p.splits;
   if (p.splits > 1) p.bytes = p.splits * keys;
   return p;
