@@ -645,8 +645,13 @@ __global__ __launch_bounds__(kThreads) void k_compact(AttnArgs a, CompactArgs c,
 
 }  // namespace
 
-// Rows of a sequence from which on its queries go through LDS. XXX
-constexpr int kManyRows = 64;
+// Rows of a sequence from which on its queries go through LDS: 8 sequences of 4,096 keys, 32 / 8 heads, us without and with: bf16 heads of
+// 128, 32 / 64 / 128 / 256 rows: 16.0 and 20.1, 19.8 and 20.6, 24.7 and 21.9, 34.0 and 27.0; fp32 rows, 32 / 64 / 128: 20.7 and 21.2, 28.2 and
+// 24.3, 40.1 and 29.8; heads of 64, 64 / 128 rows: 12.0 and 11.5, 15.9 and 13.3. Heads over 128 values leave it one wave a SIMD: 64 / 256 rows in
+// heads of 256, 35.3 and 47.6, 57.4 and 67.1; from many more rows on it is the same in 16 bits (2,048 tokens: 107 and 106) and pays in fp32 (256 and 217).
+template <int T>
+constexpr int kManyRows = T == DQ_F32 ? 64 : 128;
+constexpr int kManyRowsWide = 1024;
 
 hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, const MassArgs& m, hipStream_t s) {
   const int tiles = (a.max_len + kMassKeys - 1) / kMassKeys;
@@ -655,7 +660,7 @@ hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, co
     // (a tile holds whole tokens, whose rows are addressed from its first in 32 bits)
     constexpr int kRows = kMassRows<tq()>;
     const bool near = a.q_token < (1 << 22) && a.q_head < (1 << 22);
-    const bool many = (int64_t)a.max_q * a.group >= kManyRows && a.group <= kRows && near;
+    const bool many = (int64_t)a.max_q * a.group >= (a.dim <= 128 ? kManyRows<tq()> : kManyRowsWide) && a.group <= kRows && near;
     const auto go = [&](auto dp) {
       if (many)
         hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);

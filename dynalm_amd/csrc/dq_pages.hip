@@ -619,8 +619,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void k_page_choice(AttnArgs 
   });
 }
 
-// Both steps in one launch, for rows whose pages no other row's scores share: a workgroup's waves score a row's pages, 16 each
-// in turn, into LDS; the first wave chooses.
+// Both steps in one launch, for few rows: a workgroup's waves score a row's pages, 16 each in turn, into LDS; the first wave
+// chooses, all sum what is open.
 constexpr int kPickPages = 512;
 
 template <int T, int TC, int DP>
@@ -915,8 +915,12 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
 
 // Waves that a launch of scores aims at.
 constexpr int64_t kScoreWaves = 4096;
-// Rows of a sequence from which on their scores share what is read of a page. XXX
-constexpr int kSharedRows = 4;
+// Rows (of all kv heads) up to which one launch does both, a workgroup a row: one on every CU. More of them leave the choices, a
+// wave each, to wait for each other; few of them on many pages leave CUs idle that could read bounds. One launch against two, us, 32 / 8 bf16 heads
+// of 128: 64 pages, 8 / 64 / 256 / 512 / 1,024 rows: 8.6 against 13.7, 9.6 / 14.5, 10.0 / 14.8, 16.9 / 16.3, 30.8 / 19.1; 256 pages, 32 / 256 /
+// 512 rows: 11.6 / 14.5, 12.7 / 20.5, 23.4 / 28.1; 512 pages, 8 / 64 / 128 / 256 / 512 rows: 16.7 / 15.4, 16.2 / 16.3, 16.5 / 20.8, 19.4 / 28.2, 28.8 /
+// 28.3. Rows of one sequence share what two launches read: 64 rows of two sequences on 64 pages 9.8 / 14.9, 128 of one on 512 28.7 / 21.3.
+constexpr int64_t kPickRows = 256;
 
 // lanes that hold a head's values, 8 each: their number's logarithm
 int lanes_log2(int dim) {
@@ -949,7 +953,7 @@ hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, cons
     const int64_t rows = (a.tokens - t < c.tokens ? a.tokens - t : c.tokens) * a.cache.kv_heads;
     const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
       const int log2 = lanes_log2(a.dim);
-      if (c.pages > c.count && c.pages <= kPickPages && a.max_q < kSharedRows) {
+      if (c.pages > c.count && rows <= kPickRows && (c.pages <= kPickPages / 2 || (c.pages <= kPickPages && rows >= kPickRows / 2))) {
         const dim3 grid((uint32_t)rows);
         if (a.dim <= 64)
           hipLaunchKernelGGL((k_page_pick<tq(), tc(), 64>), grid, dim3(1024), 0, s, a, c, (int)t, log2);

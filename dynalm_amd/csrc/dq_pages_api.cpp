@@ -153,7 +153,7 @@ struct PagePlan {
 };
 
 // Items that a launch of dq_page_attention aims at, and keys that are worth one.
-constexpr int64_t kPageItems = 512, kPageKeys = 256;
+constexpr int64_t kPageItems = 256, kPageKeys = 256;
 
 PagePlan plan_pages(const dq_kv_cache* c, const dq_sequences* s, const dq_heads* q, int64_t count) {
   PagePlan p;
