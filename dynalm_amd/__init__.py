@@ -22,6 +22,8 @@ dynacore/include/dynacore/device/device.h:89-161):
     qk_norm_rope(...)              head norms and rotation (Device::rms_norm, rope)
     kv_append(cache, ...)          keys and values into a paged cache (Device::kv_store)
     shared_attention(cache, ...)   attention over a shared prefix and own pages
+    page_bounds, choose_pages, page_attention(cache, ...)  the pages that a query reads
+    attention_mass, kv_keep, kv_compact(...)               the keys that stay in a cache
     GgufFile.open(path)                dynalm's GgufFile::open / open_parts (host mmap + parse)
     GgufFile.upload(name)              Device::upload of a GGUF tensor
 

@@ -147,7 +147,10 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
 // whole tokens as kMassRows rows hold, so that a thread's rows lie at the same offsets from every tile's first token (rows that
 // are left have a weight of 0); a row's 16-byte chunks lie at their number XOR some bits of the row's, which spreads a
 // column of rows over the banks. The products of 16 rows stand beside the exponentials of the 16 before.
-// A prompt of 4,096 tokens, 32 / 8 f16 heads of 128 (68.7 GFLOP): XXX us.
+// A prompt of 4,096 tokens, 32 / 8 f16 heads of 128 (68.7 GFLOP, half of the square): 92 us and 6 for the join, 740 TFLOP/s, where a large
+// matrix product reaches 1,180. Bound by issue: 16 MFMAs (256 clocks), 16 exponentials (128) and 32 sums (128) of a wave stand for 16 rows x 64 keys;
+// the matrix cores are busy 39% of the time, the vector unit 65%. Without the LDS 257 us; with parts that are ranges of rows, not turns, 124 (a
+// third of the CUs idle at the end); with a wait for the keys inside the loop 142; four waves a SIMD spill (178).
 
 template <int T>
 constexpr int kMassRows = T == DQ_F32 ? 32 : 64;
@@ -359,8 +362,8 @@ __global__ __launch_bounds__(256) void k_mass_join(AttnArgs a, MassArgs m, int64
 // A workgroup takes a sequence's kv head. The budget-th largest weight is found on whole numbers that order as the weights do:
 // a histogram of kBins bins between their least and largest says in which bin it lies, another one of that bin's
 // numbers where in it, until a bin is one number, or taken as a whole: three passes at most. Wave w holds (or, kHeld false, reads again for each
-// pass) a run of the places, so that the list comes out ascending. Bit by bit, with a barrier each: 20 to 29 us in place of XXX
-// for 16,384 places.
+// pass) a run of the places, so that the list comes out ascending. Bound by latency and, for long rows, by issue: 15
+// rows of 5,001 places 9 us, 256 of 16,384 21 us (3.3 and 6 of them for the reads); bit by bit, with a barrier for each, 20 and 29.
 
 constexpr int kKeepWaves = 16;
 constexpr int kBinsLog2 = 11, kBins = 1 << kBinsLog2;
@@ -693,7 +696,8 @@ hipError_t launch_kv_keep(int64_t batch, const KeepArgs& k, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Sequences and heads below which a workgroup of a move in place has 512 threads. XXX
+// Sequences and heads below which a workgroup of a move in place has 512 threads, us with 256 and with 512 (8 heads of 128, 2,048 of
+// 8,192 keys, the choice before it among them): 1 / 4 / 8 / 16 / 32 sequences 39.4 and 26.9, 44.1 and 31.4, 44.7 and 36.5, 71.4 and 70.3, 119 and 126.
 constexpr int64_t kFewMoves = 128;
 
 hipError_t launch_kv_compact(const AttnArgs& a, const CompactArgs& c, hipStream_t s) {
