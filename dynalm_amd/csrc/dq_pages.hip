@@ -230,21 +230,21 @@ DQ_DEV void tile_scores(const RawQ<T, DP>& raw, const PageTile<DP>& page, const 
   }
 }
 
-// The largest over a token's `lanes` rows: of a lane's, then of two or all four lane groups.
-DQ_DEV void token_max(float (&x)[4], int lanes) {
-  if (lanes > 1) {
+// The largest over a token's `rows` rows: of a lane's, then of two or all four lane groups.
+DQ_DEV void token_max(float (&x)[4], int rows) {
+  if (rows > 1) {
     x[0] = fmaxf(x[0], x[1]);
     x[2] = fmaxf(x[2], x[3]);
   }
-  if (lanes > 2) x[0] = fmaxf(x[0], x[2]);
-  if (lanes > 4) x[0] = pair_max16(x[0]);
-  if (lanes > 8) x[0] = pair_max32(x[0]);
+  if (rows > 2) x[0] = fmaxf(x[0], x[2]);
+  if (rows > 4) x[0] = pair_max16(x[0]);
+  if (rows > 8) x[0] = pair_max32(x[0]);
 }
 
 // A wave takes 16 pages of a kv head, whose bounds it holds, and of a sequence's rows a range, 16 at a time: `slots` tokens
-// of `lanes` rows, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
+// of 2^rows_log2 rows, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int lanes, int ranges, int range_tokens,
+__global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int rows_log2, int ranges, int range_tokens,
                                                      int64_t items) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
@@ -263,10 +263,10 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   const int64_t end = min(min(hi, (int64_t)a.tokens), (int64_t)token0 + c.tokens);
   const int64_t first = max(lo, (int64_t)token0) + (int64_t)range * range_tokens, last = min(first + range_tokens, end);
   if (p0 >= pages || first >= last) return;
-  const int slots = 16 / lanes, slot = n / lanes, blocks = (a.group + 15) / 16;
+  const int rows = 1 << rows_log2, slots = 16 >> rows_log2, slot = n >> rows_log2, blocks = (a.group + 15) / 16;
   RawQ<T, DP> raw;
   auto read_q = [&](int64_t t0, int block) {  // (a row past the heads is the last again)
-    load_q<T, DP>(a, true, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + n % lanes, a.group - 1), g, raw);
+    load_q<T, DP>(a, true, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + (n & (rows - 1)), a.group - 1), g, raw);
   };
   read_q(first, 0);
   PageTile<DP> page;
@@ -286,14 +286,13 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
           read_q(t0 + slots, 0);
       });
     }
-    token_max(low, lanes);
-    token_max(high, lanes);
-    const int64_t row0 = t0 - token0;
+    token_max(low, rows);
+    token_max(high, rows);
+    uint64_t* out = c.keys + ((t0 - token0) * hk + h) * c.pages + p0 + n;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 4 * g + i, to = row / lanes;
-      if (row % lanes == 0 && t0 + to < last && p0 + n < pages)
-        *reinterpret_cast<v2f*>(c.keys + ((row0 + to) * hk + h) * c.pages + p0 + n) = v2f{low[i], high[i]};
+      const int row = 4 * g + i, to = row >> rows_log2;
+      if ((row & (rows - 1)) == 0 && t0 + to < last && p0 + n < pages) *reinterpret_cast<v2f*>(out + (int64_t)to * hk * c.pages) = v2f{low[i], high[i]};
     }
   }
 }
@@ -955,9 +954,9 @@ hipError_t launch_page_bounds(int cache_type, const AttnArgs& a, const int32_t* 
 }
 
 hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, const ChooseArgs& c, hipStream_t s) {
-  int lanes = 1;
-  while (lanes < a.group && lanes < 16) lanes *= 2;
-  const int slots = 16 / lanes;
+  int rows_log2 = 0;
+  while ((1 << rows_log2) < a.group && rows_log2 < 4) ++rows_log2;
+  const int slots = 16 >> rows_log2;
   for (int64_t t = 0; t < a.tokens; t += c.tokens) {
     const int64_t rows = (a.tokens - t < c.tokens ? a.tokens - t : c.tokens) * a.cache.kv_heads;
     const hipError_t e = by_types(type, cache_type, [&](auto tq, auto tc) {
@@ -978,11 +977,11 @@ hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, cons
         const int64_t items = waves * ranges;
         const dim3 grid((uint32_t)((items + 3) / 4));
         if (a.dim <= 64)
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 64>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 64>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
         else if (a.dim <= 128)
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 128>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 128>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
         else
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, lanes, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
       }
       if (c.pages <= 8 * 64)
