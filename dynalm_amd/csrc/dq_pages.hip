@@ -682,17 +682,21 @@ __global__ __launch_bounds__(DP <= 128 ? 1024 : 512) void k_page_pick(AttnArgs a
 // ---- attention over chosen pages ---------------------------------------------
 // An item is (token, kv head, up to 16 of its query heads, range of the list): its rows see the same keys. The four
 // waves take 32 keys each in turn, with a running softmax of their own, and add up at the end. Scores are S^T = K
-// Q^T, which leaves a lane with the weights that O^T = V^T P^T takes from it; keys and values go straight
-// from memory to registers (a lane's 16 bytes of a key are its A operand, of the values it takes DP / 16 of 8 keys).
+// Q^T, which leaves a lane with the weights that O^T = V^T P^T takes from it. Loads take 16 bytes a lane and whole lines a
+// row of lanes: of values a lane holds DP / 16 of 8 keys, as O^T takes them; of keys S^T takes 8 values of one key a
+// lane, 16 keys a row of lanes, so they turn in LDS, a wave's own part of it (16 bytes of a key at a place turned by the key's number: no two of
+// a read meet in a bank). The next tile's keys are under way from when this one's are in LDS.
 //
-// 32 sequences of 4,096 chosen keys, 32 / 8 bf16 heads of 128 (537 MB): 92 us, 5.8 TB/s (a part of them from the cache behind the L2s). 473 rows
-// of 1,024 chosen keys each, two sequences of up to 8,192: 146 us under the tracer; 2 GB come from the L2s (93% hits), 14 TB/s; waves wait
-// for the issue of loads and for the L2s, the matrix cores and the vector unit are busy 10% and 20%. Four waves a SIMD (127 registers) against two
-// (184): 163 us; a tile's loads beside the products of the one before 158.
+// 32 sequences of 4,096 chosen keys, 32 / 8 bf16 heads of 128 (537 MB): 92 to 107 us, 5.0 to 5.8 TB/s (a part of them from the cache behind the L2s).
+// 473 rows of 1,024 chosen keys each, two sequences of up to 8,192: 81 us; 2 GB come from the L2s (93% hits), 24 TB/s. Keys loaded in S^T's order,
+// whose neighbouring lanes read 16 lines: 137 us; turned, not asked for early 86; rows of sums not turned in LDS 84.
 
 template <int DP>
 struct PageLds {
-  v4f o[4][16][DP / 4];
+  union alignas(16) {  // of a wave
+    v4u k[32][DP / 8];
+    v4f o[16][DP / 4];  // (a row's turned by its number)
+  } own[4];
   float ml[4][16][2];
   int bad;
 };
@@ -749,9 +753,12 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
 
   const u32 token_bytes = (u32)ca.token * 2;
   constexpr u32 kOut = 0x80000000u;  // an offset past every buffer: such loads give 0
-  u32 koff[DP / 32], voff[DP / 128 > 0 ? DP / 128 : 1];
-#pragma unroll
-  for (int s = 0; s < DP / 32; ++s) koff[s] = 32 * s + 8 * g < a.dim ? n * token_bytes + (32 * s + 8 * g) * 2 : kOut;
+  constexpr int kChunks = DP / 8, kLine = 64 / kChunks;  // 16 bytes, of a key; keys of a load
+  constexpr int kTurn = kChunks < 16 ? 7 : 15;
+  const int key0 = lane / kChunks, chunk0 = lane % kChunks;
+  const u32 koff = 8 * chunk0 < a.dim ? key0 * token_bytes + 16 * chunk0 : kOut;
+  auto& ktile = sh.own[wave].k;
+  u32 voff[DP / 128 > 0 ? DP / 128 : 1];
 #pragma unroll
   for (int s = 0; s < (DP / 128 > 0 ? DP / 128 : 1); ++s) {
     const int d = n * NC + 8 * s;
@@ -778,34 +785,42 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
     id = __builtin_amdgcn_ds_permute(4 * to, id);
     const int halves = __popcll(full | part) * units - left;  // of tiles: runs of 16 keys
     int e = 2 * wave / units, sub = 2 * wave % units;
-    for (int half = 2 * wave; half < halves; half += 8) {
-      PageKv<DP> r;
-      int kb[2];
-      int64_t base[2];
-      {
-        const int id0 = __builtin_amdgcn_readlane(id, e);
-        kb[0] = __builtin_amdgcn_readlane(entry, e) * ca.page_size + 16 * sub;
-        base[0] = id0 * ca.page + 16 * sub * ca.token + head * ca.head;
-        kb[1] = INT32_MAX - 16;  // (no key)
-        base[1] = base[0];
-        if (half + 1 < halves) {
-          const bool over = sub + 1 == units;
-          const int e2 = over ? e + 1 : e, sub2 = over ? 0 : sub + 1;
-          kb[1] = __builtin_amdgcn_readlane(entry, e2) * ca.page_size + 16 * sub2;
-          base[1] = __builtin_amdgcn_readlane(id, e2) * ca.page + 16 * sub2 * ca.token + head * ca.head;
-        }
-        e += skip;
-        sub += skip_rest;
-        if (sub >= units) {
-          sub -= units;
-          ++e;
-        }
+    // the tile at `half`: its keys' first indexes and places; its keys are asked for (past the end nothing is)
+    PageKv<DP> r;
+    int kb[2], kb_next[2];
+    int64_t base[2], base_next[2];
+    auto next = [&](int half) {
+      const int id0 = __builtin_amdgcn_readlane(id, e);
+      kb_next[0] = __builtin_amdgcn_readlane(entry, e) * ca.page_size + 16 * sub;
+      base_next[0] = id0 * ca.page + 16 * sub * ca.token + head * ca.head;
+      kb_next[1] = INT32_MAX - 16;  // (no key)
+      base_next[1] = base_next[0];
+      if (half + 1 < halves) {
+        const bool over = sub + 1 == units;
+        const int e2 = over ? e + 1 : e, sub2 = over ? 0 : sub + 1;
+        kb_next[1] = __builtin_amdgcn_readlane(entry, e2) * ca.page_size + 16 * sub2;
+        base_next[1] = __builtin_amdgcn_readlane(id, e2) * ca.page + 16 * sub2 * ca.token + head * ca.head;
+      }
+      e += skip;
+      sub += skip_rest;
+      if (sub >= units) {
+        sub -= units;
+        ++e;
       }
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
-        const auto kr = rsrc(ca.k + base[t2], 0x7FFFFFFFu);
+        const auto kr = rsrc(ca.k + base_next[t2], half < halves ? 0x7FFFFFFFu : 0u);
 #pragma unroll
-        for (int s = 0; s < DP / 32; ++s) r.k[t2][s] = ld16(kr, koff[s]);
+        for (int s = 0; s < DP / 32; ++s)
+          r.k[t2][s] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kr, koff, s * kLine * token_bytes, 0));
+      }
+    };
+    next(2 * wave);
+    for (int half = 2 * wave; half < halves; half += 8) {
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        kb[t2] = kb_next[t2];
+        base[t2] = base_next[t2];
       }
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
@@ -826,14 +841,27 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
           }
         }
       }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) {
+          const int key = key0 + s * kLine;
+          ktile[16 * t2 + key][chunk0 ^ (key & kTurn)] = r.k[t2][s];
+        }
+      __builtin_amdgcn_wave_barrier();
+      next(half + 8);
       float x[8];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
+        v4u k[DP / 32];
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) k[s] = ktile[16 * t2 + n][(4 * s + g) ^ (n & kTurn)];
         v4f acc = {0, 0, 0, 0};
 #pragma unroll
         for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-          for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(r.k[t2][s], q[p][s], acc);
+          for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(k[s], q[p][s], acc);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * t2 + i] = acc[i];
       }
@@ -889,7 +917,7 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
   for (int i = 0; i < 4; ++i) {
     const int d = (4 * g + i) * NC;
 #pragma unroll
-    for (int w = 0; w < NC / 4; ++w) sh.o[wave][n][d / 4 + w] = v4f{o[4 * w][i], o[4 * w + 1][i], o[4 * w + 2][i], o[4 * w + 3][i]};
+    for (int w = 0; w < NC / 4; ++w) sh.own[wave].o[n][(d / 4 + w) ^ n] = v4f{o[4 * w][i], o[4 * w + 1][i], o[4 * w + 2][i], o[4 * w + 3][i]};
   }
   if (bad) sh.bad = 1;
   __syncthreads();
@@ -906,7 +934,7 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
       const float mk = sh.ml[k][r][0];
       const float f = mk == -INFINITY ? 0.f : exp2_fast(mk - mx);
       sum = fmaf(sh.ml[k][r][1], f, sum);
-      y += sh.o[k][r][d4] * f;
+      y += sh.own[k].o[r][d4 ^ r] * f;
     }
     if (sh.bad) sum = __builtin_nanf("");
     const int h = head * a.group + tile0 + r;
