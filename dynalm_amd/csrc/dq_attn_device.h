@@ -153,35 +153,36 @@ template <int T, int DP>
 struct RawQ {
   v4u x[DP / 32][T == DQ_F32 ? 2 : 1];
 };
-template <int T, int DP>
-DQ_DEV void load_q(const AttnArgs& a, bool valid, int token, int head, int g, RawQ<T, DP>& r) {
-  const int64_t base = (int64_t)token * a.q_token + (int64_t)head * a.q_head;
+// 16 bytes of them: from value d of the head, in fp32 its values 4 k .. + 3 of 8 (0 past the head's dimension).
+template <int T>
+DQ_DEV v4u load_q16(const AttnArgs& a, int token, int head, int d, int k) {
+  const int64_t at = (int64_t)token * a.q_token + (int64_t)head * a.q_head + d;
+  v4u x = {0, 0, 0, 0};
+  if (d < a.dim) {
+    if constexpr (T == DQ_F32) {
+      const float* p = static_cast<const float*>(a.q) + at + 4 * k;
+      if (a.q_vec)
+        x = *reinterpret_cast<const v4u*>(p);
+      else
 #pragma unroll
-  for (int s = 0; s < DP / 32; ++s) {
-    const int d = 32 * s + 8 * g;
+        for (int i = 0; i < 4; ++i) x[i] = as_u(p[i]);
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(a.q) + at;
+      if (a.q_vec)
+        x = *reinterpret_cast<const v4u*>(p);
+      else
 #pragma unroll
-    for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) {
-      v4u x = {0, 0, 0, 0};
-      if (valid && d < a.dim) {
-        if constexpr (T == DQ_F32) {
-          const float* p = static_cast<const float*>(a.q) + base + d + 4 * k;
-          if (a.q_vec)
-            x = *reinterpret_cast<const v4u*>(p);
-          else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = as_u(p[i]);
-        } else {
-          const uint16_t* p = static_cast<const uint16_t*>(a.q) + base + d;
-          if (a.q_vec)
-            x = *reinterpret_cast<const v4u*>(p);
-          else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (u32)p[2 * i] | ((u32)p[2 * i + 1] << 16);
-        }
-      }
-      r.x[s][k] = x;
+        for (int i = 0; i < 4; ++i) x[i] = (u32)p[2 * i] | ((u32)p[2 * i + 1] << 16);
     }
   }
+  return x;
+}
+template <int T, int DP>
+DQ_DEV void load_q(const AttnArgs& a, bool valid, int token, int head, int g, RawQ<T, DP>& r) {
+#pragma unroll
+  for (int s = 0; s < DP / 32; ++s)
+#pragma unroll
+    for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) r.x[s][k] = valid ? load_q16<T>(a, token, head, 32 * s + 8 * g, k) : v4u{0, 0, 0, 0};
 }
 template <int T, int TC, int DP>
 DQ_DEV float q_operands(const AttnArgs& a, const RawQ<T, DP>& r, v4u (&q)[kParts<T, TC>][DP / 32]) {

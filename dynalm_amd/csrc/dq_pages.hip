@@ -243,15 +243,22 @@ DQ_DEV void token_max(float (&x)[4], int rows) {
 
 // A wave takes 16 pages of a kv head, whose bounds it holds, and of a sequence's rows a range, 16 at a time: `slots` tokens
 // of 2^rows_log2 rows, a power of two of at least the kv head's query heads (16 where they are more: one 16 after the other).
+// The four waves of a workgroup take 64 pages in a row and read the same rows: each loads a part of the next ones, all take them from LDS
+// (a row's 16 bytes a lane are lines of 16 rows at once, slow to ask for; every wave for itself 41.4 us against 37.9 of scores and choice below,
+// with fp32 rows 72 against 59).
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int rows_log2, int ranges, int range_tokens,
-                                                     int64_t items) {
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int64_t item = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  if (item >= items) return;
-  const int hk = a.cache.kv_heads, page_tiles = (c.pages + 15) / 16;
-  const int p0 = (int)(item % page_tiles) * 16, h = (int)(item / page_tiles % hk);  // (a workgroup's waves read the same rows)
-  const int range = (int)(item / hk / page_tiles % ranges), b = (int)(item / hk / page_tiles / ranges);
+__global__ __launch_bounds__(256, 2) void k_page_scores(AttnArgs a, ChooseArgs c, int token0, int rows_log2, int ranges, int range_tokens) {
+  constexpr int K = T == DQ_F32 ? 2 : 1, kLoads = DP / 32 * K;  // 16 bytes a lane, of 16 rows
+  constexpr int kMine = (kLoads + 3) / 4;                       // of a wave
+  __shared__ v4u sh[2][kLoads][64];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = uniform(threadIdx.x >> 6);
+  const int hk = a.cache.kv_heads, page_groups = (c.pages + 63) / 64;
+  u32 item = blockIdx.x;
+  const int group0 = (int)(item % page_groups) * 64, p0 = group0 + 16 * wave;
+  item /= page_groups;
+  const int h = item % hk;
+  item /= hk;
+  const int range = item % ranges, b = item / ranges;
   // the range's tokens, of the launch's (offsets, length and page numbers under way together)
   const int64_t lo = a.q_offsets != nullptr ? a.q_offsets[b] : b, hi = a.q_offsets != nullptr ? a.q_offsets[b + 1] : b + 1;
   // (the last sequence's list may end with its keys)
@@ -262,30 +269,52 @@ __global__ __launch_bounds__(256) void k_page_scores(AttnArgs a, ChooseArgs c, i
   if (b + 1 == a.batch && p0 + n < pages) listed = list[p0 + n];
   const int64_t end = min(min(hi, (int64_t)a.tokens), (int64_t)token0 + c.tokens);
   const int64_t first = max(lo, (int64_t)token0) + (int64_t)range * range_tokens, last = min(first + range_tokens, end);
-  if (p0 >= pages || first >= last) return;
+  if (group0 >= pages || first >= last) return;
   const int rows = 1 << rows_log2, slots = 16 >> rows_log2, slot = n >> rows_log2, blocks = (a.group + 15) / 16;
-  RawQ<T, DP> raw;
-  auto read_q = [&](int64_t t0, int block) {  // (a row past the heads is the last again)
-    load_q<T, DP>(a, true, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + (n & (rows - 1)), a.group - 1), g, raw);
+  v4u mine[kMine];
+  auto read = [&](int64_t t0, int block) {  // (a row past the heads is the last again)
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int load = 4 * j + wave;
+      if (kLoads % 4 == 0 || load < kLoads)
+        mine[j] = load_q16<T>(a, (int)min(t0 + slot, last - 1), h * a.group + min(16 * block + (n & (rows - 1)), a.group - 1),
+                              32 * (load / K) + 8 * g, load % K);
+    }
   };
-  read_q(first, 0);
+  auto share = [&](int at) {
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int load = 4 * j + wave;
+      if (kLoads % 4 == 0 || load < kLoads) sh[at][load][lane] = mine[j];
+    }
+    __syncthreads();
+  };
+  read(first, 0);
   PageTile<DP> page;
   load_page_tile<DP>(a, c, h, p0 + n < pages ? listed : 0, g, page);
+  share(0);
   v4u most[DP / 32];
   magnitudes<DP>(page, most);
   const float error = score_error<T, TC>(a.dim);
+  int at = 0;
   for (int64_t t0 = first; t0 < last; t0 += slots) {
     float low[4], high[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
     for (int block = 0; block < blocks; ++block) {
-      tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, [&]() {
-        if (block + 1 < blocks)
-          read_q(t0, block + 1);
-        else if (t0 + slots < last)
-          read_q(t0 + slots, 0);
-      });
+      const bool same = block + 1 < blocks;
+      const int64_t t1 = same ? t0 : t0 + slots;
+      if (t1 < last) read(t1, same ? block + 1 : 0);
+      if (p0 < pages) {
+        RawQ<T, DP> raw;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) raw.x[i / K][i % K] = sh[at][i][lane];
+        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, []() {});
+      }
+      at ^= 1;
+      if (t1 < last) share(at);  // (read a tile ago, before the last barrier)
     }
+    if (p0 >= pages) continue;
     token_max(low, rows);
     token_max(high, rows);
     uint64_t* out = c.keys + ((t0 - token0) * hk + h) * c.pages + p0 + n;
@@ -949,13 +978,14 @@ __global__ __launch_bounds__(256, (T != DQ_F32 && DP <= 128 ? 3 : 1)) void k_pag
   }
 }
 
-// Waves that a launch of scores aims at.
-constexpr int64_t kScoreWaves = 4096;
+// Workgroups that a launch of scores aims at. 512 / 768 / 1,024 / 2,048, us of scores and choice, 512 rows of 4 kv heads of 8 f16 heads of 64, 128, 256
+// and 512 pages: 36 / 34 / 33 / 33, 41.7 / 39.1 / 37.9 / 40.4, 58 / 56 / 57 / 60; 2,048 rows, of 128: 111 / 100 / 94 / 94.
+constexpr int64_t kScoreGroups = 1024;
 // Rows (of all kv heads) up to which one launch does both, a workgroup a row: one on every CU. More of them leave the choices, a
 // wave each, to wait for each other; few of them on many pages leave CUs idle that could read bounds. One launch against two, us, 32 / 8 bf16 heads
-// of 128: 64 pages, 8 / 64 / 256 / 512 / 1,024 rows: 8.6 against 13.7, 9.6 / 14.5, 10.0 / 14.8, 16.9 / 16.3, 30.8 / 19.1; 256 pages, 32 / 256 /
-// 512 rows: 11.6 / 14.5, 12.7 / 20.5, 23.4 / 28.1; 512 pages, 8 / 64 / 128 / 256 / 512 rows: 16.7 / 15.4, 16.2 / 16.3, 16.5 / 20.8, 19.4 / 28.2, 28.8 /
-// 28.3. Rows of one sequence share what two launches read: 64 rows of two sequences on 64 pages 9.8 / 14.9, 128 of one on 512 28.7 / 21.3.
+// of 128: 64 pages, 8 / 64 / 256 / 512 / 1,024 rows: 8.8 against 13.0, 9.7 / 13.8, 10.1 / 14.3, 16.4 / 15.5, 29.8 / 18.0; 256 pages, 8 / 64 / 256 /
+// 512 rows: 12.2 / 13.7, 13.3 / 15.0, 13.2 / 18.6, 24.7 / 24.8; 512 pages, 8 / 64 / 128 / 256 / 512 rows: 15.8 / 13.6, 16.1 / 15.7, 16.9 / 19.1, 19.0 /
+// 25.7, 34.0 / 35.7. Rows of one sequence share what two launches read: 64 rows of two sequences on 64 pages 9.7 / 13.5, 128 of one on 512 17.3 / 18.5.
 constexpr int64_t kPickRows = 256;
 
 // lanes that hold a head's values, 8 each: their number's logarithm
@@ -1000,16 +1030,15 @@ hipError_t launch_choose_pages(int type, int cache_type, const AttnArgs& a, cons
         return hipGetLastError();
       }
       if (c.pages > c.count) {  // (else every page is read)
-        const int64_t tiles = (a.max_q + slots - 1) / slots, waves = (int64_t)a.batch * a.cache.kv_heads * ((c.pages + 15) / 16);
-        const int64_t ranges = std::max<int64_t>(1, std::min(tiles, kScoreWaves / waves)), per = (tiles + ranges - 1) / ranges * slots;
-        const int64_t items = waves * ranges;
-        const dim3 grid((uint32_t)((items + 3) / 4));
+        const int64_t tiles = (a.max_q + slots - 1) / slots, groups = (int64_t)a.batch * a.cache.kv_heads * ((c.pages + 63) / 64);
+        const int64_t ranges = std::max<int64_t>(1, std::min(tiles, kScoreGroups / groups)), per = (tiles + ranges - 1) / ranges * slots;
+        const dim3 grid((uint32_t)(groups * ranges));
         if (a.dim <= 64)
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 64>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 64>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per);
         else if (a.dim <= 128)
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 128>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 128>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per);
         else
-          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per, items);
+          hipLaunchKernelGGL((k_page_scores<tq(), tc(), 256>), grid, dim3(256), 0, s, a, c, (int)t, rows_log2, (int)ranges, (int)per);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
       }
       if (c.pages <= 8 * 64)

@@ -142,7 +142,7 @@ int check_choose(const dq_kv_cache* c, const dq_sequences* s) {
   if (int rc = check_sequences(s, c->page_size); rc != DQ_OK) return rc;
   if (s->tokens < 0) return bad("tokens must be >= 0");
   if (s->tokens > 0 && s->max_len > 0 &&
-      (choose_tokens(c, s, true) == 0 || s->batch > 4 * kMaxGroups / (ceil_div(ceil_div(s->max_len, c->page_size), 16) * c->kv_heads)))
+      (choose_tokens(c, s, true) == 0 || s->batch > (kMaxGroups - 1) / (ceil_div(ceil_div(s->max_len, c->page_size), 64) * c->kv_heads)))
     return too_many("pages and heads");
   return DQ_OK;
 }
