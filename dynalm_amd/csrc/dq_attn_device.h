@@ -130,18 +130,24 @@ DQ_DEV bool nonfinite(u32 x) {
 
 DQ_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Eight values of q from value `at` on.
-template <int T>
-DQ_DEV void load8(const AttnArgs& a, int64_t at, v4u (&x)[T == DQ_F32 ? 2 : 1]) {
-  const char* p = static_cast<const char*>(a.q) + at * (T == DQ_F32 ? 4 : 2);
+// Eight values of q from each of the values `at` on, all under way together.
+template <int T, int N>
+DQ_DEV void load8s(const AttnArgs& a, const int64_t (&at)[N], v4u (&x)[N][T == DQ_F32 ? 2 : 1]) {
+  constexpr int kBytes = T == DQ_F32 ? 4 : 2;
   if (a.q_vec) {
 #pragma unroll
-    for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) x[k] = reinterpret_cast<const v4u*>(p)[k];
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int k = 0; k < (T == DQ_F32 ? 2 : 1); ++k) x[n][k] = reinterpret_cast<const v4u*>(static_cast<const char*>(a.q) + at[n] * kBytes)[k];
   } else {
 #pragma unroll
-    for (int i = 0; i < (T == DQ_F32 ? 8 : 4); ++i)
-      x[i / 4][i % 4] = T == DQ_F32 ? reinterpret_cast<const u32*>(p)[i]
-                                    : (u32)reinterpret_cast<const uint16_t*>(p)[2 * i] | (u32)reinterpret_cast<const uint16_t*>(p)[2 * i + 1] << 16;
+    for (int n = 0; n < N; ++n) {
+      const char* p = static_cast<const char*>(a.q) + at[n] * kBytes;
+#pragma unroll
+      for (int i = 0; i < (T == DQ_F32 ? 8 : 4); ++i)
+        x[n][i / 4][i % 4] = T == DQ_F32 ? reinterpret_cast<const u32*>(p)[i]
+                                         : (u32)reinterpret_cast<const uint16_t*>(p)[2 * i] | (u32)reinterpret_cast<const uint16_t*>(p)[2 * i + 1] << 16;
+    }
   }
 }
 

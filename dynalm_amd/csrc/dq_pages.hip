@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void k_page_bounds(AttnArgs a, const int32_t* 
 // pages are certain where their intervals say so; only those that meet at the border of the choice (two or three of 512), and those whose sums
 // are not finite, are summed again in 64 bits.
 //
-// 512 tokens of 32 heads on 512 pages of 4 kv heads of 128: scores 27 us, choice 15 (64-bit sums of all of them 479; as a library product in 64
+// 512 tokens of 32 heads on 512 pages of 4 kv heads of 128: scores 23 us, choice 14 (64-bit sums of all of them 479; as a library product in 64
 // bits at 70 TFLOP/s, twice over the channels, 61). 32 sequences of up to 512 pages, 8 kv heads (51 MB of bounds), in one launch 18.6 us, 2.7
 // TB/s: the reads take 11, then the choice of a row, some 7 us of dependent steps, which few waves hide.
 
@@ -344,7 +344,7 @@ DQ_DEV double lanes_sum(double x, int log2) {
 
 // The 64-bit scores of row t's query heads on `count` pages id_of(j), as whole numbers that order as they do: most[j] (in LDS, 0 before)
 // is the largest over the heads. A wave's work: every `step`th, from its `first` on, of the steps of a page and 64 / 2^log2
-// of its heads; N steps' loads are under way together.
+// of its heads; N steps' loads are under way together (one step's after the other's, a row with an open page waits 1 us longer).
 template <int T, int TC, int N = 4, class F>
 DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int count, F&& id_of, uint64_t* most, int first, int step, int log2,
                        int lane) {
@@ -355,20 +355,27 @@ DQ_DEV void exact_keys(const AttnArgs& a, const ChooseArgs& c, int t, int h, int
     v4u lo[N], hi[N], x[N][T == DQ_F32 ? 2 : 1];
     int page[N];
     bool bad[N];
+    int64_t at[N];
+    int p = i0 / turns, turn = i0 - p * turns;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int i = min(i0 + k, steps - 1);  // (past the steps: the last again)
-      page[k] = i / turns;
-      const int head = min((i - page[k] * turns) * at_once + (lane >> log2), a.group - 1);
-      const int id = id_of(page[k]);
+      page[k] = p;
+      const int head = min(turn * at_once + (lane >> log2), a.group - 1);
+      at[k] = (int64_t)t * a.q_token + (int64_t)(h * a.group + head) * a.q_head + (in ? d : 0);
+      const int id = id_of(p);
       bad[k] = (u32)id >= (u32)a.cache.n_pages;
       const uint16_t* near = c.bounds + ((int64_t)(bad[k] ? 0 : id) * a.cache.kv_heads + h) * 2 * a.dim + (in ? d : 0);
       lo[k] = *reinterpret_cast<const v4u*>(near);
       hi[k] = *reinterpret_cast<const v4u*>(near + a.dim);
-      load8<T>(a, (int64_t)t * a.q_token + (int64_t)(h * a.group + head) * a.q_head + (in ? d : 0), x[k]);
+      if (i0 + k + 1 < steps && ++turn == turns) {  // (past the steps: the last again)
+        turn = 0;
+        ++p;
+      }
     }
+    load8s<T>(a, at, x);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
+      if (k > 0 && i0 + k >= steps) break;
       double s[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
