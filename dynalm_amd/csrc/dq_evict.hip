@@ -21,8 +21,8 @@ DQ_DEV void seq_rows(const AttnArgs& a, int b, int& first, int& n) {
 // cores leaves a lane with one key's products with four rows, so that sums over rows stay in their lane until
 // the last. z is split in a float and a rest, whose power of two is the factor that a row's weights are added with.
 
-constexpr int kMassTiles = 4;                       // of 16 keys: a wave's
-constexpr int kMassKeys = 4 * 16 * kMassTiles;      // a workgroup's
+constexpr int kMassKeys = 256;  // a workgroup's
+constexpr int kMassTiles = 4;   // of 16 keys: a wave's, of four
 
 // z = lse log2 e as a float and the power of two of what that leaves out.
 DQ_DEV void split_lse(float lse, float& hi, float& f) {
@@ -36,13 +36,13 @@ DQ_DEV void split_lse(float lse, float& hi, float& f) {
 }
 
 // A wave's keys as B operands: lane n of a group has key n, 8 (lane / 16) .. + 7 of every 32 values.
-template <int DP>
-DQ_DEV void load_keys(const AttnArgs& a, int b, int head, int k0, int len, int n, int g, v4u (&k)[kMassTiles][DP / 32], bool (&bad)[kMassTiles]) {
+template <int DP, int M>
+DQ_DEV void load_keys(const AttnArgs& a, int b, int head, int k0, int len, int n, int g, v4u (&k)[M][DP / 32], bool (&bad)[M]) {
   const CacheArgs& ca = a.cache;
   const int32_t* list = a.pages + b * a.pages_stride;
   const u32 token_bytes = (u32)ca.token * 2;
 #pragma unroll
-  for (int i = 0; i < kMassTiles; ++i) {
+  for (int i = 0; i < M; ++i) {
     const int key = k0 + 16 * i, p = min(key, len - 1) / ca.page_size;
     int id = page_at(list, p);
     bad[i] = (u32)id >= (u32)ca.n_pages;
@@ -56,17 +56,18 @@ DQ_DEV void load_keys(const AttnArgs& a, int b, int head, int k0, int len, int n
 }
 
 // The sums over a wave's rows into the weights, or into the range's part.
-DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int part, int k0, int len, int old, int n, int g, float (&sum)[kMassTiles],
-                     const bool (&bad)[kMassTiles]) {
+template <int M>
+DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int part, int k0, int len, int old, int n, int g, float (&sum)[M],
+                     const bool (&bad)[M]) {
   const CacheArgs& ca = a.cache;
 #pragma unroll
-  for (int i = 0; i < kMassTiles; ++i) sum[i] = row_sum(sum[i]);
+  for (int i = 0; i < M; ++i) sum[i] = row_sum(sum[i]);
   // lane group i writes tile i
-  static_assert(kMassTiles == 4);
-  float x = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
-  if (g == 0 ? bad[0] : g == 1 ? bad[1] : g == 2 ? bad[2] : bad[3]) x = __builtin_nanf("");
+  static_assert(M == 2 || M == 4);
+  float x = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[M - 2] : sum[M - 1];
+  if (g == 0 ? bad[0] : g == 1 ? bad[1] : g == 2 ? bad[M - 2] : bad[M - 1]) x = __builtin_nanf("");
   const int key = k0 + 16 * g + n;
-  if (key >= len) return;
+  if (g >= M || key >= len) return;
   if (m.part != nullptr) {
     m.part[(((int64_t)part * a.batch + b) * ca.kv_heads + head) * a.max_len + key] = x;
     return;
@@ -162,10 +163,16 @@ struct MassLds {
   alignas(16) int token[kMassRows<T>];  // of a tile's row
 };
 
+// Waves of a workgroup, for heads over 128 values of 32 keys each, not 64, which with their products leave one wave a SIMD (the
+// prompt above in heads of 256: 241 us and 189, with fp32 rows 673 and 449; two workgroups a CU spill, 675).
+template <int DP>
+constexpr int kMassWaves = DP <= 128 ? 4 : 8;
+
 template <int T, int TC, int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 3 : 1, DP <= 128 ? 3 : 2))) void k_mass_many(AttnArgs a, MassArgs m, int key_tiles) {
+__global__ __launch_bounds__(kMassWaves<DP> * 64) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 3 : 2, DP <= 128 ? 3 : 4))) void k_mass_many(AttnArgs a, MassArgs m, int key_tiles) {
   constexpr int NP = kParts<T, TC>, QR = kMassRows<T>, kBytes = T == DQ_F32 ? 4 : 2;
-  constexpr int kChunks = DP / 8, kPasses = QR * kChunks / 256, kPassRows = 256 / kChunks;
+  constexpr int W = kMassWaves<DP>, M = kMassKeys / 16 / W;
+  constexpr int kChunks = DP / 8, kPasses = QR * kChunks / (64 * W), kPassRows = 64 * W / kChunks;
   __shared__ MassLds<T, TC, DP> sh;
   const CacheArgs& ca = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
   const int kt = item % key_tiles, b = item / key_tiles;  // (the first keys are seen by most rows)
   const int len = seq_len(a, b);
   if (kt * kMassKeys >= len) return;
-  const int k0 = kt * kMassKeys + wave * 16 * kMassTiles;
+  const int k0 = kt * kMassKeys + wave * 16 * M;
   int first, count;
   seq_rows(a, b, first, count);
   const int old = len - count;
@@ -268,15 +275,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
   };
 
   if (t_begin < t_end) read(t_begin);
-  v4u k[kMassTiles][DP / 32];
-  bool bad[kMassTiles];
+  v4u k[M][DP / 32];
+  bool bad[M];
   load_keys<DP>(a, b, head, k0, len, n, g, k, bad);
-  float sum[kMassTiles];
+  float sum[M];
 #pragma unroll
-  for (int i = 0; i < kMassTiles; ++i) sum[i] = 0;
+  for (int i = 0; i < M; ++i) sum[i] = 0;
   // (the keys have come: else the loop would wait for them, and with them for the next rows, in every tile)
 #pragma unroll
-  for (int i = 0; i < kMassTiles; ++i)
+  for (int i = 0; i < M; ++i)
 #pragma unroll
     for (int s = 0; s < DP / 32; ++s) asm volatile("" : "+v"(k[i][s]));
   if (t_begin < t_end) write(0);
@@ -286,38 +293,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
     const bool more = t0 + stride < t_end;
     if (more) read(t0 + stride);
     const int sees = old + t0 - first + 1;  // keys of the tile's first token
-    v4f acc[2][kMassTiles];
-    auto products = [&](int q0, v4f (&out)[kMassTiles]) {
+    v4f acc[2][M];
+    auto products = [&](int q0, v4f (&out)[M]) {
 #pragma unroll
-      for (int i = 0; i < kMassTiles; ++i) out[i] = v4f{0, 0, 0, 0};
+      for (int i = 0; i < M; ++i) out[i] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
         for (int s = 0; s < DP / 32; ++s) {
           const v4u q = *reinterpret_cast<const v4u*>(&sh.q[buf][p][place(q0 + n, 4 * s + g)]);
 #pragma unroll
-          for (int i = 0; i < kMassTiles; ++i) out[i] = mma<TC>(q, k[i][s], out[i]);
+          for (int i = 0; i < M; ++i) out[i] = mma<TC>(q, k[i][s], out[i]);
         }
     };
-    auto weights = [&](int q0, v4f (&x)[kMassTiles], auto masked) {
+    auto weights = [&](int q0, v4f (&x)[M], auto masked) {
       const v4f hi = *reinterpret_cast<const v4f*>(&sh.hi[buf][q0 + 4 * g]), f = *reinterpret_cast<const v4f*>(&sh.f[buf][q0 + 4 * g]);
       v4f c = {a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
       if constexpr (T == DQ_F32) c = *reinterpret_cast<const v4f*>(&sh.c[buf][q0 + 4 * g]);
       v4i token = {0, 0, 0, 0};
       if constexpr (masked()) token = *reinterpret_cast<const v4i*>(&sh.token[q0 + 4 * g]);
 #pragma unroll
-      for (int i = 0; i < kMassTiles; ++i)
+      for (int i = 0; i < M; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][e] = fmaf(x[i][e], c[e], -hi[e]);
 #pragma unroll
-      for (int i = 0; i < kMassTiles; ++i)
+      for (int i = 0; i < M; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][e] = exp2_fast(x[i][e]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int limit = token[e] < t_end - t0 ? sees + token[e] : 0;
 #pragma unroll
-        for (int i = 0; i < kMassTiles; ++i) {
+        for (int i = 0; i < M; ++i) {
           if constexpr (masked())
             sum[i] += k0 + 16 * i + n < limit ? x[i][e] * f[e] : 0.f;
           else
@@ -333,7 +340,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
         weights(16 * j, acc[j & 1], masked);
       }
     };
-    if (t0 + step <= t_end && k0 + 16 * kMassTiles <= sees)
+    if (t0 + step <= t_end && k0 + 16 * M <= sees)
       tile(std::false_type{});
     else if (k0 < sees + min(step, t_end - t0) - 1)  // (the last token sees the most)
       tile(std::true_type{});
@@ -650,11 +657,13 @@ __global__ __launch_bounds__(kThreads) void k_compact(AttnArgs a, CompactArgs c,
 
 // Rows of a sequence from which on its queries go through LDS: 8 sequences of 4,096 keys, 32 / 8 heads, us without and with: bf16 heads of
 // 128, 32 / 64 / 128 / 256 rows: 16.0 and 20.1, 19.8 and 20.6, 24.7 and 21.9, 34.0 and 27.0; fp32 rows, 32 / 64 / 128: 20.7 and 21.2, 28.2 and
-// 24.3, 40.1 and 29.8; heads of 64, 64 / 128 rows: 12.0 and 11.5, 15.9 and 13.3. Heads over 128 values leave it one wave a SIMD: 64 / 256 rows in
-// heads of 256, 35.3 and 47.6, 57.4 and 67.1; from many more rows on it is the same in 16 bits (2,048 tokens: 107 and 106) and pays in fp32 (256 and 217).
+// 24.3, 40.1 and 29.8; heads of 64, 64 / 128 rows: 12.0 and 11.5, 15.9 and 13.3. Heads of 256 (a workgroup of
+// eight waves), 64 / 128 / 256 / 512 rows: 34.7 and 36.3, 42.8 and 42.8, 57.1 and 50.2, 104 and 72; fp32 rows, 32 / 64 / 128 / 512: 45.2 and 38.9,
+// 61.5 and 47.5, 94 and 60, 276 and 151; heads of 192, 256 / 512 rows: 47.6 and 48.7, 84 and 71.
 template <int T>
 constexpr int kManyRows = T == DQ_F32 ? 64 : 128;
-constexpr int kManyRowsWide = 1024;
+template <int T>
+constexpr int kManyRowsWide = T == DQ_F32 ? 64 : 256;
 
 hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, const MassArgs& m, hipStream_t s) {
   const int tiles = (a.max_len + kMassKeys - 1) / kMassKeys;
@@ -663,10 +672,10 @@ hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, co
     // (a tile holds whole tokens, whose rows are addressed from its first in 32 bits)
     constexpr int kRows = kMassRows<tq()>;
     const bool near = a.q_token < (1 << 22) && a.q_head < (1 << 22);
-    const bool many = (int64_t)a.max_q * a.group >= (a.dim <= 128 ? kManyRows<tq()> : kManyRowsWide) && a.group <= kRows && near;
+    const bool many = (int64_t)a.max_q * a.group >= (a.dim <= 128 ? kManyRows<tq()> : kManyRowsWide<tq()>) && a.group <= kRows && near;
     const auto go = [&](auto dp) {
       if (many)
-        hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);
+        hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(64 * kMassWaves<dp()>), 0, s, a, m, tiles);
       else
         hipLaunchKernelGGL((k_mass<tq(), tc(), dp()>), grid, dim3(256), 0, s, a, m, tiles);
       return hipGetLastError();
