@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
   put_mass(a, m, b, head, part, k0, len, old, n, g, sum, bad);
 }
 
-// Many rows: the same with the rows' queries through LDS for the four waves together, two buffers deep. A tile is as many
+// Many rows: the same with the rows' queries through LDS for all of its waves together, two buffers deep. A tile is as many
 // whole tokens as kMassRows rows hold, so that a thread's rows lie at the same offsets from every tile's first token (rows that
 // are left have a weight of 0); a row's 16-byte chunks lie at their number XOR some bits of the row's, which spreads a
 // column of rows over the banks. The products of 16 rows stand beside the exponentials of the 16 before.
