@@ -679,7 +679,9 @@ hipError_t launch_attention_mass(int type, int cache_type, const AttnArgs& a, co
     // (a tile holds whole tokens, whose rows are addressed from its first in 32 bits)
     constexpr int kRows = kMassRows<tq()>;
     const bool near = a.q_token < (1 << 22) && a.q_head < (1 << 22);
-    const bool many = (int64_t)a.max_q * a.group >= (a.dim <= 128 ? kManyRows<tq()> : kManyRowsWide<tq()>) && a.group <= kRows && near;
+    // (a launch counts its threads in 32 bits, workgroups of 512 among them)
+    const bool fits = a.dim <= 128 || grid.x < (1u << 23);
+    const bool many = (int64_t)a.max_q * a.group >= (a.dim <= 128 ? kManyRows<tq()> : kManyRowsWide<tq()>) && a.group <= kRows && near && fits;
     const auto go = [&](auto dp) {
       if (many)
         hipLaunchKernelGGL((k_mass_many<tq(), tc(), dp()>), grid, dim3(64 * kMassWaves<dp()>), 0, s, a, m, tiles);

@@ -84,6 +84,24 @@ def test_choice(cuda, new, lens, hq, hk, dim, page, first, last, count, type, ca
     assert torch.equal(L.run_choose(c, bounds, first, last, count).cpu(), L.choose(c, bounds, first, last, count))
 
 
+MANY_CHOICES = [
+    # new, lens, q heads, kv heads, dim, page, first, last, count
+    pytest.param([150], [16 * 520 + 5], 40, 2, 24, 16, 1, 1, 40, id="20 heads a kv head, 521 pages"),
+    pytest.param([90, 0, 61], [16 * 640, 3, 61], 28, 14, 96, 16, 1, 2, 30, id="two heads a kv head, 640 pages"),
+    pytest.param([70, 40], [70, 1200], 100, 20, 136, 16, 0, 1, 5, id="five heads a kv head, heads of 136"),
+    pytest.param([33, 300, 9], [16 * 70, 300, 16 * 130 + 1], 9, 3, 64, 16, 2, 2, 11, id="ragged prompts"),
+]
+
+
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("new,lens,hq,hk,dim,page,first,last,count", MANY_CHOICES)
+def test_choice_of_many_rows(cuda, new, lens, hq, hk, dim, page, first, last, count, type, cache):
+    """Scores in a launch of their own: a workgroup's waves go through many rows together."""
+    c = Call(dim + count, new, lens, hq, hk, dim, type, cache, page, heads_first=dim == 96, odd=dim == 24, tail=dim % 5)
+    bounds = L.run_bounds(c)
+    assert torch.equal(L.run_choose(c, bounds, first, last, count).cpu(), L.choose(c, bounds, first, last, count))
+
+
 def test_choice_of_equal_scores(cuda):
     """Of equal pages the lower ones; a page of zeros ties with one of minus zeros."""
     c = Call(4, [1, 1], [40 * 16, 33 * 16], 4, 2, 64, "f32", "bf16", 16)
