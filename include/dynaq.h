@@ -611,8 +611,9 @@ DQ_API int dq_choose_pages(const dq_kv_cache* cache, const dq_sequences* s, cons
 /* dq_shared_attention's rows over the keys of chosen pages alone:
  *     out[t, h] = sum_j p_j v_j,  p = softmax over the visible j on a chosen page of scale * q[t, h] . k_j
  * chosen is dq_choose_pages' list, or any other of that form: tokens x kv_heads x count indices into a sequence's pages, in any
- * order; entries outside the pages that hold visible keys are left out, a page that is given twice counts twice. out must not overlap q. Types, rounding, lse, infinite and NaN
- * values, rows without keys and page numbers outside the cache (of a chosen page) are as there. Pages of up to 2^24 places.
+ * order; entries outside the pages that hold visible keys are left out, a page that is given twice counts twice. out must not overlap q. Types, lse, infinite and NaN
+ * values, rows without keys and page numbers outside the cache (of a chosen page) are as there; so is the rounding, but that the softmax
+ * weights of 16-bit rows are kept to 2^-16 (f16: 2^-22, down to 2^-30 of the largest) in the second product. Pages of up to 2^24 places.
  * workspace: dq_page_attention_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
 DQ_API int64_t dq_page_attention_workspace(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, int64_t count);
 DQ_API int dq_page_attention(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, const dq_heads* out,

@@ -292,6 +292,39 @@ def test_attention_infinite_values(cuda, type, cache, count):
 
 
 @pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lens,hq,hk,dim,page,count", [([1] * 3, [700, 333, 64], 8, 2, 128, 16, 12), ([1], [3000], 8, 2, 96, 16, 150),
+                                                           ([40, 2], [300, 700], 6, 2, 64, 32, 5), ([1] * 2, [600, 1], 17, 1, 256, 64, 8)])
+def test_attention_weights_of_16_bit_rows(cuda, new, lens, hq, hk, dim, page, count, type):
+    """The output is off by its own rounding and little else: the softmax weights are not rounded to 16 bits."""
+    c = Call(dim + 1, new, lens, hq, hk, dim, type, type, page)
+    chosen = L.some_pages(c, count)
+    out = L.run_attention(c, chosen.cuda())
+    c.type = "f32"  # (the bound without a rounding of weights)
+    want, _, bound, _ = L.page_attention(c, chosen)
+    values, c.vs = c.vs, [v.abs() for v in c.vs]
+    size = L.page_attention(c, chosen)[0]
+    # weights in two parts: 2^-16 of each for bf16; for f16 2^-22, and 2^-24 of weights whose largest is 2^6 or more
+    most = max(v.abs().max().item() for v in values if v.numel())
+    part = 2.0**-16 * size if type == "bf16" else 2.0**-22 * size + 2.0**-30 * count * page * most
+    B.close(out[: c.rows], want, bound + part, type)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_attention_an_infinite_value_keeps_its_sign(cuda, type):
+    """Of keys that have a weight, whatever its bits."""
+    c = Call(16, [1], [400], 4, 2, 64, type, type, 16)
+    c.q.mul_(0.1)
+    chosen = L.some_pages(c, 6)
+    p = int(chosen[0, 0, 2])
+    c.kc[int(c.table[0, p]), 2, 0] = 0.0  # (one score of 0 beside the others)
+    for j in range(4):
+        for x in (math.inf, -math.inf):
+            c.vc[int(c.table[0, p]), j, 0, 9 + j] = x
+            out = L.run_attention(c, chosen.cuda())
+            assert torch.all(out[0, :2, 9 + j] == x)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
 @pytest.mark.parametrize("count", [2, 80])
 def test_attention_scores_of_minus_infinity(cuda, type, count):
     """Rows whose every score is -inf get zeros whatever the values."""
