@@ -24,11 +24,12 @@ DQ_DEV void seq_rows(const AttnArgs& a, int b, int& first, int& n) {
 constexpr int kMassKeys = 256;  // a workgroup's
 constexpr int kMassTiles = 4;   // of 16 keys: a wave's, of four
 
-// z = lse log2 e as a float and the power of two of what that leaves out.
+// z = lse log2 e as a float and the power of two of what that leaves out, half a unit of its last place. Past 2^24 that is more than
+// 1, and no more than the scores' own rounding there: 1 of it is taken, so that the factor is never 0 or infinite beside a weight that is.
 DQ_DEV void split_lse(float lse, float& hi, float& f) {
   const double z = (double)lse * 1.4426950408889634074;
   hi = (float)z;
-  f = exp2_fast((float)((double)hi - z));
+  f = exp2_fast(__builtin_amdgcn_fmed3f((float)((double)hi - z), -1.f, 1.f));
   if (fabsf(hi) == INFINITY) {
     hi = fabsf(lse) == INFINITY ? INFINITY : copysignf(FLT_MAX, lse);  // (a row whose lse is -inf has no weights)
     f = 1.f;

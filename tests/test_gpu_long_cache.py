@@ -435,6 +435,29 @@ def test_mass_lse_of_any_value(cuda):
     assert torch.isnan(got[..., :58]).all() and torch.isfinite(got[..., 58:]).all()
 
 
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("new,lens", [([4], [60]), ([150], [300])])
+def test_mass_lse_of_large_size(cuda, new, lens, type, cache):
+    """A row whose lse is far above its scores adds 0 to each key that it sees, one whose lse is far below them infinity, whatever
+    lse's bits; by few rows and by many."""
+    c = Call(24, new, lens, 4, 2, 64, type, cache, 16)
+    start = own_lse(c)
+    large = [3e9, 5e9, 1e10, 1.1e10, 1e11, 1e15, 1.5e15, 1e30, 3e30, 7e33, 2e38]
+    for first in range(3):
+        lse = start.clone()
+        for i, t in enumerate(range(0, new[0], 3)):
+            lse[t, (t + first) % 4] = large[(i + 4 * first) % len(large)]
+        got = L.run_mass(c, lse, torch.zeros((1, 2, lens[0]), device="cuda"), 0.0)
+        want, bound = L.mass(c, lse, torch.zeros((1, 2, lens[0])), 0.0)
+        B.close(got, want, bound, "f32")
+    for x in large:
+        lse = start.clone()
+        lse[1, 0] = -x
+        got = L.run_mass(c, lse, torch.zeros((1, 2, lens[0]), device="cuda"), 0.0)
+        sees = c.row(1)[1]
+        assert torch.all(got[0, 0, :sees] == math.inf) and torch.isfinite(got[0, 0, sees:]).all() and torch.isfinite(got[0, 1]).all()
+
+
 def test_mass_of_infinite_and_hidden_keys(cuda):
     """A NaN key's weight is NaN, no other's; places past the keys hold NaN and are not read into any."""
     c = Call(23, [2, 1], [50, 33], 2, 1, 64, "bf16", "bf16", 16)
