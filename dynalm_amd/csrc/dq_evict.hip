@@ -77,9 +77,50 @@ DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int 
   *out = m.decay != 0 && key < old ? fmaf(m.decay, *out, x) : x;
 }
 
+// Adds the weights of 16 of a sequence's rows (of a kv head: row r is query head r % group of token first + r / group),
+// r0 .. up to r_end, on the wave's keys. A row's weight on a key that it does not see is left out, whatever its product.
+template <int T, int TC, int DP, int M>
+DQ_DEV void add_rows(const AttnArgs& a, const MassArgs& m, int head, int first, int old, int r0, int r_end, int k0, int n, int g,
+                     const v4u (&k)[M][DP / 32], float (&sum)[M]) {
+  constexpr int NP = kParts<T, TC>;
+  const int r = min(r0 + n, r_end - 1), token = first + r / a.group, qh = head * a.group + r % a.group;
+  const bool valid = r0 + n < r_end;
+  RawQ<T, DP> raw;
+  load_q<T, DP>(a, valid, token, qh, g, raw);
+  const float lse = m.lse[(int64_t)token * a.heads + qh];
+  v4u q[NP][DP / 32];
+  const float c = q_operands<T, TC, DP>(a, raw, q);
+  float hi, f;
+  split_lse(lse, hi, f);
+  const int limit = valid ? old + (token - first) + 1 : 0;
+  // of the four rows whose products the lane holds
+  float c4[4], hi4[4], f4[4];
+  int limit4[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c4[i] = T == DQ_F32 ? __shfl(c, 4 * g + i, 64) : c;
+    hi4[i] = __shfl(hi, 4 * g + i, 64);
+    f4[i] = __shfl(f, 4 * g + i, 64);
+    limit4[i] = __shfl(limit, 4 * g + i, 64);
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    v4f acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+      for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(q[p][s], k[i][s], acc);
+    const int key = k0 + 16 * i + n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float w = exp2_fast(fmaf(acc[e], c4[e], -hi4[e])) * f4[e];
+      sum[i] += key < limit4[e] ? w : 0.f;
+    }
+  }
+}
+
 template <int T, int TC, int DP>
 __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_tiles) {
-  constexpr int NP = kParts<T, TC>;
   const CacheArgs& ca = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -103,45 +144,10 @@ __global__ __launch_bounds__(256) void k_mass(AttnArgs a, MassArgs m, int key_ti
 #pragma unroll
   for (int i = 0; i < kMassTiles; ++i) sum[i] = 0;
   // rows before the first that sees key k0 add nothing; of the others every splits-th 16 are this part's
-  const int rows = count * a.group, r_end = rows;
+  const int rows = count * a.group;
   const int64_t sees_from = max((int64_t)0, (int64_t)(k0 - old) * a.group);
-  for (int64_t at = sees_from + 16 * part; at < r_end; at += 16 * m.splits) {
-    const int r0 = (int)at;
-    const int r = min(r0 + n, rows - 1), token = first + r / a.group, qh = head * a.group + r % a.group;
-    const bool valid = r0 + n < r_end;
-    RawQ<T, DP> raw;
-    load_q<T, DP>(a, valid, token, qh, g, raw);
-    const float lse = m.lse[(int64_t)token * a.heads + qh];
-    v4u q[NP][DP / 32];
-    const float c = q_operands<T, TC, DP>(a, raw, q);
-    float hi, f;
-    split_lse(lse, hi, f);
-    const int limit = valid ? old + (token - first) + 1 : 0;
-    // of the four rows whose products the lane holds
-    float c4[4], hi4[4], f4[4];
-    int limit4[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c4[i] = T == DQ_F32 ? __shfl(c, 4 * g + i, 64) : c;
-      hi4[i] = __shfl(hi, 4 * g + i, 64);
-      f4[i] = __shfl(f, 4 * g + i, 64);
-      limit4[i] = __shfl(limit, 4 * g + i, 64);
-    }
-#pragma unroll
-    for (int i = 0; i < kMassTiles; ++i) {
-      v4f acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-        for (int s = 0; s < DP / 32; ++s) acc = mma<TC>(q[p][s], k[i][s], acc);
-      const int key = k0 + 16 * i + n;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = exp2_fast(fmaf(acc[e], c4[e], -hi4[e])) * f4[e];
-        sum[i] += key < limit4[e] ? w : 0.f;
-      }
-    }
-  }
+  for (int64_t at = sees_from + 16 * part; at < rows; at += 16 * m.splits)
+    add_rows<T, TC, DP>(a, m, head, first, old, (int)at, rows, k0, n, g, k, sum);
   put_mass(a, m, b, head, part, k0, len, old, n, g, sum, bad);
 }
 
@@ -347,6 +353,20 @@ __global__ __launch_bounds__(kMassWaves<DP> * 64) __attribute__((amdgpu_waves_pe
       tile(std::true_type{});
     if (more) write(buf ^ 1);
     __syncthreads();
+  }
+  // Rows that are left add 0 to the sums of finite keys, and NaN to others': a wave whose sums are NaN makes them once more without such rows.
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < M; ++i) odd |= sum[i] != sum[i];
+  if (__builtin_expect(__any(odd), false)) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) sum[i] = 0;
+#pragma unroll 1
+    for (int t0 = t_begin; t0 < t_end; t0 += stride) {
+      const int r_end = (min(step, t_end - t0) + t0 - first) * a.group;
+#pragma unroll 1
+      for (int r0 = (t0 - first) * a.group; r0 < r_end; r0 += 16) add_rows<T, TC, DP>(a, m, head, first, old, r0, r_end, k0, n, g, k, sum);
+    }
   }
   put_mass(a, m, b, head, part, k0, len, old, n, g, sum, bad);
 }

@@ -627,7 +627,7 @@ DQ_API int dq_page_attention(const dq_kv_cache* cache, const dq_sequences* s, co
  * whose lse is NaN makes the mass of the keys that it sees NaN.
  * mass[b][g][j] is at mass + b * seq_stride + g * head_stride + j; from lens[b] on it is left as it is. Sums are fp32
  * and do not depend on timing. q: fp32 or the cache's type; the cache's v is not read and may be NULL. A key on a page number
- * outside the cache gets NaN. 0 <= decay <= 1.
+ * outside the cache gets NaN; with fp32 q, whose products are summed in parts, so may a key with an infinite value. 0 <= decay <= 1.
  * workspace: dq_attention_mass_workspace bytes (16-byte aligned), or DQ_ATTENTION_WORKSPACE_BYTES, enough for any call. */
 DQ_API int64_t dq_attention_mass_workspace(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q);
 DQ_API int dq_attention_mass(const dq_kv_cache* cache, const dq_sequences* s, const dq_heads* q, const float* lse,

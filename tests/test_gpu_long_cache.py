@@ -458,6 +458,27 @@ def test_mass_lse_of_large_size(cuda, new, lens, type, cache):
         assert torch.all(got[0, 0, :sees] == math.inf) and torch.isfinite(got[0, 0, sees:]).all() and torch.isfinite(got[0, 1]).all()
 
 
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("group,dim,new,lens", [(3, 64, 150, 300), (5, 256, 70, 200), (7, 128, 60, 400), (22, 96, 20, 90), (4, 128, 100, 300), (3, 64, 5, 60)])
+def test_mass_of_infinite_keys(cuda, group, dim, new, lens, type, cache):
+    """A key on which every row scores -inf gathers 0, by few rows and by many, whatever the number of heads a kv head; the others what
+    they gather beside it. (With fp32 rows, whose products are summed in parts, that key's may be NaN.)"""
+    c = Call(25, [new], [lens], 2 * group, 2, dim, type, cache, 16)
+    c.q[..., 5] = c.q[..., 5].abs() + 0.5
+    for j, h in ((20, 0), (33, 1)):
+        c.ks[0][j, h, 5] = -math.inf
+        c.kc[int(c.table[0, j // 16]), j % 16, h, 5] = -math.inf
+    lse = own_lse(c)
+    got = L.run_mass(c, lse, torch.zeros((1, 2, lens), device="cuda"), 0.0)
+    want, bound = L.mass(c, lse, torch.zeros((1, 2, lens)), 0.0)
+    bound = torch.nan_to_num(bound, 0.0, 0.0, 0.0)  # (of the two keys: exactly 0)
+    for j, h in ((20, 0), (33, 1)):
+        assert want[0, h, j] == 0
+        if type == "f32" and torch.isnan(got[0, h, j]):
+            got[0, h, j] = 0.0
+    B.close(got, want, bound, "f32")
+
+
 def test_mass_of_infinite_and_hidden_keys(cuda):
     """A NaN key's weight is NaN, no other's; places past the keys hold NaN and are not read into any."""
     c = Call(23, [2, 1], [50, 33], 2, 1, 64, "bf16", "bf16", 16)
