@@ -31,7 +31,7 @@ DQ_DEV void split_lse(float lse, float& hi, float& f) {
   hi = (float)z;
   f = exp2_fast(__builtin_amdgcn_fmed3f((float)((double)hi - z), -1.f, 1.f));
   if (fabsf(hi) == INFINITY) {
-    hi = fabsf(lse) == INFINITY ? INFINITY : copysignf(FLT_MAX, lse);  // (a row whose lse is -inf has no weights)
+    hi = fabsf(lse) == INFINITY ? INFINITY : copysignf(FLT_MAX, lse);  // (-inf too: such a row has no weights)
     f = 1.f;
   }
 }
@@ -78,7 +78,8 @@ DQ_DEV void put_mass(const AttnArgs& a, const MassArgs& m, int b, int head, int 
 }
 
 // Adds the weights of 16 of a sequence's rows (of a kv head: row r is query head r % group of token first + r / group),
-// r0 .. up to r_end, on the wave's keys. A row's weight on a key that it does not see is left out, whatever its product.
+// r0 .. up to r_end, on the wave's keys. A row's weight on a key that it does not see is left out, whatever its product; all of
+// a row whose lse is -inf are.
 template <int T, int TC, int DP, int M>
 DQ_DEV void add_rows(const AttnArgs& a, const MassArgs& m, int head, int first, int old, int r0, int r_end, int k0, int n, int g,
                      const v4u (&k)[M][DP / 32], float (&sum)[M]) {
@@ -92,7 +93,7 @@ DQ_DEV void add_rows(const AttnArgs& a, const MassArgs& m, int head, int first, 
   const float c = q_operands<T, TC, DP>(a, raw, q);
   float hi, f;
   split_lse(lse, hi, f);
-  const int limit = valid ? old + (token - first) + 1 : 0;
+  const int limit = valid && lse != -INFINITY ? old + (token - first) + 1 : 0;
   // of the four rows whose products the lane holds
   float c4[4], hi4[4], f4[4];
   int limit4[4];
@@ -354,7 +355,8 @@ __global__ __launch_bounds__(kMassWaves<DP> * 64) __attribute__((amdgpu_waves_pe
     if (more) write(buf ^ 1);
     __syncthreads();
   }
-  // Rows that are left add 0 to the sums of finite keys, and NaN to others': a wave whose sums are NaN makes them once more without such rows.
+  // Rows that are left, and those whose lse is -inf, add 0 where their products are finite, and NaN elsewhere: a wave whose sums are NaN
+  // makes them once more without such rows.
   bool odd = false;
 #pragma unroll
   for (int i = 0; i < M; ++i) odd |= sum[i] != sum[i];

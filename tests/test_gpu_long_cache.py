@@ -479,6 +479,35 @@ def test_mass_of_infinite_keys(cuda, group, dim, new, lens, type, cache):
     B.close(got, want, bound, "f32")
 
 
+@pytest.mark.parametrize("type,cache", KINDS)
+@pytest.mark.parametrize("new,lens", [(5, 60), (150, 300)])
+def test_mass_of_rows_without_weights(cuda, new, lens, type, cache):
+    """A row whose lse is -inf adds nothing, whatever it scores: infinite and NaN keys and queries among them."""
+    c = Call(26, [new], [lens], 4, 2, 64, type, cache, 16)
+    dead = torch.zeros((c.tokens, 4), dtype=torch.bool)
+    dead[torch.arange(1, new, 3), torch.arange(1, new, 3) % 4] = True
+    dead[2] = True
+    # the live rows score -inf on one key, the others +inf; one of the others is NaN itself
+    c.q[..., 5] = torch.where(dead.cuda(), -1.0, 1.0) * (c.q[..., 5].abs() + 0.5)
+    c.ks[0][20, 0, 5] = -math.inf
+    c.kc[int(c.table[0, 1]), 4, 0, 5] = -math.inf
+    lse = own_lse(c)
+    lse[dead.cuda()] = -math.inf
+    c.q[2, 3, 7] = math.nan
+    c.q[2, 1, 9] = math.inf
+    got = L.run_mass(c, lse, torch.zeros((1, 2, lens), device="cuda"), 0.0)
+    want, bound = L.mass(c, lse, torch.zeros((1, 2, lens)), 0.0)
+    bound = torch.nan_to_num(bound, 0.0, 0.0, 0.0)
+    assert want[0, 0, 20] == 0 and torch.isfinite(want).all()
+    if type == "f32" and torch.isnan(got[0, 0, 20]):
+        got[0, 0, 20] = 0.0
+    B.close(got, want, bound, "f32")
+    # all of them
+    lse.fill_(-math.inf)
+    c.kc[int(c.table[0, 0]), 3, 1] = math.nan
+    assert torch.all(L.run_mass(c, lse, torch.ones((1, 2, lens), device="cuda"), 0.0) == 0)
+
+
 def test_mass_of_infinite_and_hidden_keys(cuda):
     """A NaN key's weight is NaN, no other's; places past the keys hold NaN and are not read into any."""
     c = Call(23, [2, 1], [50, 33], 2, 1, 64, "bf16", "bf16", 16)
