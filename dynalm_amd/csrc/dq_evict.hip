@@ -604,7 +604,7 @@ __global__ __launch_bounds__(kThreads, kInPlace ? 1 : 6) void k_compact(AttnArgs
   const int job = item % jobs, b = item / jobs;
   const int len = seq_len(a, b);
   const int32_t* kept = c.kept + ((int64_t)b * ca.kv_heads + h) * c.budget;
-  const int most = (int)min(c.budget, (int64_t)len);  // (entries behind are none of kv_keep's)
+  const int most = (int)min(c.budget, (int64_t)(kInPlace ? len : a.max_len));  // (in place a list ascends: it has no more)
   if (c.mass != nullptr && job == jobs - 1) {
     const int64_t at = b * c.seq + h * c.head;
     move_weights<kThreads>(kept, most, len, c.mass + at, c.mass_out + at);

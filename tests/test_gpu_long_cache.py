@@ -622,6 +622,36 @@ def test_compact_lists_of_any_values_stay_inside(cuda):
         L.same(got[others.cuda()], x[others.cuda()])
 
 
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,hk,dim,budget", [([9, 0, 40], 2, 64, 40), ([300, 100], 1, 80, 5000), ([700, 3000], 2, 24, 2900)])
+def test_compact_lists_with_gaps(cuda, cache, lens, hk, dim, budget):
+    """Into pages of their own: places in any order, some twice, some left out, lists longer than the sequence; weights beside them."""
+    page = 16
+    c = Call(33, [1] * len(lens), lens, hk, hk, dim, "f32", cache, page)
+    most, gen = min(budget, c.most), torch.Generator().manual_seed(7)
+    each = -(-most // page)
+    kept = torch.full((len(lens), hk, budget), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        kept[b] = torch.randint(-(n // 3) - 1, n + n // 3 + 1, (hk, budget), generator=gen).to(torch.int32)
+    first = c.kc.shape[0]
+    c.kc, c.vc = (torch.cat((p, torch.full((each * len(lens), *p.shape[1:]), 44.0, dtype=p.dtype, device="cuda"))) for p in (c.kc, c.vc))
+    to = (first + torch.randperm(each * len(lens), generator=gen)).to(torch.int32).view(len(lens), each)
+    w = torch.rand((len(lens), hk, c.most), generator=gen).cuda()
+    out = torch.full_like(w, 33.0)
+    want, want_w = [p.cpu().clone() for p in (c.kc, c.vc)], out.cpu().clone()
+    for b, n in enumerate(lens):
+        for h in range(hk):
+            place = kept[b, h, :most].long()
+            i = torch.arange(most)[(place >= 0) & (place < n)]
+            for pool, own in zip(want, (c.ks, c.vs)):
+                pool[to[b, i // page].long(), i % page, h] = own[b][place[i], h]
+            want_w[b, h, i] = w[b, h].cpu()[place[i]]
+    dq.kv_compact(c.c(), c.seqs(), kept.cuda(), budget, to.cuda(), each, w, out, *w.stride()[:2], stream())
+    for got, x in zip((c.kc, c.vc), want):
+        L.same(got, x)
+    assert torch.equal(out.cpu(), want_w)
+
+
 def test_compact_weights_alone_in_place(cuda):
     """Keys into pages of their own, weights in place: a long list moves as a whole."""
     c = Call(32, [1], [9000], 1, 1, 8, "f32", "f16", 16)
