@@ -643,10 +643,11 @@ DQ_API int dq_kv_keep(const dq_sequences* s, int64_t kv_heads, const float* mass
                       int64_t first, int64_t last, int64_t budget, int32_t* kept, int32_t* kept_lens, void* stream);
 
 /* Moves the keys and values of places kept[b][g][i] of sequence b to places i, in each kv head by itself, of the pages
- * to_pages[b * to_stride], ... (NULL: of the sequence's own, in place; then kept must ascend, as dq_kv_keep's does), for i <
- * min(budget, max_len). Entries
+ * to_pages[b * to_stride], ... (NULL: of the sequence's own, in place), for i < min(budget, max_len). Entries
  * outside [0, lens[b]) and pages outside the cache are left out. With mass and mass_out (both or neither), mass_out[b][g][i] is
- * mass[b][g][kept[b][g][i]] too, at the same strides; mass_out may be mass, and must not overlap it otherwise. Pages that are written to must be of one sequence and
+ * mass[b][g][kept[b][g][i]] too, at the same strides; mass_out may be mass, and must not overlap it otherwise. Where keys or masses are moved
+ * in place, kept must ascend with no entry left out before its last place, as dq_kv_keep's does; else its places may come in any
+ * order, and more than once. Pages that are written to must be of one sequence and
  * (to_pages) be read by none. Keys have been rotated to their positions when they were appended: those that stay keep them. */
 DQ_API int dq_kv_compact(const dq_kv_cache* cache, const dq_sequences* s, const int32_t* kept, int64_t budget,
                          const int32_t* to_pages, int64_t to_stride, const float* mass, float* mass_out, int64_t seq_stride,
