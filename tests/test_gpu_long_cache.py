@@ -544,6 +544,26 @@ def test_keep(cuda, lens, heads, first, last, budget, kind):
     assert kept_lens.tolist() == [min(n, budget) for n in lens]
 
 
+@pytest.mark.parametrize("lens,heads,first,last,budget", [([8193, 16384, 12000], 2, 4, 128, 4096), ([4097, 8192], 1, 0, 3, 4), ([16385], 1, 3, 0, 16384),
+                                                          ([65536, 16500], 1, 1, 1, 5000), ([65537], 1, 0, 0, 65536)])
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd", "near"])
+def test_keep_of_every_length(cuda, lens, heads, first, last, budget, kind):
+    """Around the lengths at which a lane holds more places, up to those that are read again."""
+    gen = torch.Generator().manual_seed(budget)
+    w = torch.exp(2 * torch.randn((len(lens), heads, max(lens) + 5), generator=gen))
+    if kind == "ties":
+        w = torch.randint(0, 3, w.shape, generator=gen).float()
+    if kind == "odd":
+        odd = torch.tensor([math.nan, math.inf, -math.inf, -0.0, 0.0, -1.0, 1e-42, math.nan])
+        w = torch.where(torch.rand(w.shape, generator=gen) < 0.8, odd[torch.randint(0, 8, w.shape, generator=gen)], w)
+    if kind == "near":  # (neighbours among the floats: every pass over the bins counts)
+        w = (torch.randint(0, 1 << 16, w.shape, generator=gen, dtype=torch.int32) + 0x3F000000).view(torch.float32)
+        w[..., 0], w[..., 1] = 1e30, 1e-30
+    kept, kept_lens = L.run_keep(lens, w.cuda(), first, last, budget)
+    assert torch.equal(kept.cpu(), L.keep(w, lens, first, last, budget))
+    assert kept_lens.tolist() == [min(n, budget) for n in lens]
+
+
 def test_keep_lengths_beyond_the_bounds_are_cut(cuda):
     w = torch.rand((3, 1, 40), device="cuda")
     lens = torch.tensor([1 << 30, -5, 40], dtype=torch.int32, device="cuda")
@@ -620,6 +640,32 @@ def test_compact_lists_of_any_values_stay_inside(cuda):
     others[mine.cpu()] = False
     for got, x in zip((c.kc, c.vc), before):
         L.same(got[others.cuda()], x[others.cuda()])
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,page,heads_first,weights_in_place", [(64, 16, False, True), (80, 48, True, False), (256, 64, True, True), (8, 16, False, None)])
+def test_compact_many_sequences_in_place(cuda, cache, dim, page, heads_first, weights_in_place):
+    """A serving batch: 32 sequences of 4 heads, some of which keep more than a list's part of 2,048 places."""
+    hk, budget = 4, 2500
+    lens = [5000, 2501, 0, 2100, 1, 4097] + [17 + 31 * i for i in range(26)]
+    c = Call(34, [1] * 32, lens, hk, hk, dim, "f32", cache, page, heads_first=heads_first)
+    kept = lists(c, budget)
+    w = torch.rand((32, hk, c.most), generator=torch.Generator().manual_seed(3)).cuda()
+    out = None if weights_in_place is None else w if weights_in_place else torch.full_like(w, 33.0)
+    want, table = [p.cpu().clone() for p in (c.kc, c.vc)], c.table.cpu().long()
+    want_w = None if out is None else out.cpu().clone()
+    for b in range(32):
+        for h in range(hk):
+            mine = kept[b, h][kept[b, h] >= 0].long()
+            i = torch.arange(len(mine))
+            for pool, own in zip(want, (c.ks, c.vs)):
+                pool[table[b, i // page], i % page, h] = own[b][mine, h]
+            if out is not None:
+                want_w[b, h, : len(mine)] = w[b, h].cpu()[mine]
+    dq.kv_compact(c.c(), c.seqs(), kept.cuda(), budget, None, 0, None if out is None else w, out, *w.stride()[:2], stream())
+    for got, x in zip((c.kc, c.vc), want):
+        L.same(got, x)
+    assert out is None or torch.equal(out.cpu(), want_w)
 
 
 @pytest.mark.parametrize("cache", ["f16", "bf16"])
