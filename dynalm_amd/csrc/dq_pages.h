@@ -16,7 +16,7 @@ hipError_t launch_page_bounds(int cache_type, const AttnArgs& a, const int32_t* 
 struct ChooseArgs {
   const uint16_t* bounds = nullptr;
   int32_t* chosen = nullptr;
-  uint64_t* keys = nullptr;  // scores in an order of whole numbers: [token of the launch][kv head][page]
+  uint64_t* keys = nullptr;  // [token of the launch][kv head][page]: the interval of a score (two floats), or the 64-bit score in an order of whole numbers
   int32_t pages = 0;         // of a sequence, at most
   int32_t first = 0, last = 0;
   int64_t count = 0;

@@ -171,11 +171,10 @@ DQ_DEV void magnitudes(const PageTile<DP>& p, v4u (&most)[DP / 32]) {
     }
 }
 
-// The intervals of the lane's page with rows 4 g .. + 3 of 16 query rows, where they pass low and high. next() is called once
-// the rows are no longer needed.
-template <int T, int TC, int DP, class F>
+// The intervals of the lane's page with rows 4 g .. + 3 of 16 query rows, where they pass low and high.
+template <int T, int TC, int DP>
 DQ_DEV void tile_scores(const RawQ<T, DP>& raw, const PageTile<DP>& page, const v4u (&most)[DP / 32], float error, int g, float (&low)[4],
-                        float (&high)[4], F&& next) {
+                        float (&high)[4]) {
   constexpr int NS = DP / 32, NP = kScoreParts<T>;
   int e2 = 0;
   if constexpr (T == DQ_F32 && TC == DQ_F16) {  // scaled to a largest value in [2^14, 2^15)
@@ -218,7 +217,6 @@ DQ_DEV void tile_scores(const RawQ<T, DP>& raw, const PageTile<DP>& page, const 
     }
     size = mma<TC>(mag, most[s], size);
   }
-  next();
   const v4f sum = NP == 1 ? sums[0] : sums[0] + sums[NP - 1];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -309,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void k_page_scores(AttnArgs a, ChooseArgs c
         RawQ<T, DP> raw;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) raw.x[i / K][i % K] = sh[at][i][lane];
-        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, []() {});
+        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high);
       }
       at ^= 1;
       if (t1 < last) share(at);  // (read a tile ago, before the last barrier)
@@ -690,7 +688,7 @@ __global__ __launch_bounds__(DP <= 128 ? 1024 : 512) void k_page_pick(AttnArgs a
       for (int i = 0; i < 4; ++i) low[i] = high[i] = -INFINITY;
       for (int block = 0; block < blocks; ++block) {
         if (blocks > 1) load_q<T, DP>(a, true, t, h * a.group + min(16 * block + n, a.group - 1), g, raw);
-        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high, []() {});
+        tile_scores<T, TC, DP>(raw, page, most, error, g, low, high);
       }
       token_max(low, 16);
       token_max(high, 16);
