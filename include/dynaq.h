@@ -562,8 +562,9 @@ DQ_API int dq_shared_attention(const dq_kv_cache* cache, const dq_attention* a, 
  * Beside dense attention over the pages of a cache: a decode step that reads the pages on
  * which its queries may score high, and nothing else (dq_page_bounds after an append,
  * dq_choose_pages, dq_page_attention); and a cache that keeps the keys which attention has
- * weighed most (dq_attention_mass after an attention that wrote lse, dq_kv_keep and
- * dq_kv_compact now and then; dq_page_bounds again). What is said of the attention block's
+ * weighed most (dq_attention_mass after a dense attention that wrote lse, dq_kv_keep and
+ * dq_kv_compact now and then; dq_page_bounds again). A step that reads few pages has no lse over
+ * all keys, so it does not feed the second. What is said of the attention block's
  * calls holds for these: the current device, the given stream, no memory of the library's;
  * lengths, offsets, page numbers, chosen pages and kept places are device memory, and
  * whatever they hold, no access leaves the buffers that the arguments describe. */
@@ -589,8 +590,8 @@ typedef struct dq_sequences {
  * (n_pages x kv_heads x 2 x head_dim values of the cache's type, 16-byte aligned), for the pages that hold one
  * of sequence b's keys from[b], from[b] + 1, ..., lens[b] - 1 (at most max_new of them; from NULL: all keys, max_new
  * is not read); bounds take all of such a page's keys below lens[b]. Other pages' are left as they are. A NaN
- * among the values makes both NaN. Of the zeros -0 is the smaller. A page that several sequences list gets the bounds of one of
- * them. The rows of `s` (tokens, q_offsets, max_q) are not read. */
+ * among the values makes both NaN. Of the zeros -0 is the smaller. Each bound of a page that several sequences list is
+ * that of one of them (the same, where all of its keys are below their lengths). The rows of `s` (tokens, q_offsets, max_q) are not read. */
 DQ_API int dq_page_bounds(const dq_kv_cache* cache, const dq_sequences* s, const int32_t* from, int64_t max_new,
                           void* bounds, void* stream);
 
@@ -623,7 +624,8 @@ DQ_API int dq_page_attention(const dq_kv_cache* cache, const dq_sequences* s, co
 /* The attention weight that each key gathers in each kv head, over the rows and the query heads of the kv head:
  *     mass[b][g][j] = decay * mass[b][g][j] + sum of exp(scale * q[t, h] . k_j - lse[t, h]) over b's rows t that see j
  * for j < lens[b]; the keys of the rows themselves (the last n) have no earlier mass, and with decay 0 no key has: then
- * mass is not read. lse: tokens x q heads floats, as dq_shared_attention writes it; a row whose lse is -inf adds nothing, one
+ * mass is not read. lse: tokens x q heads floats, over all keys that the row sees, as dq_shared_attention writes it (dq_page_attention's
+ * is over the chosen pages' keys: with it a key of another page may gather more than 1); a row whose lse is -inf adds nothing, one
  * whose lse is NaN makes the mass of the keys that it sees NaN.
  * mass[b][g][j] is at mass + b * seq_stride + g * head_stride + j; from lens[b] on it is left as it is. Sums are fp32
  * and do not depend on timing. q: fp32 or the cache's type; the cache's v is not read and may be NULL. A key on a page number
