@@ -721,9 +721,10 @@ __global__ __launch_bounds__(DP <= 128 ? 1024 : 512) void k_page_pick(AttnArgs a
 // lane, 16 keys a row of lanes, so they turn in LDS, a wave's own part of it (16 bytes of a key at a place turned by the key's number: no two of
 // a read meet in a bank). The next tile's keys are under way from when this one's are in LDS.
 //
-// 32 sequences of 4,096 chosen keys, 32 / 8 bf16 heads of 128 (537 MB): 92 to 107 us, 5.0 to 5.8 TB/s (a part of them from the cache behind the L2s).
-// 473 rows of 1,024 chosen keys each, two sequences of up to 8,192: 81 us; 2 GB come from the L2s (93% hits), 24 TB/s. Keys loaded in S^T's order,
-// whose neighbouring lanes read 16 lines: 137 us; turned, not asked for early 86; rows of sums not turned in LDS 84.
+// 32 sequences of 4,096 chosen keys, 32 / 8 bf16 heads of 128 (537 MB): 92 to 112 us with the pages' place in memory, 4.8 to 5.8 TB/s (a part of
+// them from the cache behind the L2s).
+// 473 rows of 1,024 chosen keys each, two sequences of up to 8,192: 86 us; 2 GB come from the L2s (93% hits), 23 TB/s. With one-part weights 81: then keys
+// loaded in S^T's order, whose neighbouring lanes read 16 lines, took 137 us; turned, not asked for early 86; rows of sums not turned in LDS 84.
 
 template <int DP>
 struct PageLds {
@@ -1009,6 +1010,9 @@ constexpr int64_t kScoreGroups = 1024;
 // of 128: 64 pages, 8 / 64 / 256 / 512 / 1,024 rows: 8.8 against 13.0, 9.7 / 13.8, 10.1 / 14.3, 16.4 / 15.5, 29.8 / 18.0; 256 pages, 8 / 64 / 256 /
 // 512 rows: 12.2 / 13.7, 13.3 / 15.0, 13.2 / 18.6, 24.7 / 24.8; 512 pages, 8 / 64 / 128 / 256 / 512 rows: 15.8 / 13.6, 16.1 / 15.7, 16.9 / 19.1, 19.0 /
 // 25.7, 34.0 / 35.7. Rows of one sequence share what two launches read: 64 rows of two sequences on 64 pages 9.7 / 13.5, 128 of one on 512 17.3 / 18.5.
+// The one limit for all numbers of pages costs 2 us at 512 rows of 512 pages. kPickPages ends the rule, and with it the choice by one wave: 8 intervals
+// a lane. Beyond, a row takes 16 waves, and 8 / 64 / 256 / 512 rows of 512, 513, 683 and 1,024 pages take 13 / 15 / 19 / 36, 22 / 24 / 33 / 58, 21 / 25 /
+// 37 / 65 and 21 / 27 / 43 / 77 us: a step of 8 to 22 us at 513 pages.
 constexpr int64_t kPickRows = 256;
 
 // lanes that hold a head's values, 8 each: their number's logarithm
