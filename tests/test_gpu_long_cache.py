@@ -845,6 +845,49 @@ def test_the_calls_in_a_graph(cuda):
         assert_same(*got)
 
 
+@pytest.mark.parametrize("type,cache", KINDS)
+def test_prompts_in_a_graph(cuda, type, cache):
+    """The calls over many rows captured once, replayed with other queries, an infinite key and rows without weights among them."""
+    c = Call(56, [150, 40], [700, 333], 6, 2, 128, type, cache, 16)
+    bounds = torch.zeros((c.kc.shape[0], 2, 2, 128), dtype=c.kc.dtype, device="cuda")
+    chosen = torch.empty((c.tokens, 2, 12), dtype=torch.int32, device="cuda")
+    out, dense = torch.empty_like(c.q), torch.empty_like(c.q)
+    lse, page_lse = (torch.empty((c.tokens, 6), device="cuda") for _ in range(2))
+    mass = torch.zeros((2, 2, 700), device="cuda")
+    work = torch.empty(dq.ATTENTION_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    dead = torch.zeros((c.tokens, 6), dtype=torch.bool, device="cuda")
+    dead[::7, 1] = True
+
+    def run():
+        kv, s, q = c.c(), c.seqs(), B.heads(c.q)
+        dq.page_bounds(kv, s, None, 0, bounds, stream())
+        dq.choose_pages(kv, s, q, bounds, 1, 2, 12, chosen, work, work.numel(), stream())
+        dq.page_attention(kv, s, q, B.heads(out), page_lse, chosen, 12, c.scale, work, work.numel(), stream())
+        dq.shared_attention(kv, q, B.heads(dense), lse, c.tokens, 2, c.offsets_d, c.max_q, None, 0, c.table, c.table.stride(0), c.lens_d, c.most,
+                            c.scale, work, work.numel(), stream())
+        lse.masked_fill_(dead, -math.inf)
+        dq.attention_mass(kv, s, q, lse, c.scale, 0.5, mass, 1400, 700, work, work.numel(), stream())
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(4):
+        c.q.normal_()
+        if i == 2:  # (every row scores -inf on it)
+            c.q[..., 3] = c.q[..., 3].abs() + 0.5
+            c.kc[int(c.table[0, 2]), 1, 0, 3] = -math.inf
+        got = []
+        for go in (run, graph.replay):
+            mass.fill_(0.25)
+            torch.cuda.synchronize()
+            go()
+            torch.cuda.synchronize()
+            got.append([x.clone() for x in (bounds, chosen, out, page_lse, mass)])
+        assert_same(*got)
+
+
 def test_calls_run_on_their_stream(cuda):
     """On a stream of their own, behind work that it waits for; another cycle on another stream at the same time."""
     plain = Cycle(53, "bf16", "bf16")
